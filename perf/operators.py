@@ -207,6 +207,7 @@ def prepare(case, seed):
         s["caches"] = torch.empty(shape, dtype=_DTYPES[c["cache"]], device="cuda")
         for layer in s["caches"]:
             layer.copy_(_randn(g, *shape[1:]).clamp(-_E4M3_MAX, _E4M3_MAX))
+        s["layers"] = list(s["caches"].unbind(0))     # a model keeps one cache per layer
         order = torch.randperm(c["pages"], generator=g, device="cuda").to(torch.int32)
         s["src"], s["dst"] = order[:c["pairs"]].contiguous(), order[c["pairs"]:2 * c["pairs"]].contiguous()
     else:
@@ -330,7 +331,7 @@ def _own(s):
                                     s["ks"], s["vs"], interleaved=c["interleaved"], attention_factor=s["factor"])
         return [q, s["kc"], s["vc"]]
     if c["op"] == "copy":
-        ops.zentorch_cache_copy_pages(s["caches"].unbind(0), s["src"], s["dst"])
+        ops.zentorch_cache_copy_pages(s["layers"], s["src"], s["dst"])
         return [s["caches"]]
     return ops.zentorch_paged_attention(s["q"], s["kc"], s["vc"], s["cu"], s["lens"], s["table"], s["max_q"],
                                         causal=c["causal"], window=c["window"], k_scale=s["ks"], v_scale=s["vs"])
