@@ -31,7 +31,8 @@ typedef enum {
   ZT_DEVICE_TIMEOUT = 5 /* a bounded device-side wait expired; the context stays usable */
 } zt_status_t;
 
-typedef enum { ZT_BF16 = 0, ZT_F32 = 1, ZT_U8 = 2, ZT_S8 = 3 } zt_dtype_t; /* 8-bit types: static qlinear only */
+typedef enum { ZT_BF16 = 0, ZT_F32 = 1, ZT_U8 = 2, ZT_S8 = 3, ZT_F16 = 4, ZT_E4M3 = 5 } zt_dtype_t;
+/* U8 / S8: static qlinear only; F16 and E4M3 (8-bit float, no infinities): rotary positions, paged cache and attention only */
 
 /* Post-op ids; same values as UNARY_POST_OP / BINARY_POST_OP in src/cpu/cpp/Utils.hpp:56-72. */
 typedef enum {
@@ -91,7 +92,8 @@ ZT_API const char *zt_version(void);
  * is_avx512_supported, src/cpu/cpp/Utils.hpp:28-35). */
 ZT_API int zt_device_supported(void);
 /* Reads the device-side status word that a kernel sets when one of its bounded waits expires
- * (0 = none; 101..104 name the waiting role of a linear, 105 a peer that did not show up in zt_allreduce_bf16).  Synchronises with the device; `reset` clears it.
+ * (0 = none; 101..104 name the waiting role of a linear, 105 a peer that did not show up in zt_allreduce_bf16), or when an
+ * index in device memory points outside its tensor (106: a page, slot or length of the paged cache; the access is skipped).  Synchronises with the device; `reset` clears it.
  * No counterpart in the reference (its failures are host exceptions, src/cpu/cpp/Utils.hpp:21-23). */
 ZT_API int zt_poll_device_status(int *status, int reset);
 /* Exercises that path without a fault: launches a one-thread kernel whose wait on a barrier nobody
@@ -376,6 +378,121 @@ typedef struct {
 
 ZT_API size_t zt_allreduce_symmetric_bytes(size_t max_bytes);
 ZT_API int zt_allreduce_bf16(const zt_allreduce_args_t *args, void *stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Rotary positions of queries and keys, optionally storing the rotated keys and the values in a paged cache.  The reference
+ * leaves these to its host framework (no counterpart in its tree); they are what stands between a decoder layer's qkv projection
+ * and its attention.
+ *
+ *   angle_i = position * inv_freq[i],  i < rot_dim / 2        (formed and reduced in 64 bits)
+ *   (a, b) -> (a cos - b sin, b cos + a sin) * attention_factor
+ *
+ * The pairs of a head are (x[i], x[i + rot_dim/2]), or (x[2i], x[2i+1]) with `interleaved`; elements from rot_dim on pass through
+ * unchanged.  Stretched frequencies for long contexts are the caller's inv_freq and attention_factor.
+ *
+ * q, k, v    [tokens, heads, head_dim] of dtype (ZT_BF16, ZT_F16, ZT_F32), strides {token, head} in elements, unit inner stride
+ * positions  [tokens] int32, or int64 with positions_64; |position| < 2^31
+ * q_out      as q; may be q itself.   k_out  as k, written only without a cache; may be k itself
+ * caches     NULL, or [num_pages, page_size, kv_heads, head_dim] with strides {page, slot, head}, of dtype or ZT_E4M3.  Token t's
+ *            key and value go to row slots[t] = page * page_size + offset (int32, or int64 with slots_64).  A negative slot
+ *            stores nothing (padding); one past the cache stores nothing and sets the device status word (106).  The slots of a
+ *            call must differ from one another: of two tokens with one slot either may remain, element by element.
+ * scales     ZT_E4M3 only: [kv_heads] fp32 each; what is stored is x / scale, rounded to nearest even and saturated */
+typedef struct {
+  const void *q, *k, *v;
+  int64_t tokens;
+  int32_t q_heads, kv_heads, head_dim, rot_dim;
+  int32_t dtype;
+  int64_t q_stride[2], k_stride[2], v_stride[2];
+  const void *positions;
+  int32_t positions_64;
+  const float *inv_freq; /* [rot_dim / 2] */
+  float attention_factor;
+  int32_t interleaved;
+  void *q_out, *k_out;
+  int64_t q_out_stride[2], k_out_stride[2];
+  void *k_cache, *v_cache;
+  int32_t cache_dtype;
+  int64_t k_cache_stride[3], v_cache_stride[3];
+  int64_t num_pages;
+  int32_t page_size;
+  const void *slots;
+  int32_t slots_64;
+  const float *k_scale, *v_scale;
+} zt_rope_args_t;
+
+ZT_API int zt_rope(const zt_rope_args_t *args, void *stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Copies pages within paged caches: cache[dst[i]] = cache[src[i]] for every pair i, in all `n_caches` caches (the layers of a
+ * model) by one launch per 64 of them.  Forks copy the page that two sequences go on to write; compaction moves pages to the front.
+ *
+ * caches, page_stride_bytes, page_bytes  host arrays of n_caches: first page, page to page, bytes of a page (contiguous)
+ * src, dst  [n_pairs] int32 in device memory, or int64 with index_64.  A pair with a negative index is skipped (padding); one past
+ *           num_pages is skipped and sets the device status word (106).  The pairs are copied in no particular order: the
+ *           destinations must differ from one another and from every source. */
+typedef struct {
+  int32_t n_caches;
+  void *const *caches;
+  const int64_t *page_stride_bytes, *page_bytes;
+  int32_t num_pages;
+  int64_t n_pairs;
+  const void *src, *dst;
+  int32_t index_64;
+} zt_cache_copy_args_t;
+
+ZT_API int zt_cache_copy_pages(const zt_cache_copy_args_t *args, void *stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Attention of the new tokens of a batch of sequences over a paged cache that holds their keys and values already.
+ *
+ *   new token i (of n) of a sequence with `len` keys is at position p = len - n + i and sees the keys j of [0, len) with
+ *   j <= p (causal) and j > p - window (window > 0);  out = sum_j softmax_j(scale * q . k_j) v_j, zeros where it sees none
+ *
+ * Single tokens (decode), chunks of a prompt over a context, and whole prompts are one call, mixed in any way.  Lengths stay on
+ * the device: a captured call follows them.
+ *
+ * q, out       [tokens, q_heads, head_dim] ZT_BF16 / ZT_F16, strides {token, head} in elements; 16-byte aligned rows.  Query head
+ *              h reads kv head h / (q_heads / kv_heads).
+ * caches       [num_pages, page_size, kv_heads, head_dim], strides {page, slot, head} in elements, of q's type, or ZT_E4M3 with
+ *              k_scale / v_scale [kv_heads] fp32 that its values are multiplied by; 16-byte aligned rows.  Slots past a
+ *              sequence's length are not read, whatever they hold.
+ * head_dim     a multiple of 8 (16 for ZT_E4M3) up to 128
+ * cu_seqlens_q [batch + 1] int32: the new tokens of sequence b are rows [cu[b], cu[b+1]); ascending
+ * seq_lens     [batch] int32: keys of a sequence, its new tokens' among them
+ * block_table  [batch, max_blocks] int32, row stride in elements: the pages of a sequence in order
+ * max_query_len  the most new tokens of a sequence, 0 if unknown: chooses the kernel, results do not depend on it being exact
+ * zero_tail    rows of out behind cu[batch] are zeroed; otherwise they are left as they were
+ * workspace    zt_paged_attention_workspace_bytes() bytes, 256-byte aligned, contents irrelevant; calls that can overlap need one each
+ * Lengths that do not fit the tensors are cut, page ids outside the cache read as zeros; both set the device status word (106). */
+typedef struct {
+  const void *q;
+  void *out;
+  int64_t tokens;
+  int32_t batch, q_heads, kv_heads, head_dim;
+  int32_t dtype;
+  int64_t q_stride[2], out_stride[2];
+  const void *k_cache, *v_cache;
+  int32_t cache_dtype;
+  int64_t k_cache_stride[3], v_cache_stride[3];
+  int64_t num_pages;
+  int32_t page_size;
+  const int32_t *cu_seqlens_q, *seq_lens, *block_table;
+  int64_t block_table_stride;
+  int32_t max_blocks;
+  int32_t max_query_len;
+  float scale;
+  int32_t causal;
+  int32_t window; /* 0: none */
+  const float *k_scale, *v_scale;
+  int32_t zero_tail;
+  void *workspace;
+  size_t workspace_bytes;
+  int32_t algo; /* zt_algo_t: ZT_ALGO_AUTO, ZT_ALGO_SKINNY (streaming kernel), ZT_ALGO_TCGEN05 */
+} zt_paged_attention_args_t;
+
+ZT_API size_t zt_paged_attention_workspace_bytes(const zt_paged_attention_args_t *args);
+ZT_API int zt_paged_attention(const zt_paged_attention_args_t *args, void *stream);
 
 #ifdef __cplusplus
 }

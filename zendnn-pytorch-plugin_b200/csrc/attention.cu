@@ -1,0 +1,173 @@
+// Entry points of the paged attention: argument checks, the choice of the kernel, and the kernel that joins items which were
+// cut between CTAs.
+#include <cmath>
+
+#include "attention.cuh"
+
+namespace zt {
+
+namespace {
+
+constexpr int kMaxBatch = 16384;   // the division of a batch keeps one int per sequence in shared memory
+constexpr int kCombineWarps = 4;   // rows per block
+
+// Joins the pieces of the item that is cut at the end of CTA blockIdx.x's range: one warp per row, each lane DP / 32 columns.
+// Bound by memory; the pieces are mostly still in L2.
+template <typename T, int DP>
+__global__ void __launch_bounds__(kCombineWarps * 32) attention_combine_kernel(const __grid_constant__ AttnParams p, int R) {
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const int4 item = p.meta[blockIdx.x];
+  if (item.x < 0) return;
+  const SeqInfo seq = load_seq(p, item.x);
+  const int64_t r0 = (int64_t)item.y * R, rows = (int64_t)seq.n * p.group;
+  const int row = blockIdx.y * kCombineWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (row >= R || r0 + row >= rows) return;
+  const int first = blockIdx.x, count = item.w - first + 1;
+  auto slot = [&](int i) { return (int64_t)(2 * (first + i) + (i == 0 ? 1 : 0)) * R + row; };
+  float top = -INFINITY;
+  for (int i = lane; i < count; i += 32) top = fmaxf(top, p.part_ml[slot(i)].x);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  constexpr int V = DP / 32;
+  float acc[V] = {}, sum = 0.f;
+  for (int base = 0; base < count; base += 32) {
+    float f = 0.f, l = 0.f;
+    if (base + lane < count) {
+      const float2 ml = p.part_ml[slot(base + lane)];
+      f = ml.x == -INFINITY ? 0.f : exp2_fast(ml.x - top);
+      l = ml.y * f;
+    }
+    const int n = min(32, count - base);
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) {
+      const float fi = __shfl_sync(0xffffffffu, f, i);
+      sum += __shfl_sync(0xffffffffu, l, i);
+      const float *src = p.part_o + slot(base + i) * DP + lane * V;
+      if constexpr (V == 4) {
+        const float4 x = *reinterpret_cast<const float4 *>(src);
+        acc[0] = fmaf(fi, x.x, acc[0]), acc[1] = fmaf(fi, x.y, acc[1]), acc[2] = fmaf(fi, x.z, acc[2]), acc[3] = fmaf(fi, x.w, acc[3]);
+      } else {
+        const float2 x = *reinterpret_cast<const float2 *>(src);
+        acc[0] = fmaf(fi, x.x, acc[0]), acc[1] = fmaf(fi, x.y, acc[1]);
+      }
+    }
+  }
+  if (lane * V >= p.d) return;
+  const float f = top == -INFINITY ? 0.f : 1.f / sum;
+  const int tok = (int)((r0 + row) / p.group), qh = item.z * p.group + (int)((r0 + row) % p.group);
+  char *dst = reinterpret_cast<char *>(p.out) + ((seq.q0 + tok) * p.o_st + qh * p.o_sh + lane * V) * 2;
+  if constexpr (V == 4)
+    *reinterpret_cast<uint2 *>(dst) = make_uint2(pack2(acc[0] * f, acc[1] * f, T(0.f)), pack2(acc[2] * f, acc[3] * f, T(0.f)));
+  else
+    *reinterpret_cast<uint32_t *>(dst) = pack2(acc[0] * f, acc[1] * f, T(0.f));
+}
+
+size_t align256(size_t v) { return (v + 255) / 256 * 256; }
+
+AttnPlan make_plan(const zt_paged_attention_args_t &a) {
+  AttnPlan plan{};
+  const int group = a.kv_heads > 0 ? a.q_heads / a.kv_heads : 1;
+  // rows that the longest piece of new tokens gives a kv head
+  const int64_t bound = a.tokens - a.batch + 1 > 1 ? a.tokens - a.batch + 1 : 1;
+  const int64_t longest = a.max_query_len > 0 && a.max_query_len < bound ? a.max_query_len : bound;
+  const int64_t rows = longest * group;
+  plan.tcgen05 = false;
+  plan.dp = a.head_dim <= 64 ? 64 : 128;
+  plan.rows = rows <= 16 ? 16 : 32;
+  plan.grid = attention_stream_grid();
+  plan.meta_bytes = align256((size_t)plan.grid * sizeof(int4));
+  plan.ml_bytes = align256((size_t)2 * plan.grid * plan.rows * sizeof(float2));
+  plan.o_bytes = align256((size_t)2 * plan.grid * plan.rows * plan.dp * sizeof(float));
+  return plan;
+}
+
+bool aligned(const void *ptr, const int64_t *strides, int n, int elem_bytes) {
+  int64_t s = (int64_t)(reinterpret_cast<uintptr_t>(ptr) % 16);
+  for (int i = 0; i < n; ++i) s |= strides[i] * elem_bytes;
+  return s % 16 == 0;
+}
+
+}  // namespace
+}  // namespace zt
+
+using namespace zt;
+
+extern "C" size_t zt_paged_attention_workspace_bytes(const zt_paged_attention_args_t *a) {
+  if (!a || a->tokens <= 0 || a->q_heads <= 0 || a->kv_heads <= 0) return 256;
+  return make_plan(*a).total();
+}
+
+extern "C" int zt_paged_attention(const zt_paged_attention_args_t *a, void *stream) {
+  ZT_REQUIRE(a != nullptr, ZT_INVALID_ARGUMENT, "zt_paged_attention: null argument block");
+  ZT_REQUIRE(a->tokens >= 0 && a->batch >= 0 && a->max_blocks >= 0 && a->num_pages >= 0 && a->max_query_len >= 0, ZT_INVALID_ARGUMENT,
+             "zt_paged_attention: negative size");
+  ZT_REQUIRE(a->tokens <= (1 << 30) && a->num_pages <= (1 << 30), ZT_UNSUPPORTED, "zt_paged_attention: more than 2^30 tokens or pages");
+  ZT_REQUIRE(a->batch <= kMaxBatch, ZT_UNSUPPORTED, "zt_paged_attention: %d sequences, at most %d", a->batch, kMaxBatch);
+  ZT_REQUIRE(a->q_heads >= 1 && a->kv_heads >= 1 && a->q_heads % a->kv_heads == 0 && a->q_heads <= 4096, ZT_INVALID_ARGUMENT,
+             "zt_paged_attention: the query heads (%d) must be a multiple of the key/value heads (%d)", a->q_heads, a->kv_heads);
+  ZT_REQUIRE(a->dtype == ZT_BF16 || a->dtype == ZT_F16, ZT_INVALID_ARGUMENT, "zt_paged_attention: query must be bfloat16 or float16");
+  ZT_REQUIRE(a->cache_dtype == a->dtype || a->cache_dtype == ZT_E4M3, ZT_INVALID_ARGUMENT,
+             "zt_paged_attention: the cache must have the type of the query or be float8_e4m3");
+  const bool e4m3 = a->cache_dtype == ZT_E4M3;
+  ZT_REQUIRE(a->head_dim >= 8 && a->head_dim <= 128 && a->head_dim % (e4m3 ? 16 : 8) == 0, ZT_UNSUPPORTED,
+             "zt_paged_attention: head_dim must be a multiple of %d up to 128, got %d", e4m3 ? 16 : 8, a->head_dim);
+  ZT_REQUIRE(a->page_size >= 1, ZT_INVALID_ARGUMENT, "zt_paged_attention: the page size must be positive");
+  ZT_REQUIRE((int64_t)a->page_size * a->max_blocks <= (1 << 30), ZT_UNSUPPORTED,
+             "zt_paged_attention: block_table holds more than 2^30 keys per sequence");
+  ZT_REQUIRE(a->window >= 0, ZT_INVALID_ARGUMENT, "zt_paged_attention: the window must not be negative");
+  ZT_REQUIRE(std::isfinite(a->scale) && a->scale > 0.f, ZT_INVALID_ARGUMENT, "zt_paged_attention: the scale must be positive and finite");
+  ZT_REQUIRE(!e4m3 || (a->k_scale && a->v_scale), ZT_INVALID_ARGUMENT,
+             "zt_paged_attention: a float8_e4m3 cache needs k_scale and v_scale");
+  ZT_REQUIRE(a->algo == ZT_ALGO_AUTO || a->algo == ZT_ALGO_SKINNY || a->algo == ZT_ALGO_TCGEN05, ZT_INVALID_ARGUMENT,
+             "zt_paged_attention: unknown algo %d", a->algo);
+  if (a->tokens == 0) return ZT_SUCCESS;
+  ZT_REQUIRE(a->q && a->out && a->cu_seqlens_q, ZT_INVALID_ARGUMENT, "zt_paged_attention: null tensor pointer");
+  ZT_REQUIRE(a->batch == 0 || (a->seq_lens && (a->max_blocks == 0 || a->block_table)), ZT_INVALID_ARGUMENT,
+             "zt_paged_attention: null tensor pointer");
+  ZT_REQUIRE(a->num_pages == 0 || (a->k_cache && a->v_cache), ZT_INVALID_ARGUMENT, "zt_paged_attention: null cache pointer");
+  const int es = e4m3 ? 1 : 2;
+  ZT_REQUIRE(aligned(a->q, a->q_stride, 2, 2) && aligned(a->out, a->out_stride, 2, 2), ZT_INVALID_ARGUMENT,
+             "zt_paged_attention: rows of query and output must be 16-byte aligned");
+  ZT_REQUIRE(a->num_pages == 0 || (aligned(a->k_cache, a->k_cache_stride, 3, es) && aligned(a->v_cache, a->v_cache_stride, 3, es)),
+             ZT_INVALID_ARGUMENT, "zt_paged_attention: rows of the caches must be 16-byte aligned");
+  const AttnPlan plan = make_plan(*a);
+  ZT_REQUIRE(a->workspace && a->workspace_bytes >= plan.total(), ZT_WORKSPACE_TOO_SMALL,
+             "zt_paged_attention: workspace of %zu bytes is smaller than the %zu required", a->workspace_bytes, plan.total());
+  ZT_REQUIRE((reinterpret_cast<uintptr_t>(a->workspace) & 255) == 0, ZT_INVALID_ARGUMENT,
+             "zt_paged_attention: workspace must be 256-byte aligned");
+  int *status = device_status_ptr();
+  ZT_REQUIRE(status != nullptr, ZT_CUDA_ERROR, "zt_paged_attention: no device status word");
+
+  AttnParams p{};
+  p.q = a->q, p.out = a->out, p.k = a->k_cache, p.v = a->v_cache;
+  p.q_st = a->q_stride[0], p.q_sh = a->q_stride[1], p.o_st = a->out_stride[0], p.o_sh = a->out_stride[1];
+  p.k_sp = a->k_cache_stride[0], p.k_ss = a->k_cache_stride[1], p.k_sh = a->k_cache_stride[2];
+  p.v_sp = a->v_cache_stride[0], p.v_ss = a->v_cache_stride[1], p.v_sh = a->v_cache_stride[2];
+  p.cu = a->cu_seqlens_q, p.lens = a->seq_lens, p.table = a->block_table, p.table_stride = a->block_table_stride;
+  p.k_scale = e4m3 ? a->k_scale : nullptr, p.v_scale = e4m3 ? a->v_scale : nullptr;
+  p.batch = a->batch, p.tokens = (int)a->tokens, p.hq = a->q_heads, p.hkv = a->kv_heads, p.group = a->q_heads / a->kv_heads;
+  p.d = a->head_dim, p.page = a->page_size, p.max_blocks = a->max_blocks, p.num_pages = (int)a->num_pages;
+  p.page_shift = -1;
+  for (int s = 0; s < 31; ++s)
+    if (a->page_size == 1 << s) p.page_shift = s;
+  p.causal = a->causal != 0, p.window = a->window, p.scale_log2 = a->scale * 1.4426950408889634f, p.zero_tail = a->zero_tail != 0;
+  char *ws = reinterpret_cast<char *>(a->workspace);
+  p.meta = reinterpret_cast<int4 *>(ws);
+  p.part_ml = reinterpret_cast<float2 *>(ws + plan.meta_bytes);
+  p.part_o = reinterpret_cast<float *>(ws + plan.meta_bytes + plan.ml_bytes);
+  p.status = status;
+
+  cudaStream_t st = (cudaStream_t)stream;
+  const int rc = attention_stream_launch(p, plan, a->dtype, a->cache_dtype, st);
+  if (rc != ZT_SUCCESS) return rc;
+  const dim3 grid((unsigned)plan.grid, (unsigned)ceil_div(plan.rows, kCombineWarps)), block(kCombineWarps * 32);
+  const bool bf16 = a->dtype == ZT_BF16;
+  if (plan.dp == 64)
+    ZT_CUDA_OK(bf16 ? launch_overlapped(attention_combine_kernel<__nv_bfloat16, 64>, grid, block, (size_t)0, st, p, plan.rows)
+                    : launch_overlapped(attention_combine_kernel<__half, 64>, grid, block, (size_t)0, st, p, plan.rows));
+  else
+    ZT_CUDA_OK(bf16 ? launch_overlapped(attention_combine_kernel<__nv_bfloat16, 128>, grid, block, (size_t)0, st, p, plan.rows)
+                    : launch_overlapped(attention_combine_kernel<__half, 128>, grid, block, (size_t)0, st, p, plan.rows));
+  return launch_status("attention_combine_kernel");
+}

@@ -1,0 +1,448 @@
+// Paged attention for few rows per kv head (decode, short chunks) and for every shape that has no other kernel: K and V stream
+// from HBM once, with a running maximum and sum.
+//
+// A CTA of four warps takes units of 64 keys of an item; each warp streams its own 16 keys of every unit through a private ring
+// in shared memory (16-byte asynchronous copies, whose zero fill also blanks slots past the visible keys, so stale contents of a
+// page never meet the arithmetic) and keeps its own maxima, sums and output rows in registers: no barrier between warps until
+// the item ends, where the four are added through shared memory.  Two CTAs share an SM, so that one streams while the other is
+// in such an end.  Rows are the 16-row (or twice 16) operand of mma.sync.m16n8k16, keys its columns; the accumulator layout of
+// the scores is the operand layout of the probabilities.  e4m3 keys and values become halves in registers, which is exact; the
+// products then run in fp16 with query rows brought to a maximum below 2 by a power of two (what that takes from an element is
+// below 2^-25 of its row's largest).  Probabilities are rounded to the type of the product (half a step of 2^-8 or 2^-11 of
+// each, added by the tensor cores in fp32); the sum that divides them is of the unrounded fp32 values.
+#include "attention.cuh"
+
+namespace zt {
+
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int kKeys = 16;                  // of a warp per unit
+constexpr int kUnit = kWarps * kKeys;
+constexpr int kCtasPerSm = 2;
+
+template <int DP, bool E4M3>
+__host__ __device__ constexpr int stage_bytes() { return 2 * kKeys * DP * (E4M3 ? 1 : 2); }
+template <bool E4M3>
+__host__ __device__ constexpr int stages() { return E4M3 ? 6 : 3; }
+template <int DP, bool E4M3>
+__host__ __device__ constexpr int ring_bytes() { return kWarps * stages<E4M3>() * stage_bytes<DP, E4M3>(); }
+template <int R, int DP>
+__host__ __device__ constexpr int merge_bytes() { return kWarps * R * (DP + 8) * 4 + kWarps * R * 8; }
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, int bytes) {   // the rest of the 16 is zero
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __nv_bfloat16) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __half) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+template <typename T, bool E4M3>
+struct MmaType {
+  using type = T;
+};
+template <typename T>
+struct MmaType<T, true> {
+  using type = __half;
+};
+
+__device__ __forceinline__ float2 unpack2(uint32_t w, __nv_bfloat16) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+__device__ __forceinline__ float2 unpack2(uint32_t w, __half) { return __half22float2(*reinterpret_cast<const __half2 *>(&w)); }
+
+template <typename T, bool E4M3, int DP, int MT>
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_stream_kernel(const __grid_constant__ AttnParams p) {
+  using M = typename MmaType<T, E4M3>::type;
+  constexpr int R = 16 * MT, S = stages<E4M3>(), SB = stage_bytes<DP, E4M3>();
+  constexpr int ES = E4M3 ? 1 : 2;
+  constexpr int CH = DP * ES / 16;            // 16-byte chunks of a key's row
+  constexpr int KS = DP / 16;                 // 16-element steps of the score product
+  constexpr int NT = DP / 8;                  // 8-column tiles of the output
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ long long s_scan[40];
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const int lane = threadIdx.x & 31, warp = tc::uniform_warp();
+  const int g = lane >> 2, t4 = lane & 3;
+  AttnRange range = attention_range<R, kUnit, kThreads>(p, 1, reinterpret_cast<int *>(smem), s_scan);
+  zero_tail_rows<T>(p, kThreads);
+  unsigned char *ring = smem + warp * S * SB;
+  const uint32_t ring_addr = smem_u32(ring);
+  float *merge_o = reinterpret_cast<float *>(smem);                                   // [warp][R][DP + 8]
+  float2 *merge_ml = reinterpret_cast<float2 *>(smem + kWarps * R * (DP + 8) * 4);    // [warp][R]
+  if (threadIdx.x == 0) p.meta[blockIdx.x] = make_int4(-1, 0, 0, 0);
+
+  long long w = range.w0;
+  int b = range.b, tile = range.tile;
+  long long item0 = range.item0;
+  SeqInfo seq = range.w0 < range.w1 ? load_seq(p, b) : SeqInfo{0, 0, 0};
+  while (w < range.w1) {
+    // ---- the next piece of an item in this CTA's range --------------------------------------------------
+    while (tile >= row_tiles<R>(p, seq)) seq = load_seq(p, ++b), tile = 0;   // (sequences without new tokens have no tiles)
+    const TileUnits units = tile_units<R, kUnit>(p, seq, tile);
+    const int head = (int)((w - item0) / units.count);
+    const long long h0 = item0 + (long long)head * units.count, h1 = h0 + units.count;   // the item's units
+    const long long w_end = h1 < range.w1 ? h1 : range.w1;
+    const int n_units = (int)(w_end - w), unit0 = units.first + (int)(w - h0);
+    const int64_t rows = (int64_t)seq.n * p.group, r0 = (int64_t)tile * R;
+    const int n_rows = (int)(rows - r0 < R ? rows - r0 : R);
+    const int tok0 = (int)(r0 / p.group), tok1 = (int)((r0 + n_rows - 1) / p.group);
+    // keys that some row sees, within this piece
+    const int k_begin = max(key_lo(p, seq, tok0), unit0 * kUnit);
+    const int k_end = min((long long)key_hi(p, seq, tok1), ((long long)unit0 + n_units) * kUnit);
+
+    // ---- query rows as operand fragments ------------------------------------------------------------------
+    uint32_t qf[MT][KS][4];
+    int lo[MT][2], hi[MT][2];
+    float mul[MT][2];
+    const float head_scale = p.scale_log2 * (E4M3 ? fabsf(p.k_scale[head]) : 1.f);
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int row = m * 16 + half * 8 + g;
+        const bool live = row < n_rows;
+        const int tok = live ? (int)((r0 + row) / p.group) : tok0;
+        const int qh = head * p.group + (live ? (int)((r0 + row) % p.group) : 0);
+        lo[m][half] = live ? key_lo(p, seq, tok) : 0;
+        hi[m][half] = live ? key_hi(p, seq, tok) : 0;
+        const char *src = reinterpret_cast<const char *>(p.q) + ((seq.q0 + tok) * p.q_st + qh * p.q_sh) * 2;
+        float top = 0.f;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+#pragma unroll
+          for (int part = 0; part < 2; ++part) {
+            // e4m3: a lane's four bytes of a key are elements 4t..4t+3 of a step, whichever column of the product they are
+            const int e = 16 * s + (E4M3 ? 4 * t4 + 2 * part : 8 * part + 2 * t4);
+            const uint32_t x = live && e < p.d ? *reinterpret_cast<const uint32_t *>(src + e * 2) : 0u;
+            qf[m][s][2 * part + half] = x;
+            if constexpr (E4M3) {
+              const float2 f = unpack2(x, T(0.f));
+              top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+            }
+          }
+        }
+        mul[m][half] = head_scale;
+        if constexpr (E4M3) {
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          const int ex = top > 0.f && top < __int_as_float(0x7f800000) ? min(max(ilogbf(top), -126), 126) : 0;
+          const float down = copysignf(ldexpf(1.f, -ex), p.k_scale[head]);
+          mul[m][half] = head_scale * ldexpf(1.f, ex);
+#pragma unroll
+          for (int s = 0; s < KS; ++s) {
+#pragma unroll
+            for (int part = 0; part < 2; ++part) {
+              const float2 f = unpack2(qf[m][s][2 * part + half], T(0.f));
+              qf[m][s][2 * part + half] = pack2(f.x * down, f.y * down, M(0.f));
+            }
+          }
+        }
+      }
+    }
+    // keys that every live row sees: pieces of them need no masks
+    const int all_lo = key_lo(p, seq, tok1), all_hi = key_hi(p, seq, tok0);
+
+    // ---- the ring -------------------------------------------------------------------------------------------
+    const char *kb = reinterpret_cast<const char *>(p.k) + head * p.k_sh * ES;
+    const char *vb = reinterpret_cast<const char *>(p.v) + head * p.v_sh * ES;
+    const int32_t *pages = p.table + b * p.table_stride;
+    const int key0 = unit0 * kUnit + warp * kKeys;
+    // the page of this lane's key (lanes 0-15) one piece ahead of its copies
+    auto page_id = [&](int i) -> int {
+      const int key = key0 + i * kUnit + (lane & 15);
+      if (i >= n_units || key < k_begin || key >= k_end) return -1;
+      const int id = pages[page_of(p, key)];
+      if (id >= 0 && id < p.num_pages) return id;
+      tc::report_timeout(p.status, kStatusBadIndex);
+      return -1;
+    };
+    int ahead = page_id(0);
+    auto issue = [&](int i) {
+      const int id = ahead;
+      ahead = page_id(i + 1);
+      if (i < n_units) {
+        const int key = key0 + i * kUnit + (lane & 15);
+        const int slot = key - page_of(p, key) * p.page;
+        const uint32_t dst = ring_addr + (i % S) * SB;
+        constexpr int RP = 32 / CH;            // rows per pass of the warp
+        const int c = lane % CH;
+        const int bytes = min(max(p.d * ES - c * 16, 0), 16);
+#pragma unroll
+        for (int j = 0; j < kKeys / RP; ++j) {
+          const int row = j * RP + lane / CH;
+          const int rid = __shfl_sync(0xffffffffu, id, row), rslot = __shfl_sync(0xffffffffu, slot, row);
+          const bool live = rid >= 0 && bytes > 0;
+          const int64_t ko = live ? (rid * p.k_sp + rslot * p.k_ss) * ES + c * 16 : 0;
+          const int64_t vo = live ? (rid * p.v_sp + rslot * p.v_ss) * ES + c * 16 : 0;
+          const int sw = CH == 4 ? (c ^ ((row >> 1) & 3)) : (c ^ (row & 7));
+          const uint32_t at = row * (CH * 16) + sw * 16;
+          cp_async16(dst + at, live ? kb + ko : kb, live ? bytes : 0);
+          cp_async16(dst + SB / 2 + at, live ? vb + vo : vb, live ? bytes : 0);
+        }
+      }
+      cp_async_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < S - 1; ++i) issue(i);
+
+    // ---- one pass over the keys -------------------------------------------------------------------------------
+    float o[MT][NT][4], top[MT][2], sum[MT][2];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) o[m][n][0] = o[m][n][1] = o[m][n][2] = o[m][n][3] = 0.f;
+      top[m][0] = top[m][1] = -INFINITY;
+      sum[m][0] = sum[m][1] = 0.f;
+    }
+    for (int i = 0; i < n_units; ++i) {
+      issue(i + S - 1);
+      cp_async_wait<S - 1>();
+      __syncwarp();
+      const uint32_t ks = ring_addr + (i % S) * SB, vs = ks + SB / 2;
+      // scores
+      float sc[MT][2][4];
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int n = 0; n < 2; ++n) sc[m][n][0] = sc[m][n][1] = sc[m][n][2] = sc[m][n][3] = 0.f;
+      auto frag_addr = [&](uint32_t base, int row, int c) {
+        const int sw = CH == 4 ? (c ^ ((row >> 1) & 3)) : (c ^ (row & 7));
+        return base + row * (CH * 16) + sw * 16;
+      };
+      if constexpr (!E4M3) {
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          uint32_t kf[4];   // keys 0-7: both halves of the step, keys 8-15: both halves
+          ldmatrix4(kf, frag_addr(ks, (lane & 7) + ((lane >> 4) << 3), 2 * s + ((lane >> 3) & 1)));
+#pragma unroll
+          for (int m = 0; m < MT; ++m) {
+            mma16816(sc[m][0], qf[m][s], kf[0], kf[1], M(0.f));
+            mma16816(sc[m][1], qf[m][s], kf[2], kf[3], M(0.f));
+          }
+        }
+      } else {
+#pragma unroll
+        for (int s = 0; s < KS; s += 2) {
+          uint32_t kf[4];   // step s: keys 0-7, keys 8-15; step s + 1: the same
+          ldmatrix4(kf, frag_addr(ks, (lane & 7) + (((lane >> 3) & 1) << 3), s + (lane >> 4)));
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t a0 = e4m3x2_to_f16x2(kf[2 * h]), a1 = e4m3x2_to_f16x2(kf[2 * h] >> 16);
+            const uint32_t b0 = e4m3x2_to_f16x2(kf[2 * h + 1]), b1 = e4m3x2_to_f16x2(kf[2 * h + 1] >> 16);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+              mma16816(sc[m][0], qf[m][s + h], a0, a1, M(0.f));
+              mma16816(sc[m][1], qf[m][s + h], b0, b1, M(0.f));
+            }
+          }
+        }
+      }
+      // masks, running maximum, probabilities
+      const int kbase = key0 + i * kUnit;
+      const bool inside = kbase >= all_lo && kbase + kKeys <= all_hi && kbase >= k_begin && kbase + kKeys <= k_end;
+      uint32_t pf[MT][4];
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          float x[4] = {sc[m][0][2 * half] * mul[m][half], sc[m][0][2 * half + 1] * mul[m][half],
+                        sc[m][1][2 * half] * mul[m][half], sc[m][1][2 * half + 1] * mul[m][half]};
+          if (!inside) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int key = kbase + (e >> 1) * 8 + 2 * t4 + (e & 1);
+              if (key < max(lo[m][half], k_begin) || key >= min(hi[m][half], k_end)) x[e] = -INFINITY;
+            }
+          }
+          float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+          // the reference of the exponents follows the maximum only when it has fallen far behind
+          if (__any_sync(0xffffffffu, mx > top[m][half] + kLazyRescale)) {
+            const float to = fmaxf(top[m][half], mx);
+            const float f = top[m][half] == -INFINITY ? 0.f : exp2_fast(top[m][half] - to);
+            sum[m][half] *= f;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) o[m][n][2 * half] *= f, o[m][n][2 * half + 1] *= f;
+            top[m][half] = to;
+          }
+          const float ref = top[m][half] == -INFINITY ? 0.f : top[m][half];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            x[e] = exp2_fast(x[e] - ref);
+            sum[m][half] += x[e];
+          }
+          pf[m][half] = pack2(x[0], x[1], M(0.f));
+          pf[m][2 + half] = pack2(x[2], x[3], M(0.f));
+        }
+      }
+      // output rows
+      if constexpr (!E4M3) {
+#pragma unroll
+        for (int n = 0; n < NT; n += 2) {
+          uint32_t vf[4];   // columns 8n..: keys 0-7, 8-15; the next eight columns: the same
+          ldmatrix4_trans(vf, frag_addr(vs, (lane & 7) + (((lane >> 3) & 1) << 3), n + (lane >> 4)));
+#pragma unroll
+          for (int m = 0; m < MT; ++m) {
+            mma16816(o[m][n], pf[m], vf[0], vf[1], M(0.f));
+            mma16816(o[m][n + 1], pf[m], vf[2], vf[3], M(0.f));
+          }
+        }
+      } else {
+#pragma unroll
+        for (int n = 0; n < NT; n += 4) {
+          uint32_t vf[4];   // chunk n/2: keys 0-7, 8-15; the next chunk.  A transposed unit is two neighbours of one key.
+          ldmatrix4_trans(vf, frag_addr(vs, (lane & 7) + (((lane >> 3) & 1) << 3), n / 2 + (lane >> 4)));
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t x = __byte_perm(vf[2 * h], 0, 0x3120), y = __byte_perm(vf[2 * h + 1], 0, 0x3120);
+            const uint32_t e0 = e4m3x2_to_f16x2(x), e1 = e4m3x2_to_f16x2(y);              // even columns of the chunk
+            const uint32_t d0 = e4m3x2_to_f16x2(x >> 16), d1 = e4m3x2_to_f16x2(y >> 16);   // odd columns
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+              mma16816(o[m][n + 2 * h], pf[m], e0, e1, M(0.f));
+              mma16816(o[m][n + 2 * h + 1], pf[m], d0, d1, M(0.f));
+            }
+          }
+        }
+      }
+      __syncwarp();   // the stage is read before the next copies overwrite it
+    }
+    cp_async_wait<0>();
+    __syncthreads();   // the merge overlays the rings
+
+    // ---- the four warps' rows added ----------------------------------------------------------------------------
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        sum[m][half] += __shfl_xor_sync(0xffffffffu, sum[m][half], 1);
+        sum[m][half] += __shfl_xor_sync(0xffffffffu, sum[m][half], 2);
+        if (sum[m][half] != sum[m][half]) top[m][half] = INFINITY;   // a NaN outweighs the other warps' rows
+        if (t4 == 0) merge_ml[warp * R + m * 16 + half * 8 + g] = make_float2(top[m][half], sum[m][half]);
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int row = m * 16 + half * 8 + g;
+        float best = -INFINITY;
+#pragma unroll
+        for (int v = 0; v < kWarps; ++v) best = fmaxf(best, merge_ml[v * R + row].x);
+        const float f = top[m][half] == -INFINITY ? 0.f : exp2_fast(top[m][half] - best);
+        float *dst = merge_o + (warp * R + row) * (DP + 8);
+        if constexpr (!E4M3) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+            *reinterpret_cast<float2 *>(dst + 8 * n + 2 * t4) = make_float2(o[m][n][2 * half] * f, o[m][n][2 * half + 1] * f);
+        } else {
+#pragma unroll
+          for (int n = 0; n < NT; n += 2)
+            *reinterpret_cast<float4 *>(dst + 8 * n + 4 * t4) =
+                make_float4(o[m][n][2 * half] * f, o[m][n + 1][2 * half] * f, o[m][n][2 * half + 1] * f, o[m][n + 1][2 * half + 1] * f);
+        }
+      }
+    }
+    __syncthreads();
+    const bool whole = w == h0 && w_end == h1;
+    const int slot = 2 * blockIdx.x + (w == h0 ? 1 : 0);
+    const float v_scale = E4M3 ? p.v_scale[head] : 1.f;
+    for (int idx = threadIdx.x; idx < n_rows * (DP / 4); idx += kThreads) {
+      const int row = idx / (DP / 4), c = (idx % (DP / 4)) * 4;
+      float best = -INFINITY, l = 0.f;
+#pragma unroll
+      for (int v = 0; v < kWarps; ++v) best = fmaxf(best, merge_ml[v * R + row].x);
+#pragma unroll
+      for (int v = 0; v < kWarps; ++v) {
+        const float2 ml = merge_ml[v * R + row];
+        l += ml.x == -INFINITY ? 0.f : ml.y * exp2_fast(ml.x - best);
+      }
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int v = 0; v < kWarps; ++v) {
+        const float4 x = *reinterpret_cast<const float4 *>(merge_o + (v * R + row) * (DP + 8) + c);
+        acc.x += x.x, acc.y += x.y, acc.z += x.z, acc.w += x.w;
+      }
+      if (whole) {
+        if (c < p.d) {
+          const float f = best == -INFINITY ? 0.f : v_scale / l;
+          const int tok = (int)((r0 + row) / p.group), qh = head * p.group + (int)((r0 + row) % p.group);
+          char *dst = reinterpret_cast<char *>(p.out) + ((seq.q0 + tok) * p.o_st + qh * p.o_sh + c) * 2;
+          *reinterpret_cast<uint2 *>(dst) = make_uint2(pack2(acc.x * f, acc.y * f, T(0.f)), pack2(acc.z * f, acc.w * f, T(0.f)));
+        }
+      } else {
+        *reinterpret_cast<float4 *>(p.part_o + ((int64_t)slot * R + row) * DP + c) =
+            make_float4(acc.x * v_scale, acc.y * v_scale, acc.z * v_scale, acc.w * v_scale);
+        if (c == 0) p.part_ml[(int64_t)slot * R + row] = make_float2(best, l);
+      }
+    }
+    if (threadIdx.x == 0 && !whole && w == h0) p.meta[blockIdx.x] = make_int4(b, tile, head, (int)((h1 - 1) / range.per));
+    __syncthreads();   // the merge area is read before the next rings fill it
+
+    w = w_end;
+    if (w_end == h1 && head == p.hkv - 1) {
+      ++tile;
+      item0 = h1;
+    }
+  }
+}
+
+template <typename T, bool E4M3, int DP, int MT>
+int launch(const AttnParams &p, const AttnPlan &plan, cudaStream_t st) {
+  constexpr int ring = ring_bytes<DP, E4M3>(), merge = merge_bytes<16 * MT, DP>();
+  constexpr int fixed = ring > merge ? ring : merge;
+  const int prefix = (p.batch + 1) * 4;
+  const int smem = prefix > fixed ? prefix : fixed;   // the division of the batch comes before the first copy
+  static PerDeviceOnce once;
+  auto kern = attention_stream_kernel<T, E4M3, DP, MT>;
+  const int rc = allow_dynamic_smem(once, kern, 110 * 1024);
+  if (rc != ZT_SUCCESS) return rc;
+  ZT_CUDA_OK(launch_overlapped(kern, dim3(plan.grid), dim3(kThreads), (size_t)smem, st, p));
+  return launch_status("attention_stream_kernel");
+}
+template <typename T, bool E4M3>
+int launch_sized(const AttnParams &p, const AttnPlan &plan, cudaStream_t st) {
+  if (plan.dp == 64) return plan.rows == 16 ? launch<T, E4M3, 64, 1>(p, plan, st) : launch<T, E4M3, 64, 2>(p, plan, st);
+  return plan.rows == 16 ? launch<T, E4M3, 128, 1>(p, plan, st) : launch<T, E4M3, 128, 2>(p, plan, st);
+}
+
+}  // namespace
+
+int attention_stream_grid() { return kCtasPerSm * sm_count(); }
+
+int attention_stream_launch(const AttnParams &p, const AttnPlan &plan, int dtype, int cache_dtype, cudaStream_t st) {
+  const bool e4m3 = cache_dtype == ZT_E4M3;
+  if (dtype == ZT_BF16)
+    return e4m3 ? launch_sized<__nv_bfloat16, true>(p, plan, st) : launch_sized<__nv_bfloat16, false>(p, plan, st);
+  return e4m3 ? launch_sized<__half, true>(p, plan, st) : launch_sized<__half, false>(p, plan, st);
+}
+
+}  // namespace zt

@@ -23,6 +23,7 @@ enum DeviceStatus : int {
   kStatusMmaTimeout = 102,       // MMA issuer waited for data
   kStatusEpilogueTimeout = 103,  // epilogue waited for the accumulator
   kStatusConvertTimeout = 104,   // dequant warps waited for a stage
+  kStatusBadIndex = 106,         // a page, slot or length outside the cache (the access was skipped)
   kStatusSelfTest = 199          // zt_selftest_expire_wait: the deliberately unanswered wait gave up
 };
 

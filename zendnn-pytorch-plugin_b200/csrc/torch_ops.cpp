@@ -25,16 +25,11 @@
 #include <vector>
 
 #include "../../include/zentorch_b200.h"
+#include "torch_util.h"
 
 namespace zentorch_b200 {
 
 namespace {
-
-#define ZT_TORCH_CALL(expr)                                         \
-  do {                                                              \
-    const int rc__ = (expr);                                        \
-    TORCH_CHECK(rc__ == ZT_SUCCESS, zt_last_error());               \
-  } while (0)
 
 int to_zt_dtype(const at::Tensor &t, const char *what) {
   if (t.scalar_type() == at::kBFloat16) return ZT_BF16;
@@ -50,16 +45,6 @@ at::Tensor as_2d(const at::Tensor &t) {
   at::Tensor c = (t.is_contiguous() && !zero_stride) ? t : t.contiguous();
   const int64_t last = c.size(c.dim() - 1);
   return c.view({last == 0 ? 0 : c.numel() / last, last});
-}
-
-// Every tensor argument must live on the input's GPU: the kernels take raw pointers, and a host pointer or
-// another device's pointer would fault on the GPU instead of raising here.
-void check_on_device(const at::Tensor &t, const at::Tensor &input, const char *op, const char *name) {
-  TORCH_CHECK(t.is_cuda() && t.device() == input.device(), op, ": ", name, " must be on the input's device (",
-              input.device(), "), got ", t.device());
-}
-void check_on_device(const std::optional<at::Tensor> &t, const at::Tensor &input, const char *op, const char *name) {
-  if (t.has_value() && t->defined()) check_on_device(*t, input, op, name);
 }
 
 // Weights are constants of a model, and the kernels read them before ordering themselves after earlier work

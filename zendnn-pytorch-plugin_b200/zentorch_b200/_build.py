@@ -4,7 +4,7 @@ Two shared objects are produced under ``zendnn-pytorch-plugin_b200/lib``:
 
 * ``libzentorch_b200.so`` -- the CUDA kernels and the C ABI (``include/zentorch_b200.h``), compiled with
   nvcc for sm_100a only.  It does not depend on PyTorch.
-* ``libzentorch_b200_torch.so`` -- the operator registrations (``csrc/torch_ops.cpp``) compiled with the
+* ``libzentorch_b200_torch.so`` -- the operator registrations (``csrc/torch_*.cpp``) compiled with the
   host compiler against the installed PyTorch, linked to the first.
 
 Run ``python -m zentorch_b200._build`` (or ``__graft_entry__.build()``) after changing sources.
@@ -80,9 +80,9 @@ def build_torch_ext(force: bool = False, verbose: bool = False) -> Path:
     import torch
     from torch.utils import cpp_extension
 
-    src = CSRC / "torch_ops.cpp"
-    deps = [src, *INCLUDE.glob("*.h"), KERNEL_LIB]
-    if not force and _newer(TORCH_LIB, deps):
+    sources = sorted(CSRC.glob("*.cpp"))
+    headers = [*CSRC.glob("*.h"), *INCLUDE.glob("*.h")]
+    if not force and _newer(TORCH_LIB, [*sources, *headers, KERNEL_LIB]):
         return TORCH_LIB
     torch_lib = Path(torch.__file__).parent / "lib"
     inc = []
@@ -91,14 +91,21 @@ def build_torch_ext(force: bool = False, verbose: bool = False) -> Path:
     import sysconfig
     inc += ["-isystem", sysconfig.get_paths()["include"]]
     cxx = "g++"
-    cmd = [
-        cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-D_GLIBCXX_USE_CXX11_ABI=1",
-        "-DTORCH_API_INCLUDE_EXTENSION_H", *inc, src, "-o", TORCH_LIB,
-        f"-L{torch_lib}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch",
-        f"-L{LIB_DIR}", "-lzentorch_b200", "-L/usr/local/cuda/lib64", "-lcudart",
-        "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{torch_lib}",
-    ]
-    _run(cmd, verbose)
+    OBJ_DIR.mkdir(parents=True, exist_ok=True)
+    jobs, objs = [], []
+    for src in sources:
+        obj = OBJ_DIR / (src.stem + ".cpp.o")
+        objs.append(obj)
+        if force or not _newer(obj, [src, *headers]):
+            jobs.append([cxx, "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-D_GLIBCXX_USE_CXX11_ABI=1",
+                         "-DTORCH_API_INCLUDE_EXTENSION_H", *inc, "-c", src, "-o", obj])
+    if jobs:
+        with concurrent.futures.ThreadPoolExecutor(max_workers=len(jobs)) as ex:
+            list(ex.map(lambda c: _run(c, verbose), jobs))
+    _run([cxx, "-shared", "-o", TORCH_LIB, *objs,
+          f"-L{torch_lib}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch",
+          f"-L{LIB_DIR}", "-lzentorch_b200", "-L/usr/local/cuda/lib64", "-lcudart",
+          "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{torch_lib}"], verbose)
     return TORCH_LIB
 
 

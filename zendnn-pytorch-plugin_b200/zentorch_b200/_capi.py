@@ -13,7 +13,7 @@ from pathlib import Path
 LIB_PATH = Path(__file__).resolve().parent.parent / "lib" / "libzentorch_b200.so"
 
 ZT_SUCCESS = 0
-ZT_BF16, ZT_F32, ZT_U8, ZT_S8 = 0, 1, 2, 3
+ZT_BF16, ZT_F32, ZT_U8, ZT_S8, ZT_F16, ZT_E4M3 = range(6)
 ZT_MAX_POST_OPS = 4
 ZT_WOQ_COUNTER_BYTES = 16384
 ZT_ALGO_AUTO, ZT_ALGO_GENERIC, ZT_ALGO_SKINNY, ZT_ALGO_TCGEN05 = 0, 1, 2, 3
@@ -34,6 +34,7 @@ EXPORTED_SYMBOLS = (
     "zt_int8_weight_rowsum", "zt_qlinear_prequantized", "zt_dynamic_qlinear_static",
     "zt_static_qlinear_workspace_bytes", "zt_static_qlinear", "zt_static_quantize",
     "zt_moe_woq_workspace_bytes", "zt_moe_woq", "zt_allreduce_symmetric_bytes", "zt_allreduce_bf16",
+    "zt_rope", "zt_cache_copy_pages", "zt_paged_attention_workspace_bytes", "zt_paged_attention",
 )
 
 
@@ -91,6 +92,41 @@ class AllReduceArgs(C.Structure):
     ]
 
 
+class RopeArgs(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("tokens", C.c_int64), ("q_heads", C.c_int32),
+        ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("rot_dim", C.c_int32), ("dtype", C.c_int32),
+        ("q_stride", C.c_int64 * 2), ("k_stride", C.c_int64 * 2), ("v_stride", C.c_int64 * 2), ("positions", C.c_void_p),
+        ("positions_64", C.c_int32), ("inv_freq", C.c_void_p), ("attention_factor", C.c_float),
+        ("interleaved", C.c_int32), ("q_out", C.c_void_p), ("k_out", C.c_void_p), ("q_out_stride", C.c_int64 * 2),
+        ("k_out_stride", C.c_int64 * 2), ("k_cache", C.c_void_p), ("v_cache", C.c_void_p), ("cache_dtype", C.c_int32),
+        ("k_cache_stride", C.c_int64 * 3), ("v_cache_stride", C.c_int64 * 3), ("num_pages", C.c_int64),
+        ("page_size", C.c_int32), ("slots", C.c_void_p), ("slots_64", C.c_int32), ("k_scale", C.c_void_p),
+        ("v_scale", C.c_void_p),
+    ]
+
+
+class CacheCopyArgs(C.Structure):
+    _fields_ = [
+        ("n_caches", C.c_int32), ("caches", C.POINTER(C.c_void_p)), ("page_stride_bytes", C.POINTER(C.c_int64)),
+        ("page_bytes", C.POINTER(C.c_int64)), ("num_pages", C.c_int32), ("n_pairs", C.c_int64), ("src", C.c_void_p),
+        ("dst", C.c_void_p), ("index_64", C.c_int32),
+    ]
+
+
+class PagedAttentionArgs(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("out", C.c_void_p), ("tokens", C.c_int64), ("batch", C.c_int32), ("q_heads", C.c_int32),
+        ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("dtype", C.c_int32), ("q_stride", C.c_int64 * 2),
+        ("out_stride", C.c_int64 * 2), ("k_cache", C.c_void_p), ("v_cache", C.c_void_p), ("cache_dtype", C.c_int32),
+        ("k_cache_stride", C.c_int64 * 3), ("v_cache_stride", C.c_int64 * 3), ("num_pages", C.c_int64),
+        ("page_size", C.c_int32), ("cu_seqlens_q", C.c_void_p), ("seq_lens", C.c_void_p), ("block_table", C.c_void_p),
+        ("block_table_stride", C.c_int64), ("max_blocks", C.c_int32), ("max_query_len", C.c_int32), ("scale", C.c_float),
+        ("causal", C.c_int32), ("window", C.c_int32), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+        ("zero_tail", C.c_int32), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("algo", C.c_int32),
+    ]
+
+
 class ZtError(RuntimeError):
     def __init__(self, code: int, message: str):
         super().__init__(message or f"zentorch_b200 error {code}")
@@ -144,6 +180,11 @@ def lib() -> C.CDLL:
     L.zt_allreduce_symmetric_bytes.restype = C.c_size_t
     L.zt_allreduce_symmetric_bytes.argtypes = [C.c_size_t]
     L.zt_allreduce_bf16.argtypes = [C.POINTER(AllReduceArgs), C.c_void_p]
+    L.zt_rope.argtypes = [C.POINTER(RopeArgs), C.c_void_p]
+    L.zt_cache_copy_pages.argtypes = [C.POINTER(CacheCopyArgs), C.c_void_p]
+    L.zt_paged_attention_workspace_bytes.restype = C.c_size_t
+    L.zt_paged_attention_workspace_bytes.argtypes = [C.POINTER(PagedAttentionArgs)]
+    L.zt_paged_attention.argtypes = [C.POINTER(PagedAttentionArgs), C.c_void_p]
     _lib = L
     return L
 
@@ -415,4 +456,36 @@ def moe_woq(x, topk_weights, topk_ids, w13, s13, w2, s2):
     a.scale_dtype, a.group_size = _dtype_code(s13), h // s13.shape[1]
     a.y, a.workspace, a.workspace_bytes = y.data_ptr(), ws.data_ptr(), nbytes
     check(lib().zt_moe_woq(C.byref(a), _stream_ptr()))
+    return y
+
+
+def _dtype_code_cache(dtype) -> int:
+    """Codes of the tensor dtypes of the rotary positions, the paged cache and its attention."""
+    import torch
+    return {torch.bfloat16: ZT_BF16, torch.float16: ZT_F16, torch.float32: ZT_F32, torch.float8_e4m3fn: ZT_E4M3}[dtype]
+
+
+def paged_attention(q, k_cache, v_cache, cu_seqlens_q, seq_lens, block_table, max_query_len=0, scale=None, causal=True,
+                    window=0, k_scale=None, v_scale=None, out=None, algo=ZT_ALGO_AUTO):
+    """zt_paged_attention on torch tensors: q [T, Hq, D], caches [P, page, Hkv, D], int32 lengths and pages.  `algo` forces
+    one kernel."""
+    import torch
+    a = PagedAttentionArgs()
+    y = out if out is not None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    a.q, a.out, a.tokens, a.batch = q.data_ptr(), y.data_ptr(), q.shape[0], seq_lens.shape[0]
+    a.q_heads, a.kv_heads, a.head_dim, a.dtype = q.shape[1], k_cache.shape[2], q.shape[2], _dtype_code_cache(q.dtype)
+    a.q_stride[:], a.out_stride[:] = q.stride()[:2], y.stride()[:2]
+    a.k_cache, a.v_cache, a.cache_dtype = k_cache.data_ptr(), v_cache.data_ptr(), _dtype_code_cache(k_cache.dtype)
+    a.k_cache_stride[:], a.v_cache_stride[:] = k_cache.stride()[:3], v_cache.stride()[:3]
+    a.num_pages, a.page_size = k_cache.shape[0], k_cache.shape[1]
+    a.cu_seqlens_q, a.seq_lens, a.block_table = cu_seqlens_q.data_ptr(), seq_lens.data_ptr(), block_table.data_ptr()
+    a.block_table_stride, a.max_blocks, a.max_query_len = block_table.stride(0), block_table.shape[1], max_query_len
+    a.scale = scale if scale is not None else q.shape[2] ** -0.5
+    a.causal, a.window = 1 if causal else 0, window
+    a.k_scale = k_scale.data_ptr() if k_scale is not None else None
+    a.v_scale = v_scale.data_ptr() if v_scale is not None else None
+    a.zero_tail, a.algo = 1 if out is None else 0, algo
+    ws = torch.empty(lib().zt_paged_attention_workspace_bytes(C.byref(a)), dtype=torch.uint8, device=q.device)
+    a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+    check(lib().zt_paged_attention(C.byref(a), _stream_ptr()))
     return y
