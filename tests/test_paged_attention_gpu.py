@@ -8,7 +8,7 @@ from _cache_ref import assert_attention, attention_ref, make_batch
 pytestmark = pytest.mark.gpu
 
 BF16, F16, E4M3 = torch.bfloat16, torch.float16, torch.float8_e4m3fn
-ALGOS = ["skinny"]
+ALGOS = ["skinny", "tcgen05"]
 
 
 @pytest.fixture(scope="module")

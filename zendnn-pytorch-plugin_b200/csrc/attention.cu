@@ -10,6 +10,7 @@ namespace {
 
 constexpr int kMaxBatch = 16384;   // the division of a batch keeps one int per sequence in shared memory
 constexpr int kCombineWarps = 4;   // rows per block
+constexpr int kMaxStreamRows = 32; // rows per kv head up to which a pass of the streaming kernel holds all of them
 
 // Joins the pieces of the item that is cut at the end of CTA blockIdx.x's range: one warp per row, each lane DP / 32 columns.
 // Bound by memory; the pieces are mostly still in L2.
@@ -72,10 +73,10 @@ AttnPlan make_plan(const zt_paged_attention_args_t &a) {
   const int64_t bound = a.tokens - a.batch + 1 > 1 ? a.tokens - a.batch + 1 : 1;
   const int64_t longest = a.max_query_len > 0 && a.max_query_len < bound ? a.max_query_len : bound;
   const int64_t rows = longest * group;
-  plan.tcgen05 = false;
+  plan.tcgen05 = a.algo == ZT_ALGO_TCGEN05 || (a.algo == ZT_ALGO_AUTO && rows > kMaxStreamRows);
   plan.dp = a.head_dim <= 64 ? 64 : 128;
-  plan.rows = rows <= 16 ? 16 : 32;
-  plan.grid = attention_stream_grid();
+  plan.rows = plan.tcgen05 ? 256 : rows <= 16 ? 16 : 32;
+  plan.grid = plan.tcgen05 ? sm_count() : attention_stream_grid();
   plan.meta_bytes = align256((size_t)plan.grid * sizeof(int4));
   plan.ml_bytes = align256((size_t)2 * plan.grid * plan.rows * sizeof(float2));
   plan.o_bytes = align256((size_t)2 * plan.grid * plan.rows * plan.dp * sizeof(float));
@@ -159,7 +160,8 @@ extern "C" int zt_paged_attention(const zt_paged_attention_args_t *a, void *stre
   p.status = status;
 
   cudaStream_t st = (cudaStream_t)stream;
-  const int rc = attention_stream_launch(p, plan, a->dtype, a->cache_dtype, st);
+  const int rc = plan.tcgen05 ? attention_tcgen05_launch(p, plan, a->dtype, a->cache_dtype, st)
+                              : attention_stream_launch(p, plan, a->dtype, a->cache_dtype, st);
   if (rc != ZT_SUCCESS) return rc;
   const dim3 grid((unsigned)plan.grid, (unsigned)ceil_div(plan.rows, kCombineWarps)), block(kCombineWarps * 32);
   const bool bf16 = a->dtype == ZT_BF16;

@@ -14,6 +14,8 @@
 
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "tc05.cuh"
 
 namespace zt {
@@ -201,6 +203,48 @@ __device__ AttnRange attention_range(const AttnParams &p, int min_units, int *pr
   return r;
 }
 
+// The pieces of items in a CTA's range, in order.
+template <int R, int UK>
+struct AttnWalk {
+  SeqInfo seq;
+  int b, tile, head;
+  int unit0, n_units;          // the piece's units of the item's keys
+  int n_rows;                  // rows of the item
+  int64_t r0;                  // first row
+  bool first_piece, whole;     // the item begins in this range; it lies in it
+  int last_cta;                // the CTA where the item ends
+
+  __device__ explicit AttnWalk(const AttnRange &r)
+      : seq{0, 0, 0}, b(r.b), tile(r.tile), head(-1), unit0(0), n_units(0), n_rows(0), r0(0), first_piece(false), whole(false),
+        last_cta(0), w_end_(r.w0), w1_(r.w1), per_(r.per), item0_(r.item0), h1_(-1), started_(false) {}
+  __device__ bool next(const AttnParams &p) {
+    const long long w = w_end_;
+    if (w >= w1_) return false;
+    if (!started_) seq = load_seq(p, b);
+    else if (w == h1_ && head == p.hkv - 1) ++tile, item0_ = h1_;
+    started_ = true;
+    while (tile >= row_tiles<R>(p, seq)) seq = load_seq(p, ++b), tile = 0;   // (sequences without new tokens have no tiles)
+    const TileUnits u = tile_units<R, UK>(p, seq, tile);
+    head = (int)(w - item0_) / u.count;                  // units of a tile over its kv heads fit 32 bits
+    const long long h0 = item0_ + (long long)head * u.count;
+    h1_ = h0 + u.count;
+    w_end_ = h1_ < w1_ ? h1_ : w1_;
+    n_units = (int)(w_end_ - w), unit0 = u.first + (int)(w - h0);
+    r0 = (int64_t)tile * R;
+    const int64_t rows = (int64_t)seq.n * p.group;
+    n_rows = (int)(rows - r0 < R ? rows - r0 : R);
+    first_piece = w == h0, whole = first_piece && w_end_ == h1_;
+    last_cta = (int)((h1_ - 1) / per_);
+    return true;
+  }
+  __device__ int token(const AttnParams &p, int row) const { return (int)((r0 + row) / p.group); }
+  __device__ int q_head(const AttnParams &p, int row) const { return head * p.group + (int)((r0 + row) % p.group); }
+
+ private:
+  long long w_end_, w1_, per_, item0_, h1_;
+  bool started_;
+};
+
 // Row of the cache that holds a key: page id, slot in it.  An id outside the cache reads as no row and is reported.
 __device__ __forceinline__ int page_of(const AttnParams &p, int key) { return p.page_shift >= 0 ? key >> p.page_shift : key / p.page; }
 
@@ -223,6 +267,14 @@ __device__ __forceinline__ uint32_t pack2(float x, float y, __nv_bfloat16) {
 __device__ __forceinline__ uint32_t pack2(float x, float y, __half) {
   const __half2 v = __floats2half2_rn(x, y);
   return *reinterpret_cast<const uint32_t *>(&v);
+}
+__device__ __forceinline__ float2 unpack2(uint32_t w, __nv_bfloat16) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+__device__ __forceinline__ float2 unpack2(uint32_t w, __half) { return __half22float2(*reinterpret_cast<const __half2 *>(&w)); }
+// Power of two that brings a row whose largest element is `top` to a maximum in [1, 2); none for rows of zeros or not finite.
+__device__ __forceinline__ int row_exponent(float top) {
+  return top > 0.f && top < __int_as_float(0x7f800000) ? min(max(ilogbf(top), -126), 126) : 0;
 }
 // Two e4m3 values (the low 16 bits) as halves; exact.
 __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two) {

@@ -61,23 +61,9 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-template <typename T, bool E4M3>
-struct MmaType {
-  using type = T;
-};
-template <typename T>
-struct MmaType<T, true> {
-  using type = __half;
-};
-
-__device__ __forceinline__ float2 unpack2(uint32_t w, __nv_bfloat16) {
-  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
-}
-__device__ __forceinline__ float2 unpack2(uint32_t w, __half) { return __half22float2(*reinterpret_cast<const __half2 *>(&w)); }
-
 template <typename T, bool E4M3, int DP, int MT>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_stream_kernel(const __grid_constant__ AttnParams p) {
-  using M = typename MmaType<T, E4M3>::type;
+  using M = std::conditional_t<E4M3, __half, T>;
   constexpr int R = 16 * MT, S = stages<E4M3>(), SB = stage_bytes<DP, E4M3>();
   constexpr int ES = E4M3 ? 1 : 2;
   constexpr int CH = DP * ES / 16;            // 16-byte chunks of a key's row
@@ -89,7 +75,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_stream_kernel(
   grid_dependency_wait();
   const int lane = threadIdx.x & 31, warp = tc::uniform_warp();
   const int g = lane >> 2, t4 = lane & 3;
-  AttnRange range = attention_range<R, kUnit, kThreads>(p, 1, reinterpret_cast<int *>(smem), s_scan);
+  const AttnRange range = attention_range<R, kUnit, kThreads>(p, 1, reinterpret_cast<int *>(smem), s_scan);
   zero_tail_rows<T>(p, kThreads);
   unsigned char *ring = smem + warp * S * SB;
   const uint32_t ring_addr = smem_u32(ring);
@@ -97,21 +83,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_stream_kernel(
   float2 *merge_ml = reinterpret_cast<float2 *>(smem + kWarps * R * (DP + 8) * 4);    // [warp][R]
   if (threadIdx.x == 0) p.meta[blockIdx.x] = make_int4(-1, 0, 0, 0);
 
-  long long w = range.w0;
-  int b = range.b, tile = range.tile;
-  long long item0 = range.item0;
-  SeqInfo seq = range.w0 < range.w1 ? load_seq(p, b) : SeqInfo{0, 0, 0};
-  while (w < range.w1) {
-    // ---- the next piece of an item in this CTA's range --------------------------------------------------
-    while (tile >= row_tiles<R>(p, seq)) seq = load_seq(p, ++b), tile = 0;   // (sequences without new tokens have no tiles)
-    const TileUnits units = tile_units<R, kUnit>(p, seq, tile);
-    const int head = (int)((w - item0) / units.count);
-    const long long h0 = item0 + (long long)head * units.count, h1 = h0 + units.count;   // the item's units
-    const long long w_end = h1 < range.w1 ? h1 : range.w1;
-    const int n_units = (int)(w_end - w), unit0 = units.first + (int)(w - h0);
-    const int64_t rows = (int64_t)seq.n * p.group, r0 = (int64_t)tile * R;
-    const int n_rows = (int)(rows - r0 < R ? rows - r0 : R);
-    const int tok0 = (int)(r0 / p.group), tok1 = (int)((r0 + n_rows - 1) / p.group);
+  AttnWalk<R, kUnit> it(range);
+  while (it.next(p)) {
+    const SeqInfo seq = it.seq;
+    const int b = it.b, head = it.head, n_units = it.n_units, unit0 = it.unit0, n_rows = it.n_rows;
+    const int tok0 = it.token(p, 0), tok1 = it.token(p, n_rows - 1);
     // keys that some row sees, within this piece
     const int k_begin = max(key_lo(p, seq, tok0), unit0 * kUnit);
     const int k_end = min((long long)key_hi(p, seq, tok1), ((long long)unit0 + n_units) * kUnit);
@@ -127,8 +103,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_stream_kernel(
       for (int half = 0; half < 2; ++half) {
         const int row = m * 16 + half * 8 + g;
         const bool live = row < n_rows;
-        const int tok = live ? (int)((r0 + row) / p.group) : tok0;
-        const int qh = head * p.group + (live ? (int)((r0 + row) % p.group) : 0);
+        const int tok = it.token(p, live ? row : 0), qh = it.q_head(p, live ? row : 0);
         lo[m][half] = live ? key_lo(p, seq, tok) : 0;
         hi[m][half] = live ? key_hi(p, seq, tok) : 0;
         const char *src = reinterpret_cast<const char *>(p.q) + ((seq.q0 + tok) * p.q_st + qh * p.q_sh) * 2;
@@ -151,7 +126,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_stream_kernel(
         if constexpr (E4M3) {
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-          const int ex = top > 0.f && top < __int_as_float(0x7f800000) ? min(max(ilogbf(top), -126), 126) : 0;
+          const int ex = row_exponent(top);
           const float down = copysignf(ldexpf(1.f, -ex), p.k_scale[head]);
           mul[m][half] = head_scale * ldexpf(1.f, ex);
 #pragma unroll
@@ -372,8 +347,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_stream_kernel(
       }
     }
     __syncthreads();
-    const bool whole = w == h0 && w_end == h1;
-    const int slot = 2 * blockIdx.x + (w == h0 ? 1 : 0);
+    const int slot = 2 * blockIdx.x + (it.first_piece ? 1 : 0);
     const float v_scale = E4M3 ? p.v_scale[head] : 1.f;
     for (int idx = threadIdx.x; idx < n_rows * (DP / 4); idx += kThreads) {
       const int row = idx / (DP / 4), c = (idx % (DP / 4)) * 4;
@@ -391,10 +365,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_stream_kernel(
         const float4 x = *reinterpret_cast<const float4 *>(merge_o + (v * R + row) * (DP + 8) + c);
         acc.x += x.x, acc.y += x.y, acc.z += x.z, acc.w += x.w;
       }
-      if (whole) {
+      if (it.whole) {
         if (c < p.d) {
           const float f = best == -INFINITY ? 0.f : v_scale / l;
-          const int tok = (int)((r0 + row) / p.group), qh = head * p.group + (int)((r0 + row) % p.group);
+          const int tok = it.token(p, row), qh = it.q_head(p, row);
           char *dst = reinterpret_cast<char *>(p.out) + ((seq.q0 + tok) * p.o_st + qh * p.o_sh + c) * 2;
           *reinterpret_cast<uint2 *>(dst) = make_uint2(pack2(acc.x * f, acc.y * f, T(0.f)), pack2(acc.z * f, acc.w * f, T(0.f)));
         }
@@ -404,14 +378,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_stream_kernel(
         if (c == 0) p.part_ml[(int64_t)slot * R + row] = make_float2(best, l);
       }
     }
-    if (threadIdx.x == 0 && !whole && w == h0) p.meta[blockIdx.x] = make_int4(b, tile, head, (int)((h1 - 1) / range.per));
+    if (threadIdx.x == 0 && !it.whole && it.first_piece) p.meta[blockIdx.x] = make_int4(b, it.tile, head, it.last_cta);
     __syncthreads();   // the merge area is read before the next rings fill it
-
-    w = w_end;
-    if (w_end == h1 && head == p.hkv - 1) {
-      ++tile;
-      item0 = h1;
-    }
   }
 }
 

@@ -229,6 +229,14 @@ __device__ __forceinline__ uint64_t smem_desc_k_sw128(uint32_t smem_addr) {
   return d;
 }
 
+// High word of the descriptor of a tile stored as above whose rows are K: the operand's other dimension runs along the 128-byte
+// rows (64 16-bit elements), its next 64 are the leading byte offset away, and 8-row groups of K are 1024 bytes apart.
+constexpr uint32_t kDescHiSw128 = (1024 >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_lo_mn_sw128(uint32_t smem_addr, uint32_t leading_bytes) {
+  return ((smem_addr & 0x3FFFF) >> 4) | ((leading_bytes >> 4) << 16);
+}
+constexpr uint32_t kInstrBMnMajor = 1u << 16;   // instruction descriptor bit: B is such a tile
+
 // Instruction descriptor (dense, no negate, both operands K-major).
 //   c_format: 1 = f32, 2 = s32.   a/b_format: kind::f16 -> 0 f16, 1 bf16;  kind::i8 -> 0 u8, 1 s8.
 __host__ __device__ constexpr uint32_t instr_desc(uint32_t c_format, uint32_t a_format, uint32_t b_format, uint32_t m,
@@ -250,6 +258,14 @@ __device__ __forceinline__ void mma_commit_if(bool lane_does, uint32_t bar_addr)
       "{.reg .pred p; setp.ne.b32 p, %0, 0; @p tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%1];}" ::"r"(
           (uint32_t)lane_does),
       "r"(bar_addr)
+      : "memory");
+}
+// Both operands in shared memory.
+__device__ __forceinline__ void mma_f16_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 // A operand (128 rows, two bf16 of K per 32-bit column) in tensor memory.
