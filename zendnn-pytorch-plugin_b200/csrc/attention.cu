@@ -21,7 +21,7 @@ __global__ void __launch_bounds__(kCombineWarps * 32) attention_combine_kernel(c
   const int4 item = p.meta[blockIdx.x];
   if (item.x < 0) return;
   const SeqInfo seq = load_seq(p, item.x);
-  const int64_t r0 = (int64_t)item.y * R, rows = (int64_t)seq.n * p.group;
+  const int r0 = item.y * R, rows = seq.n * p.group;
   const int row = blockIdx.y * kCombineWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (row >= R || r0 + row >= rows) return;
   const int first = blockIdx.x, count = item.w - first + 1;
@@ -56,12 +56,63 @@ __global__ void __launch_bounds__(kCombineWarps * 32) attention_combine_kernel(c
   }
   if (lane * V >= p.d) return;
   const float f = top == -INFINITY ? 0.f : 1.f / sum;
-  const int tok = (int)((r0 + row) / p.group), qh = item.z * p.group + (int)((r0 + row) % p.group);
+  const int tok = (r0 + row) / p.group, qh = item.z * p.group + (r0 + row) % p.group;
   char *dst = reinterpret_cast<char *>(p.out) + ((seq.q0 + tok) * p.o_st + qh * p.o_sh + lane * V) * 2;
   if constexpr (V == 4)
     *reinterpret_cast<uint2 *>(dst) = make_uint2(pack2(acc[0] * f, acc[1] * f, T(0.f)), pack2(acc[2] * f, acc[3] * f, T(0.f)));
   else
     *reinterpret_cast<uint32_t *>(dst) = pack2(acc[0] * f, acc[1] * f, T(0.f));
+}
+
+// The same for the pieces of the tcgen05 kernel, whose rows are neighbours in the workspace: a lane per row, a warp per 16 columns.
+template <typename T, int DP>
+__global__ void __launch_bounds__(DP * 2) attention_combine_rows_kernel(const __grid_constant__ AttnParams p, int R) {
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const int4 item = p.meta[blockIdx.x];
+  if (item.x < 0) return;
+  const SeqInfo seq = load_seq(p, item.x);
+  const int row = blockIdx.y * 32 + (threadIdx.x & 31), c0 = (threadIdx.x >> 5) * 16;
+  const int first = blockIdx.x, count = item.w - first + 1, r = item.y * R + row;
+  if (r >= seq.n * p.group || c0 >= p.d) return;
+  auto slot = [&](int i) { return (int64_t)(2 * (first + i) + (i == 0 ? 1 : 0)); };
+  float acc[16] = {}, sum = 0.f, top = -INFINITY;
+  for (int i = 0; i < count; ++i) {
+    const float2 ml = p.part_ml[slot(i) * R + row];
+    const float4 *src = reinterpret_cast<const float4 *>(p.part_o) + (slot(i) * (DP / 4) + c0 / 4) * R + row;
+    float4 x[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) x[q] = src[(int64_t)q * R];
+    const float to = fmaxf(top, ml.x);
+    const float f_old = top == -INFINITY ? 0.f : exp2_fast(top - to), f = ml.x == -INFINITY ? 0.f : exp2_fast(ml.x - to);
+    top = to;
+    sum = sum * f_old + ml.y * f;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      acc[4 * q] = acc[4 * q] * f_old + x[q].x * f, acc[4 * q + 1] = acc[4 * q + 1] * f_old + x[q].y * f;
+      acc[4 * q + 2] = acc[4 * q + 2] * f_old + x[q].z * f, acc[4 * q + 3] = acc[4 * q + 3] * f_old + x[q].w * f;
+    }
+  }
+  const float f = top == -INFINITY ? 0.f : 1.f / sum;
+  const int tok = r / p.group, qh = item.z * p.group + r % p.group;
+  uint4 *dst = reinterpret_cast<uint4 *>(reinterpret_cast<char *>(p.out) + ((seq.q0 + tok) * p.o_st + qh * p.o_sh + c0) * 2);
+#pragma unroll
+  for (int q = 0; q < 2; ++q)
+    if (c0 + 8 * q < p.d)
+      dst[q] = make_uint4(pack2(acc[8 * q] * f, acc[8 * q + 1] * f, T(0.f)), pack2(acc[8 * q + 2] * f, acc[8 * q + 3] * f, T(0.f)),
+                          pack2(acc[8 * q + 4] * f, acc[8 * q + 5] * f, T(0.f)), pack2(acc[8 * q + 6] * f, acc[8 * q + 7] * f, T(0.f)));
+}
+
+template <typename T>
+cudaError_t launch_combine(const AttnParams &p, const AttnPlan &plan, cudaStream_t st) {
+  if (plan.tcgen05) {
+    const dim3 grid((unsigned)plan.grid, (unsigned)(plan.rows / 32)), block((unsigned)plan.dp * 2);
+    return plan.dp == 64 ? launch_overlapped(attention_combine_rows_kernel<T, 64>, grid, block, (size_t)0, st, p, plan.rows)
+                         : launch_overlapped(attention_combine_rows_kernel<T, 128>, grid, block, (size_t)0, st, p, plan.rows);
+  }
+  const dim3 grid((unsigned)plan.grid, (unsigned)ceil_div(plan.rows, kCombineWarps)), block(kCombineWarps * 32);
+  return plan.dp == 64 ? launch_overlapped(attention_combine_kernel<T, 64>, grid, block, (size_t)0, st, p, plan.rows)
+                       : launch_overlapped(attention_combine_kernel<T, 128>, grid, block, (size_t)0, st, p, plan.rows);
 }
 
 size_t align256(size_t v) { return (v + 255) / 256 * 256; }
@@ -104,6 +155,7 @@ extern "C" int zt_paged_attention(const zt_paged_attention_args_t *a, void *stre
   ZT_REQUIRE(a->tokens >= 0 && a->batch >= 0 && a->max_blocks >= 0 && a->num_pages >= 0 && a->max_query_len >= 0, ZT_INVALID_ARGUMENT,
              "zt_paged_attention: negative size");
   ZT_REQUIRE(a->tokens <= (1 << 30) && a->num_pages <= (1 << 30), ZT_UNSUPPORTED, "zt_paged_attention: more than 2^30 tokens or pages");
+  ZT_REQUIRE(a->q_heads <= 0 || a->tokens * a->q_heads < (1 << 30), ZT_UNSUPPORTED, "zt_paged_attention: 2^30 or more query rows");
   ZT_REQUIRE(a->batch <= kMaxBatch, ZT_UNSUPPORTED, "zt_paged_attention: %d sequences, at most %d", a->batch, kMaxBatch);
   ZT_REQUIRE(a->q_heads >= 1 && a->kv_heads >= 1 && a->q_heads % a->kv_heads == 0 && a->q_heads <= 4096, ZT_INVALID_ARGUMENT,
              "zt_paged_attention: the query heads (%d) must be a multiple of the key/value heads (%d)", a->q_heads, a->kv_heads);
@@ -163,13 +215,6 @@ extern "C" int zt_paged_attention(const zt_paged_attention_args_t *a, void *stre
   const int rc = plan.tcgen05 ? attention_tcgen05_launch(p, plan, a->dtype, a->cache_dtype, st)
                               : attention_stream_launch(p, plan, a->dtype, a->cache_dtype, st);
   if (rc != ZT_SUCCESS) return rc;
-  const dim3 grid((unsigned)plan.grid, (unsigned)ceil_div(plan.rows, kCombineWarps)), block(kCombineWarps * 32);
-  const bool bf16 = a->dtype == ZT_BF16;
-  if (plan.dp == 64)
-    ZT_CUDA_OK(bf16 ? launch_overlapped(attention_combine_kernel<__nv_bfloat16, 64>, grid, block, (size_t)0, st, p, plan.rows)
-                    : launch_overlapped(attention_combine_kernel<__half, 64>, grid, block, (size_t)0, st, p, plan.rows));
-  else
-    ZT_CUDA_OK(bf16 ? launch_overlapped(attention_combine_kernel<__nv_bfloat16, 128>, grid, block, (size_t)0, st, p, plan.rows)
-                    : launch_overlapped(attention_combine_kernel<__half, 128>, grid, block, (size_t)0, st, p, plan.rows));
+  ZT_CUDA_OK(a->dtype == ZT_BF16 ? launch_combine<__nv_bfloat16>(p, plan, st) : launch_combine<__half>(p, plan, st));
   return launch_status("attention_combine_kernel");
 }

@@ -7,7 +7,8 @@
 //
 // Work.  The units of all items, in the order (sequence, tile, kv head, unit), are dealt to the CTAs in equal contiguous ranges,
 // found by every CTA for itself from the lengths in device memory: nothing about the lengths is known on the host, and a
-// captured launch follows them.  An item that lies in one range is written directly; one that is cut leaves unnormalised sums
+// captured launch follows them.  An item counts for a few units more than it has, for its query rows, first and last loads and
+// output (`EXTRA`, per kernel; they come before its first unit).  An item that lies in one range is written directly; one that is cut leaves unnormalised sums
 // with their maxima in the workspace, at most one at either end of a CTA's range, and attention_combine_kernel joins them in CTA
 // order.
 #pragma once
@@ -86,7 +87,7 @@ __device__ __forceinline__ int key_lo(const AttnParams &p, const SeqInfo &s, int
 
 template <int R>
 __device__ __forceinline__ int row_tiles(const AttnParams &p, const SeqInfo &s) {
-  return (int)(((int64_t)s.n * p.group + R - 1) / R);
+  return (int)(((unsigned)s.n * (unsigned)p.group + R - 1) / R);       // (tokens * q_heads stays below 2^30)
 }
 
 // Units of UK keys of a tile: [first, first + count).  A tile that sees nothing still has one, in which its zeros are written.
@@ -95,9 +96,8 @@ struct TileUnits {
 };
 template <int R, int UK>
 __device__ __forceinline__ TileUnits tile_units(const AttnParams &p, const SeqInfo &s, int tile) {
-  const int64_t rows = (int64_t)s.n * p.group, r0 = (int64_t)tile * R;
-  const int64_t r1 = (r0 + R < rows ? r0 + R : rows) - 1;
-  const int lo = key_lo(p, s, (int)(r0 / p.group)), hi = key_hi(p, s, (int)(r1 / p.group));
+  const int rows = s.n * p.group, r0 = tile * R, r1 = min(r0 + R, rows) - 1;
+  const int lo = key_lo(p, s, r0 / p.group), hi = key_hi(p, s, r1 / p.group);
   if (hi <= lo) return {0, 1};
   return {lo / UK, (hi + UK - 1) / UK - lo / UK};
 }
@@ -138,7 +138,7 @@ struct AttnRange {
 };
 
 // Whole-block call.  `prefix`: batch + 1 ints of shared memory; `scratch`: 40 long longs.
-template <int R, int UK, int NT>
+template <int R, int UK, int EXTRA, int NT>
 __device__ AttnRange attention_range(const AttnParams &p, int min_units, int *prefix, long long *scratch) {
   // tiles of the sequences before each sequence
   const int chunk = (p.batch + NT - 1) / NT;
@@ -173,7 +173,7 @@ __device__ AttnRange attention_range(const AttnParams &p, int min_units, int *pr
     SeqInfo s = load_seq(p, bb);
     for (int t = t0; t < t1; ++t) {
       while (t >= prefix[bb + 1]) s = load_seq(p, ++bb);
-      mine += (long long)tile_units<R, UK>(p, s, t - prefix[bb]).count * p.hkv;
+      mine += (long long)(tile_units<R, UK>(p, s, t - prefix[bb]).count + EXTRA) * p.hkv;
     }
   }
   long long total;
@@ -188,7 +188,7 @@ __device__ AttnRange attention_range(const AttnParams &p, int min_units, int *pr
       SeqInfo s = load_seq(p, b);
       for (int t = t0; t < t1; ++t) {
         while (t >= prefix[b + 1]) s = load_seq(p, ++b);
-        const long long u = (long long)tile_units<R, UK>(p, s, t - prefix[b]).count * p.hkv;
+        const long long u = (long long)(tile_units<R, UK>(p, s, t - prefix[b]).count + EXTRA) * p.hkv;
         if (r.w0 < at + u) {
           scratch[36] = at, scratch[37] = b, scratch[38] = t - prefix[b];
           break;
@@ -204,41 +204,42 @@ __device__ AttnRange attention_range(const AttnParams &p, int min_units, int *pr
 }
 
 // The pieces of items in a CTA's range, in order.
-template <int R, int UK>
+template <int R, int UK, int EXTRA>
 struct AttnWalk {
   SeqInfo seq;
   int b, tile, head;
   int unit0, n_units;          // the piece's units of the item's keys
-  int n_rows;                  // rows of the item
-  int64_t r0;                  // first row
-  bool first_piece, whole;     // the item begins in this range; it lies in it
-  int last_cta;                // the CTA where the item ends
+  int n_rows, r0;              // rows of the item, first of them
+  bool first_piece, whole;     // the item's first unit is in this piece; all of them are
 
   __device__ explicit AttnWalk(const AttnRange &r)
       : seq{0, 0, 0}, b(r.b), tile(r.tile), head(-1), unit0(0), n_units(0), n_rows(0), r0(0), first_piece(false), whole(false),
-        last_cta(0), w_end_(r.w0), w1_(r.w1), per_(r.per), item0_(r.item0), h1_(-1), started_(false) {}
+        w_end_(r.w0), w1_(r.w1), per_(r.per), item0_(r.item0), h1_(-1), started_(false) {}
   __device__ bool next(const AttnParams &p) {
-    const long long w = w_end_;
-    if (w >= w1_) return false;
-    if (!started_) seq = load_seq(p, b);
-    else if (w == h1_ && head == p.hkv - 1) ++tile, item0_ = h1_;
-    started_ = true;
-    while (tile >= row_tiles<R>(p, seq)) seq = load_seq(p, ++b), tile = 0;   // (sequences without new tokens have no tiles)
-    const TileUnits u = tile_units<R, UK>(p, seq, tile);
-    head = (int)(w - item0_) / u.count;                  // units of a tile over its kv heads fit 32 bits
-    const long long h0 = item0_ + (long long)head * u.count;
-    h1_ = h0 + u.count;
-    w_end_ = h1_ < w1_ ? h1_ : w1_;
-    n_units = (int)(w_end_ - w), unit0 = u.first + (int)(w - h0);
-    r0 = (int64_t)tile * R;
-    const int64_t rows = (int64_t)seq.n * p.group;
-    n_rows = (int)(rows - r0 < R ? rows - r0 : R);
-    first_piece = w == h0, whole = first_piece && w_end_ == h1_;
-    last_cta = (int)((h1_ - 1) / per_);
-    return true;
+    for (;;) {
+      const long long w = w_end_;
+      if (w >= w1_) return false;
+      if (!started_) seq = load_seq(p, b);
+      else if (w == h1_ && head == p.hkv - 1) ++tile, item0_ = h1_;
+      started_ = true;
+      while (tile >= row_tiles<R>(p, seq)) seq = load_seq(p, ++b), tile = 0;   // (sequences without new tokens have no tiles)
+      const TileUnits u = tile_units<R, UK>(p, seq, tile);
+      const int cost = u.count + EXTRA;
+      head = (int)(w - item0_) / cost;                   // units of a tile over its kv heads fit 32 bits
+      const long long h0 = item0_ + (long long)head * cost;
+      h1_ = h0 + cost;
+      w_end_ = h1_ < w1_ ? h1_ : w1_;
+      const int from = max((int)(w - h0) - EXTRA, 0), to = (int)(w_end_ - h0) - EXTRA;
+      if (to <= from) continue;                          // the range ends before the item's first unit
+      n_units = to - from, unit0 = u.first + from;
+      r0 = tile * R, n_rows = min(seq.n * p.group - r0, R);
+      first_piece = from == 0, whole = first_piece && w_end_ == h1_;
+      return true;
+    }
   }
-  __device__ int token(const AttnParams &p, int row) const { return (int)((r0 + row) / p.group); }
-  __device__ int q_head(const AttnParams &p, int row) const { return head * p.group + (int)((r0 + row) % p.group); }
+  __device__ int last_cta() const { return (int)((h1_ - 1) / per_); }   // where the item ends
+  __device__ int token(const AttnParams &p, int row) const { return (r0 + row) / p.group; }
+  __device__ int q_head(const AttnParams &p, int row) const { return head * p.group + (r0 + row) % p.group; }
 
  private:
   long long w_end_, w1_, per_, item0_, h1_;

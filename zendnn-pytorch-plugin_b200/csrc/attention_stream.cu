@@ -21,6 +21,7 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kKeys = 16;                  // of a warp per unit
 constexpr int kUnit = kWarps * kKeys;
 constexpr int kCtasPerSm = 2;
+constexpr int kExtra = 2;                  // units that an item costs beside its own
 
 template <int DP, bool E4M3>
 __host__ __device__ constexpr int stage_bytes() { return 2 * kKeys * DP * (E4M3 ? 1 : 2); }
@@ -75,7 +76,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_stream_kernel(
   grid_dependency_wait();
   const int lane = threadIdx.x & 31, warp = tc::uniform_warp();
   const int g = lane >> 2, t4 = lane & 3;
-  const AttnRange range = attention_range<R, kUnit, kThreads>(p, 1, reinterpret_cast<int *>(smem), s_scan);
+  const AttnRange range = attention_range<R, kUnit, kExtra, kThreads>(p, 1, reinterpret_cast<int *>(smem), s_scan);
   zero_tail_rows<T>(p, kThreads);
   unsigned char *ring = smem + warp * S * SB;
   const uint32_t ring_addr = smem_u32(ring);
@@ -83,7 +84,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_stream_kernel(
   float2 *merge_ml = reinterpret_cast<float2 *>(smem + kWarps * R * (DP + 8) * 4);    // [warp][R]
   if (threadIdx.x == 0) p.meta[blockIdx.x] = make_int4(-1, 0, 0, 0);
 
-  AttnWalk<R, kUnit> it(range);
+  AttnWalk<R, kUnit, kExtra> it(range);
   while (it.next(p)) {
     const SeqInfo seq = it.seq;
     const int b = it.b, head = it.head, n_units = it.n_units, unit0 = it.unit0, n_rows = it.n_rows;
@@ -378,7 +379,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_stream_kernel(
         if (c == 0) p.part_ml[(int64_t)slot * R + row] = make_float2(best, l);
       }
     }
-    if (threadIdx.x == 0 && !it.whole && it.first_piece) p.meta[blockIdx.x] = make_int4(b, it.tile, head, it.last_cta);
+    if (threadIdx.x == 0 && !it.whole && it.first_piece) p.meta[blockIdx.x] = make_int4(b, it.tile, head, it.last_cta());
     __syncthreads();   // the merge area is read before the next rings fill it
   }
 }

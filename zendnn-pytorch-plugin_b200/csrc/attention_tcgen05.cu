@@ -1,15 +1,17 @@
 // Paged attention on the tensor cores of sm_100a, for chunks and prompts.
 //
 // An item is 256 (token, head of the group) rows of one kv head, as two tiles of 128 that share every K and V tile of 128 keys.
-// Scores S = Q K^T of a tile go to tensor memory (128 columns), one thread per row turns them into probabilities that replace
-// them there as 16-bit pairs, and O += P V accumulates in tensor memory with P as the tensor-memory operand.  Of the two tiles
+// Scores S = Q K^T of a tile go to tensor memory (128 columns), one thread per row turns them into probabilities, 16-bit pairs in
+// 64 of the same columns, and O += P V accumulates in tensor memory with P as the tensor-memory operand.  Of the two tiles
 // one is in its exponentials while the tensor core works for the other.
 //
 //   warps 0-3, 4-7   a row of tile 0 / 1 each thread: query rows to shared memory, running maximum and sum, probabilities, output
-//   warps 8-11       K and V tiles into a ring, row by row from the pages (any page size), 16 bytes per asynchronous copy; slots past
-//                    the visible keys become zeros, so stale contents of a page never meet the arithmetic.  e4m3 caches come
-//                    through registers and are stored as halves (exact)
+//   warps 8-11       K and V tiles into a ring, 32 keys each: by TMA, in boxes of up to 32 slots of a page, where the pages hold a power
+//                    of two of at least 8 slots and all 32 keys are visible; else row by row, 16 bytes per asynchronous copy (any
+//                    page size).  Slots past the visible keys become zeros that way, so stale contents of a page never meet the
+//                    arithmetic.  e4m3 caches come through registers and are stored as halves (exact)
 //   warp 12          issues the MMAs
+//   warp 13          walks the CTA's range and hands its pieces to the others
 //
 // The reference of the exponents follows the row maximum only when that has run 8 (log2) ahead of it, so the rows of O are
 // rescaled a few times at the start and hardly ever after; the thread that finds it does it itself.  Probabilities are rounded
@@ -23,9 +25,11 @@ namespace {
 
 constexpr int kTile = 128;                 // rows of a tile, keys of a unit
 constexpr int kRows = 2 * kTile;
-constexpr int kThreads = 512;              // four warpgroups: tile 0, tile 1, copies, MMA (and three idle warps)
+constexpr int kThreads = 512;              // four warpgroups: tile 0, tile 1, copies, MMA and walk (and two idle warps)
+constexpr int kExtra = 2;                  // units that an item costs beside its own
 constexpr int kHalf = kTile * 128;         // bytes of 64 columns of a tile: 128 rows of 128 bytes, swizzled
-constexpr int kLag = 2;                    // stages whose copies are in flight behind the newest
+constexpr int kLag = 2;                    // stages whose row copies are in flight behind the newest
+constexpr int kBoxSlots = 32;              // slots of a page per TMA box, at most
 
 template <int DP>
 struct Smem {
@@ -36,14 +40,19 @@ struct Smem {
 };
 
 // Registers per thread after the split; the sum over the four warpgroups is that of the launch, 4 * 128.
-constexpr int kRegsSoftmax = 184, kRegsCopy = 88, kRegsMma = 56;
-static_assert(2 * kRegsSoftmax + kRegsCopy + kRegsMma <= 4 * 128, "register split above the launch's registers");
+constexpr int kRegsRows = 152, kRegsCopy = 104, kRegsMma = 104;
+static_assert(2 * kRegsRows + kRegsCopy + kRegsMma <= 4 * 128, "register split above the launch's registers");
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, int bytes) {   // the rest of the 16 is zero
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void st_shared16(uint32_t dst, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ uint4 ld_shared16(uint32_t src) {
+  uint4 x;
+  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(src) : "memory");
+  return x;
 }
 __device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
@@ -66,29 +75,87 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return d;
 }
 
+// One box of a page: columns c0.., slots, head, page.
+__device__ __forceinline__ void tma_load_4d_if(bool lane_does, uint32_t dst, const CUtensorMap *m, uint32_t bar, int c0, int slot, int head,
+                                               int page) {
+  asm volatile(
+      "{.reg .pred p; setp.ne.b32 p, %0, 0;\n\t"
+      "@p cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%1], [%2, {%4, %5, %6, %7}], [%3];}" ::"r"(
+          (uint32_t)lane_does),
+      "r"(dst), "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(c0), "r"(slot), "r"(head), "r"(page)
+      : "memory");
+}
+
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(*reinterpret_cast<unsigned long long *>(&d))
+      : "l"(*reinterpret_cast<const unsigned long long *>(&a)), "l"(*reinterpret_cast<const unsigned long long *>(&b)));
+  return d;
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+
+// 2^x for x below 128 on the multiply-add pipes: 2^n 2^f with n the nearest whole number (which an addition of 1.5 2^23 leaves in
+// the low bits) and a minimax polynomial of degree 4 for 2^f on [-1/2, 1/2], fitted for this file by the exchange algorithm with
+// the relative error as its target: 2.7e-6 (2^-18.5) with fp32 coefficients and arithmetic.  Below 2^-126.5 the result is zero;
+// NaN stays NaN.
+__device__ __forceinline__ float2 exp2_poly2(float2 x) {
+  constexpr float kMagic = 12582912.f + 127.f;    // the low bits become n + 127, the exponent field of 2^n
+  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x.x));   // -127
+  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x.y));
+  const float2 r = add2(x, both(kMagic));
+  const float2 f = add2(x, mul2(add2(r, both(-kMagic)), both(-1.f)));
+  float2 y = fma2(both(0.009570102207362652f), f, both(0.05591785907745361f));
+  y = fma2(y, f, both(0.240247443318367f));
+  y = fma2(y, f, both(0.6931217908859253f));
+  y = fma2(y, f, both(0.9999992847442627f));
+  return mul2(y, make_float2(__uint_as_float(__float_as_uint(r.x) << 23), __uint_as_float(__float_as_uint(r.y) << 23)));
+}
+// Of 16 pairs of exponentials this many go that way, the others to the special-function unit, whose 4 lanes per cycle would
+// otherwise be the longest part of a row's work.
+#ifndef POLY16
+#define POLY16 5
+#endif
+constexpr int kPolyOf16 = POLY16;
+__host__ __device__ constexpr bool by_polynomial(int pair) { return (pair * kPolyOf16) / 16 != ((pair + 1) * kPolyOf16) / 16; }
+
 struct Barriers {
   uint64_t kv_full[8], kv_free[8];
-  uint64_t q_full[2], s_full[2], p_full[2], o_full[2];
+  uint64_t q_full[2], s_full[2], p_half[2], p_full[2], o_full[2];
+  uint64_t piece_full[4], piece_free[4];
   uint32_t tmem;
 };
 
-// Units that a tile of a piece works on, from the piece's first.
-template <int UK>
-__device__ __forceinline__ int tile_count(const AttnParams &p, const AttnWalk<kRows, UK> &it, int i) {
+// A piece of an item, as the walk hands it out; b < 0: there are no more.
+struct Piece {
+  SeqInfo seq;
+  int b, tile, head, unit0, n_units, r0, n_rows, first_piece, whole, last_cta;
+  int count[2];      // units that each tile works on, from the piece's first
+
+  __device__ int token(const AttnParams &p, int row) const { return (r0 + row) / p.group; }
+  __device__ int q_head(const AttnParams &p, int row) const { return head * p.group + (r0 + row) % p.group; }
+};
+constexpr int kPieces = 4;             // handed out ahead
+constexpr int kPieceReaders = 13;      // warps
+
+using Walk = AttnWalk<kRows, kTile, kExtra>;
+
+__device__ __forceinline__ int tile_count(const AttnParams &p, const Walk &it, int i) {
   const int rows = it.n_rows - i * kTile;
   if (rows <= 0) return 0;
-  const int last = i * kTile + min(rows, kTile) - 1;
-  const int hi = key_hi(p, it.seq, it.token(p, last));
-  return min(max((hi + UK - 1) / UK - it.unit0, 0), it.n_units);
+  const int hi = key_hi(p, it.seq, it.token(p, i * kTile + min(rows, kTile) - 1));
+  return min(max((hi + kTile - 1) / kTile - it.unit0, 0), it.n_units);
 }
 
 template <typename T, bool E4M3, int DP>
-__global__ void __launch_bounds__(kThreads, 1) attention_tcgen05_kernel(const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(kThreads, 1) attention_tcgen05_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUtensorMap k_map,
+                                                                        const __grid_constant__ CUtensorMap v_map, int box) {
   using M = std::conditional_t<E4M3, __half, T>;
   using L = Smem<DP>;
   constexpr int S = L::kStages, CHUNKS = DP / 8;
   extern __shared__ unsigned char smem_raw[];
   __shared__ Barriers bars;
+  __shared__ Piece pieces[kPieces];
   __shared__ long long s_scan[40];
   unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   const uint32_t base = smem_u32(smem);
@@ -96,74 +163,102 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tcgen05_kernel(const __
   if (threadIdx.x == 0) {
     for (int i = 0; i < S; ++i) tc::mbar_init(&bars.kv_full[i], 4), tc::mbar_init(&bars.kv_free[i], 1);
     for (int i = 0; i < 2; ++i) {
-      tc::mbar_init(&bars.q_full[i], 4), tc::mbar_init(&bars.p_full[i], 4);
+      tc::mbar_init(&bars.q_full[i], 4), tc::mbar_init(&bars.p_half[i], 4), tc::mbar_init(&bars.p_full[i], 4);
       tc::mbar_init(&bars.s_full[i], 1), tc::mbar_init(&bars.o_full[i], 1);
     }
+    for (int i = 0; i < kPieces; ++i) tc::mbar_init(&bars.piece_full[i], 1), tc::mbar_init(&bars.piece_free[i], kPieceReaders);
     tc::mbar_fence_init();
   }
   if (warp == 12) tc::tmem_alloc(&bars.tmem, 512);
   grid_launch_dependents();
   grid_dependency_wait();
-  const AttnRange range = attention_range<kRows, kTile, kThreads>(p, 1, reinterpret_cast<int *>(smem), s_scan);
+  const AttnRange range = attention_range<kRows, kTile, kExtra, kThreads>(p, 1, reinterpret_cast<int *>(smem), s_scan);
   zero_tail_rows<T>(p, kThreads);
   if (threadIdx.x == 0) p.meta[blockIdx.x] = make_int4(-1, 0, 0, 0);
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
   const uint32_t tmem = bars.tmem;
-  AttnWalk<kRows, kTile> it(range);
   bool ok = true;
+  uint32_t n_piece = 0;        // pieces taken
+  auto take = [&]() -> const Piece * {     // the next piece, or null (at the end, and with ok unset after a wait that gave up)
+    const uint32_t i = n_piece % kPieces;
+    if (!(ok = tc::warp_wait(smem_u32(&bars.piece_full[i]), (n_piece / kPieces) & 1))) return nullptr;
+    ++n_piece;
+    return pieces[i].b >= 0 ? &pieces[i] : nullptr;
+  };
+  auto give_back = [&]() {                 // of the last piece taken
+    __syncwarp();
+    tc::arrive_if(lane == 0, smem_u32(&bars.piece_free[(n_piece - 1) % kPieces]));
+  };
 
   if (warp < 8) {
     // ---- a tile's rows -----------------------------------------------------------------------------------------
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsRows));
     const int i = warp >> 2, row = threadIdx.x & (kTile - 1);     // tile, row of it (= lane of tensor memory)
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_tmem = tmem + i * kTile + lanes, o_tmem = tmem + 2 * kTile + i * kTile + lanes;
+    const uint32_t s_tmem = tmem + i * kTile + lanes, p_tmem = s_tmem + kTile / 2, o_tmem = tmem + 2 * kTile + i * kTile + lanes;
     const uint32_t s_full = smem_u32(&bars.s_full[i]), o_full = smem_u32(&bars.o_full[i]);
-    const uint32_t q_full = smem_u32(&bars.q_full[i]), p_full = smem_u32(&bars.p_full[i]);
+    const uint32_t q_full = smem_u32(&bars.q_full[i]), p_full = smem_u32(&bars.p_full[i]),
+                   p_half = smem_u32(&bars.p_half[i]);
     uint32_t n_s = 0, n_o = 0;     // phases of s_full and o_full so far
 
-    auto load_query = [&]() -> float {   // this thread's row of the piece to shared memory; returns the factor of its scores
-      const bool live = i * kTile + row < it.n_rows;
-      const int r = live ? i * kTile + row : 0;
-      const char *src = reinterpret_cast<const char *>(p.q) + ((it.seq.q0 + it.token(p, r)) * p.q_st + it.q_head(p, r) * p.q_sh) * 2;
-      const uint32_t dst = base + i * L::kTileBytes;
+    // Rows of queries come in, and rows of the output go out, 16 lanes (8 for heads of up to 64) to a row, so that a warp's access
+    // covers whole lines; the tile of shared memory that held the queries takes the output rows in between.
+    constexpr int RP = 32 / CHUNKS, PASSES = 32 / RP;    // rows per pass of the warp
+    const int c = lane % CHUNKS, sub = lane / CHUNKS;
+    const uint32_t tile = base + i * L::kTileBytes;
+    const int row0 = (warp & 3) * 32;                             // first row of the warp
+    auto row_of = [&](int64_t mine, int pass) -> int64_t {        // lane's value of the row that this lane works on
+      return __shfl_sync(0xffffffffu, mine, pass * RP + sub);
+    };
+
+    auto load_query = [&](const Piece &it) -> float {   // the piece's rows to shared memory; returns the factor of this row's scores
+      const int r = i * kTile + row;
+      const int64_t at = r < it.n_rows ? (it.seq.q0 + it.token(p, r)) * p.q_st + it.q_head(p, r) * p.q_sh : -1;
+      const char *src = reinterpret_cast<const char *>(p.q);
       float mul = p.scale_log2;
       if constexpr (!E4M3) {
 #pragma unroll
-        for (int c = 0; c < CHUNKS; ++c) {
-          const uint4 x = live && c * 8 < p.d ? *reinterpret_cast<const uint4 *>(src + c * 16) : make_uint4(0, 0, 0, 0);
-          st_shared16(dst + tile_at(row, c), x.x, x.y, x.z, x.w);
+        for (int q = 0; q < PASSES; ++q) {
+          const int64_t o = row_of(at, q);
+          const bool in = o >= 0 && c * 8 < p.d;
+          cp_async16(tile + tile_at(row0 + q * RP + sub, c), in ? src + (o + c * 8) * 2 : src, in ? 16 : 0);
         }
+        asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
       } else {
-        float top = 0.f;
-        uint4 x[CHUNKS];
+        const float k_scale = p.k_scale[it.head];
+        uint4 x[PASSES];
+        int my_ex = 0;
 #pragma unroll
-        for (int c = 0; c < CHUNKS; ++c) {
-          x[c] = live && c * 8 < p.d ? *reinterpret_cast<const uint4 *>(src + c * 16) : make_uint4(0, 0, 0, 0);
-          const uint32_t w[4] = {x[c].x, x[c].y, x[c].z, x[c].w};
+        for (int q = 0; q < PASSES; ++q) {
+          const int64_t o = row_of(at, q);
+          x[q] = o >= 0 && c * 8 < p.d ? *reinterpret_cast<const uint4 *>(src + (o + c * 8) * 2) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int q = 0; q < PASSES; ++q) {
+          const uint32_t w[4] = {x[q].x, x[q].y, x[q].z, x[q].w};
+          float top = 0.f;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const float2 f = unpack2(w[e], T(0.f));
             top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
           }
-        }
-        const float k_scale = p.k_scale[it.head];
-        const int ex = row_exponent(top);
-        const float down = copysignf(ldexpf(1.f, -ex), k_scale);
 #pragma unroll
-        for (int c = 0; c < CHUNKS; ++c) {
-          const uint32_t w[4] = {x[c].x, x[c].y, x[c].z, x[c].w};
+          for (int m = 1; m < CHUNKS; m *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
+          const int ex = row_exponent(top);
+          const float down = copysignf(ldexpf(1.f, -ex), k_scale);
           uint32_t h[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const float2 f = unpack2(w[e], T(0.f));
             h[e] = pack2(f.x * down, f.y * down, M(0.f));
           }
-          st_shared16(dst + tile_at(row, c), h[0], h[1], h[2], h[3]);
+          st_shared16(tile + tile_at(row0 + q * RP + sub, c), h[0], h[1], h[2], h[3]);
+          const int mine = __shfl_sync(0xffffffffu, ex, lane % RP * CHUNKS);
+          if (lane / RP == q) my_ex = mine;
         }
-        mul *= fabsf(k_scale) * ldexpf(1.f, ex);
+        mul *= fabsf(k_scale) * ldexpf(1.f, my_ex);
       }
       fence_async_proxy();
       __syncwarp();
@@ -171,52 +266,63 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tcgen05_kernel(const __
       return fmaxf(mul, 1e-30f);    // a scale of zero: masked scores stay minus infinity
     };
 
-    bool has = it.next(p);
-    int count = has ? tile_count(p, it, i) : 0;
+    const Piece *it = take();
     float mul = 0.f;
-    if (count > 0) mul = load_query();
-    while (has && ok) {
-      const int rows = min(max(it.n_rows - i * kTile, 0), kTile);
+    if (it && it->count[i] > 0) mul = load_query(*it);
+    while (it) {
+      const int rows = min(max(it->n_rows - i * kTile, 0), kTile), count = it->count[i], unit0 = it->unit0;
       const bool live = row < rows;
       int lo = 0, hi = 0, all_lo = 0, all_hi = 0;      // keys that this row sees; that every row of the tile sees
       if (rows > 0) {
-        const int tok = it.token(p, i * kTile + (live ? row : 0));
-        lo = key_lo(p, it.seq, tok), hi = live ? key_hi(p, it.seq, tok) : 0;
-        all_lo = key_lo(p, it.seq, it.token(p, i * kTile + rows - 1)), all_hi = key_hi(p, it.seq, it.token(p, i * kTile));
+        const int tok = it->token(p, i * kTile + (live ? row : 0));
+        lo = key_lo(p, it->seq, tok), hi = live ? key_hi(p, it->seq, tok) : 0;
+        all_lo = key_lo(p, it->seq, it->token(p, i * kTile + rows - 1)), all_hi = key_hi(p, it->seq, it->token(p, i * kTile));
       }
       float ref = -INFINITY, sum = 0.f;
       for (int j = 0; j < count; ++j) {
-        const int key0 = (it.unit0 + j) * kTile;
+        const int key0 = (unit0 + j) * kTile;
         if (!(ok = tc::warp_wait(s_full, n_s & 1))) break;
         ++n_s;
         tc::fence_after_sync();
-        uint32_t s[4][32];
+        // Two passes over the row in pieces of 32 scores: its maximum, then the exponentials.  The last 64 scores stay in registers
+        // in between and go first; their columns take the probabilities of all, so the others can be read again.
+        const bool masked = key0 < all_lo || key0 + kTile > all_hi;
+        auto mask = [&](uint32_t (&x)[32], int c) {
+          const int f = lo - key0 - 32 * c, t = hi - key0 - 32 * c;
+          const uint32_t seen = (t <= 0 ? 0u : t >= 32 ? ~0u : (1u << t) - 1) & (f <= 0 ? ~0u : f >= 32 ? 0u : ~0u << f);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) tc::tmem_ld_32x32b_x32(s_tmem + 32 * c, s[c]);
+          for (int e = 0; e < 32; ++e)
+            if (!(seen >> e & 1)) x[e] = 0xff800000u;
+        };
+        float best[2] = {-INFINITY, -INFINITY};
+        auto maximum = [&](const uint32_t (&x)[32]) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) {
+            best[0] = fmaxf(fmaxf(best[0], __uint_as_float(x[e])), __uint_as_float(x[e + 1]));
+            best[1] = fmaxf(fmaxf(best[1], __uint_as_float(x[e + 2])), __uint_as_float(x[e + 3]));
+          }
+        };
+        uint32_t x[2][32];
+        tc::tmem_ld_32x32b_x32(s_tmem, x[0]);
+        tc::tmem_ld_32x32b_x32(s_tmem + 32, x[1]);
         tc::tmem_ld_wait();
-        if (key0 < all_lo || key0 + kTile > all_hi) {
-          const int from = lo - key0, to = hi - key0;
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (32 * c + e < from || 32 * c + e >= to) s[c][e] = 0xff800000u;
-        }
-        float mx[4];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          mx[c] = fmaxf(__uint_as_float(s[c][0]), __uint_as_float(s[c][1]));
-#pragma unroll
-          for (int e = 2; e < 32; e += 2) mx[c] = fmaxf(fmaxf(mx[c], __uint_as_float(s[c][e])), __uint_as_float(s[c][e + 1]));
-        }
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * mul;
+        if (masked) mask(x[0], 0), mask(x[1], 1);
+        maximum(x[0]);
+        maximum(x[1]);
+        tc::tmem_ld_32x32b_x32(s_tmem + 64, x[0]);
+        tc::tmem_ld_32x32b_x32(s_tmem + 96, x[1]);
+        tc::tmem_ld_wait();
+        if (masked) mask(x[0], 2), mask(x[1], 3);
+        maximum(x[0]);
+        maximum(x[1]);
+        const float top = fmaxf(best[0], best[1]) * mul;
         if (j == 0) {
           ref = top;
         } else if (__any_sync(0xffffffffu, top > ref + kLazyRescale)) {
           const float to = fmaxf(ref, top), f = ref == -INFINITY ? 0.f : exp2_fast(ref - to);
           if (!(ok = tc::warp_wait(o_full, (n_o - 1) & 1))) break;      // the products so far are in O
           tc::fence_after_sync();
-#pragma unroll
+#pragma unroll 1
           for (int c = 0; c < DP; c += 16) {
             uint32_t o[16];
             tc::tmem_ld_32x32b_x16(o_tmem + c, o);
@@ -228,78 +334,102 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tcgen05_kernel(const __
           sum *= f;
           ref = to;
         }
-        const float neg = ref == -INFINITY ? 0.f : -ref;
-        const float2 mul2 = make_float2(mul, mul), neg2 = make_float2(neg, neg);
+        const float2 mul_2 = both(mul), neg_2 = both(ref == -INFINITY ? 0.f : -ref);
         float2 part[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        auto probabilities = [&](const uint32_t (&s)[32], int c) {
           uint32_t pk[16];
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
-            float2 x = fma2(make_float2(__uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1])), mul2, neg2);
-            x.x = exp2_fast(x.x), x.y = exp2_fast(x.y);
-            part[(e >> 1) & 1] = add2(part[(e >> 1) & 1], x);
-            pk[e / 2] = pack2(x.x, x.y, M(0.f));
+            float2 y = fma2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), mul_2, neg_2);
+            if (by_polynomial(e / 2)) y = exp2_poly2(y);
+            else y.x = exp2_fast(y.x), y.y = exp2_fast(y.y);
+            part[(e >> 1) & 1] = add2(part[(e >> 1) & 1], y);
+            pk[e / 2] = pack2(y.x, y.y, M(0.f));
           }
-          tc::tmem_st_32x32b_x16(s_tmem + 16 * c, pk);
-        }
-        const float2 both = add2(part[0], part[1]);
-        sum += both.x + both.y;
-        tc::tmem_st_wait();
-        tc::fence_before_sync();
-        __syncwarp();
-        tc::arrive_if(lane == 0, p_full);
+          tc::tmem_st_32x32b_x16(p_tmem + 16 * c, pk);
+        };
+        auto ready = [&](uint32_t bar) {      // the product of 64 keys begins while the others are in their exponentials
+          tc::tmem_st_wait();
+          tc::fence_before_sync();
+          __syncwarp();
+          tc::arrive_if(lane == 0, bar);
+        };
+        probabilities(x[0], 2);
+        tc::tmem_ld_32x32b_x32(s_tmem, x[0]);
+        probabilities(x[1], 3);
+        tc::tmem_ld_32x32b_x32(s_tmem + 32, x[1]);
+        ready(p_half);
+        tc::tmem_ld_wait();
+        if (masked) mask(x[0], 0), mask(x[1], 1);
+        probabilities(x[0], 0);
+        probabilities(x[1], 1);
+        ready(p_full);
+        part[0] = add2(part[0], part[1]);
+        sum += part[0].x + part[0].y;
         ++n_o;
       }
       if (!ok) break;
-      // what the output needs, before the walk moves on; the next query rows go ahead of the wait for the last product
-      const bool whole = it.whole;
-      const int head = it.head, done = count;
-      const int64_t slot_row = (int64_t)(2 * blockIdx.x + (it.first_piece ? 1 : 0)) * kRows + i * kTile + row;
-      char *out = nullptr;
+      const bool whole = it->whole;
+      const float v_scale = E4M3 ? p.v_scale[it->head] : 1.f;
+      const int slot = 2 * blockIdx.x + (it->first_piece ? 1 : 0);
+      int64_t out_at = -1;
       if (live) {
         const int r = i * kTile + row;
-        out = reinterpret_cast<char *>(p.out) + ((it.seq.q0 + it.token(p, r)) * p.o_st + it.q_head(p, r) * p.o_sh) * 2;
+        out_at = (it->seq.q0 + it->token(p, r)) * p.o_st + it->q_head(p, r) * p.o_sh;
       }
-      if (threadIdx.x == 0 && !whole && it.first_piece) p.meta[blockIdx.x] = make_int4(it.b, it.tile, head, it.last_cta);
-      has = it.next(p);
-      count = has ? tile_count(p, it, i) : 0;
-      if (count > 0) mul = load_query();
-      if (done > 0) {
+      if (threadIdx.x == 0 && !whole && it->first_piece) p.meta[blockIdx.x] = make_int4(it->b, it->tile, it->head, it->last_cta);
+      give_back();
+      if (count > 0) {
         if (!(ok = tc::warp_wait(o_full, (n_o - 1) & 1))) break;
         tc::fence_after_sync();
       }
-      const float v_scale = E4M3 ? p.v_scale[head] : 1.f;
-      const float f = !whole ? v_scale : sum == 0.f ? 0.f : v_scale / sum;
+      if (rows > 0) {
+        const float f = !whole ? v_scale : sum == 0.f ? 0.f : v_scale / sum;
 #pragma unroll 1
-      for (int c = 0; c < p.d; c += 32) {
-        uint32_t o[32];
-        if (done > 0) {
-          tc::tmem_ld_32x32b_x32(o_tmem + c, o);
-          tc::tmem_ld_wait();
-        } else {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = 0;
-        }
-        if (!live) continue;
-#pragma unroll
-        for (int e = 0; e < 32; e += 8) {
-          if (c + e >= p.d) break;
-          float x[8];
-#pragma unroll
-          for (int q = 0; q < 8; ++q) x[q] = __uint_as_float(o[e + q]) * f;
-          if (whole) {
-            *reinterpret_cast<uint4 *>(out + (c + e) * 2) =
-                make_uint4(pack2(x[0], x[1], T(0.f)), pack2(x[2], x[3], T(0.f)), pack2(x[4], x[5], T(0.f)), pack2(x[6], x[7], T(0.f)));
+        for (int col = 0; col < p.d; col += 32) {
+          uint32_t o[32];
+          if (count > 0) {
+            tc::tmem_ld_32x32b_x32(o_tmem + col, o);
+            tc::tmem_ld_wait();
           } else {
-            float4 *dst = reinterpret_cast<float4 *>(p.part_o + slot_row * DP + c + e);
-            dst[0] = make_float4(x[0], x[1], x[2], x[3]), dst[1] = make_float4(x[4], x[5], x[6], x[7]);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = 0;
+          }
+          if (whole) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 8) {
+              uint32_t h[4];
+#pragma unroll
+              for (int q = 0; q < 4; ++q)
+                h[q] = pack2(__uint_as_float(o[e + 2 * q]) * f, __uint_as_float(o[e + 2 * q + 1]) * f, T(0.f));
+              if (col + e < DP) st_shared16(tile + tile_at(row, (col + e) / 8), h[0], h[1], h[2], h[3]);
+            }
+          } else if (live) {     // [slot][column / 4][row] in units of four columns: a warp's rows are neighbours
+            float4 *dst = reinterpret_cast<float4 *>(p.part_o) + ((int64_t)slot * (DP / 4) + col / 4) * kRows + i * kTile + row;
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              if (col + e < DP)
+                dst[(e / 4) * kRows] = make_float4(__uint_as_float(o[e]) * f, __uint_as_float(o[e + 1]) * f,
+                                                   __uint_as_float(o[e + 2]) * f, __uint_as_float(o[e + 3]) * f);
           }
         }
+        if (whole) {
+          __syncwarp();
+#pragma unroll
+          for (int q = 0; q < PASSES; ++q) {
+            const int64_t o = row_of(out_at, q);
+            if (o >= 0 && c * 8 < p.d)
+              *reinterpret_cast<uint4 *>(reinterpret_cast<char *>(p.out) + (o + c * 8) * 2) = ld_shared16(tile + tile_at(row0 + q * RP + sub, c));
+          }
+          __syncwarp();     // the rows are read before the next queries come
+        } else if (live) {  // (a NaN outweighs the other pieces' rows)
+          p.part_ml[(int64_t)slot * kRows + i * kTile + row] = make_float2(sum != sum ? INFINITY : sum == 0.f ? -INFINITY : ref, sum);
+        }
       }
-      // (a NaN outweighs the other pieces' rows)
-      if (live && !whole) p.part_ml[slot_row] = make_float2(sum != sum ? INFINITY : sum == 0.f ? -INFINITY : ref, sum);
       tc::fence_before_sync();   // O is read before the next piece's first product, which waits for this warp's probabilities
+      it = take();
+      if (!ok) break;
+      if (it && it->count[i] > 0) mul = load_query(*it);
     }
     if (!ok && lane == 0) tc::report_timeout(p.status, kStatusEpilogueTimeout);
   } else if (warp < 12) {
@@ -312,15 +442,24 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tcgen05_kernel(const __
     constexpr int PASSES = 32 / RP;
     const int c = lane % CH, sub = lane / CH;
     const int bytes = min(max(p.d * ES - c * 16, 0), 16);
-    uint32_t n = 0;                           // stages begun
-    while (ok && it.next(p)) {
-      const int units = max(tile_count(p, it, 0), tile_count(p, it, 1));
+    uint32_t n = 0, pending = 0;              // stages begun; which of the last have row copies that were not reported yet
+    auto arrived = [&](uint32_t k) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kLag) : "memory");
+      fence_async_proxy();
+      __syncwarp();
+      tc::arrive_if(lane == 0, smem_u32(&bars.kv_full[k % S]));
+      pending &= ~(1u << (k & 31));
+    };
+    while (const Piece *piece = take()) {
+      const Piece &it = *piece;
+      const int units = max(it.count[0], it.count[1]), head = it.head;
       const int k_begin = max(key_lo(p, it.seq, it.token(p, 0)), it.unit0 * kTile);
       const int k_end = min((long long)key_hi(p, it.seq, it.token(p, it.n_rows - 1)), ((long long)it.unit0 + it.n_units) * kTile);
-      const char *kb = reinterpret_cast<const char *>(p.k) + it.head * p.k_sh * ES;
-      const char *vb = reinterpret_cast<const char *>(p.v) + it.head * p.v_sh * ES;
+      const char *kb = reinterpret_cast<const char *>(p.k) + head * p.k_sh * ES;
+      const char *vb = reinterpret_cast<const char *>(p.v) + head * p.v_sh * ES;
       const int32_t *pages = p.table + it.b * p.table_stride;
       const int first = it.unit0 * kTile + w4 * 32 + lane;            // this lane's key of the piece's first unit
+      give_back();
       auto page_id = [&](int j) -> int {
         const int key = first + j * kTile;
         if (j >= units || key < k_begin || key >= k_end) return -1;
@@ -329,9 +468,20 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tcgen05_kernel(const __
         tc::report_timeout(p.status, kStatusBadIndex);
         return -1;
       };
+      auto slot_of = [&](int key) { return key - page_of(p, key) * p.page; };
+      uint4 xk[E4M3 ? PASSES : 1], xv[E4M3 ? PASSES : 1];      // e4m3: 16 bytes of PASSES rows, in flight
+      auto fetch = [&](uint4 (&x)[E4M3 ? PASSES : 1], const char *src, int64_t sp, int64_t ss, int id, int slot) {
+#pragma unroll
+        for (int q = 0; q < (E4M3 ? PASSES : 1); ++q) {
+          const int r = q * RP + sub;
+          const int rid = __shfl_sync(0xffffffffu, id, r), rslot = __shfl_sync(0xffffffffu, slot, r);
+          x[q] = rid >= 0 && bytes > 0 ? *reinterpret_cast<const uint4 *>(src + rid * sp + rslot * ss + c * 16) : make_uint4(0, 0, 0, 0);
+        }
+      };
       int ahead = page_id(0);
+      if (E4M3 && units > 0) fetch(xk, kb, p.k_sp, p.k_ss, ahead, slot_of(first));
       for (int j = 0; j < units && ok; ++j) {
-        const int id = ahead, key = first + j * kTile, slot = key - page_of(p, key) * p.page;
+        const int id = ahead, key = first + j * kTile, slot = slot_of(key);
         ahead = page_id(j + 1);
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
@@ -340,37 +490,43 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tcgen05_kernel(const __
           const char *src = kv ? vb : kb;
           const int64_t sp = kv ? p.v_sp : p.k_sp, ss = kv ? p.v_ss : p.k_ss;
           if constexpr (!E4M3) {
-            if (n >= S && !(ok = tc::warp_wait_idle(smem_u32(&bars.kv_free[st]), (n / S - 1) & 1))) break;
+            if (n >= S && !(ok = tc::warp_wait(smem_u32(&bars.kv_free[st]), (n / S - 1) & 1))) break;
+            const uint32_t full = smem_u32(&bars.kv_full[st]);
+            if (box > 0 && __all_sync(0xffffffffu, id >= 0)) {
+              // lane l of the first (boxes x halves): box l / halves of this warp's 32 keys, 64 columns of it
+              constexpr int HALVES = DP / 64;
+              const int b_i = lane / HALVES, half = lane % HALVES;
+              const int bid = __shfl_sync(0xffffffffu, id, b_i * box & 31), bslot = __shfl_sync(0xffffffffu, slot, b_i * box & 31);
+              tc::expect_tx_if(lane == 0, full, 32 * DP * 2);
+              __syncwarp();
+              tma_load_4d_if(b_i * box < 32, dst + half * kHalf + (w4 * 32 + b_i * box) * 128, kv ? &v_map : &k_map, full, half * 64, bslot,
+                             head, bid);
+            } else {
 #pragma unroll
-            for (int q = 0; q < PASSES; ++q) {
-              const int r = q * RP + sub;
-              const int rid = __shfl_sync(0xffffffffu, id, r), rslot = __shfl_sync(0xffffffffu, slot, r);
-              const bool live = rid >= 0 && bytes > 0;
-              cp_async16(dst + tile_at(w4 * 32 + r, c), live ? src + (rid * sp + rslot * ss) * ES + c * 16 : src, live ? bytes : 0);
+              for (int q = 0; q < PASSES; ++q) {
+                const int r = q * RP + sub;
+                const int rid = __shfl_sync(0xffffffffu, id, r), rslot = __shfl_sync(0xffffffffu, slot, r);
+                const bool live = rid >= 0 && bytes > 0;
+                cp_async16(dst + tile_at(w4 * 32 + r, c), live ? src + (rid * sp + rslot * ss) * ES + c * 16 : src, live ? bytes : 0);
+              }
+              pending |= 1u << (n & 31);
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
-            if (n >= kLag) {     // the stage kLag behind this one has arrived
-              asm volatile("cp.async.wait_group %0;" ::"n"(kLag) : "memory");
-              fence_async_proxy();
-              __syncwarp();
-              tc::arrive_if(lane == 0, smem_u32(&bars.kv_full[(n - kLag) % S]));
-            }
+            // the row copies of the stage kLag behind this one have arrived
+            if (n >= kLag && (pending >> ((n - kLag) & 31) & 1)) arrived(n - kLag);
           } else {
-            uint4 x[PASSES];     // 16 bytes of PASSES rows, in flight while the ring's slot drains
-#pragma unroll
-            for (int q = 0; q < PASSES; ++q) {
-              const int r = q * RP + sub;
-              const int rid = __shfl_sync(0xffffffffu, id, r), rslot = __shfl_sync(0xffffffffu, slot, r);
-              x[q] = rid >= 0 && bytes > 0 ? *reinterpret_cast<const uint4 *>(src + rid * sp + rslot * ss + c * 16) : make_uint4(0, 0, 0, 0);
-            }
-            if (n >= S && !(ok = tc::warp_wait_idle(smem_u32(&bars.kv_free[st]), (n / S - 1) & 1))) break;
+            // the rows of the stage after this one go out before this one is converted
+            if (kv == 0) fetch(xv, vb, p.v_sp, p.v_ss, id, slot);
+            else if (j + 1 < units) fetch(xk, kb, p.k_sp, p.k_ss, ahead, slot_of(key + kTile));
+            if (n >= S && !(ok = tc::warp_wait(smem_u32(&bars.kv_free[st]), (n / S - 1) & 1))) break;
 #pragma unroll
             for (int q = 0; q < PASSES; ++q) {
               const int r = w4 * 32 + q * RP + sub;
-              st_shared16(dst + tile_at(r, 2 * c), e4m3x2_to_f16x2(x[q].x), e4m3x2_to_f16x2(x[q].x >> 16), e4m3x2_to_f16x2(x[q].y),
-                          e4m3x2_to_f16x2(x[q].y >> 16));
-              st_shared16(dst + tile_at(r, 2 * c + 1), e4m3x2_to_f16x2(x[q].z), e4m3x2_to_f16x2(x[q].z >> 16), e4m3x2_to_f16x2(x[q].w),
-                          e4m3x2_to_f16x2(x[q].w >> 16));
+              const uint4 x = kv ? xv[q] : xk[q];
+              st_shared16(dst + tile_at(r, 2 * c), e4m3x2_to_f16x2(x.x), e4m3x2_to_f16x2(x.x >> 16), e4m3x2_to_f16x2(x.y),
+                          e4m3x2_to_f16x2(x.y >> 16));
+              st_shared16(dst + tile_at(r, 2 * c + 1), e4m3x2_to_f16x2(x.z), e4m3x2_to_f16x2(x.z >> 16), e4m3x2_to_f16x2(x.w),
+                          e4m3x2_to_f16x2(x.w >> 16));
             }
             fence_async_proxy();
             __syncwarp();
@@ -379,13 +535,12 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tcgen05_kernel(const __
           ++n;
         }
       }
+      if (!ok) break;
     }
     if constexpr (!E4M3) {
       asm volatile("cp.async.wait_group 0;" ::: "memory");
-      fence_async_proxy();
-      __syncwarp();
-      if (ok)
-        for (uint32_t s = n > kLag ? n - kLag : 0; s < n; ++s) tc::arrive_if(lane == 0, smem_u32(&bars.kv_full[s % S]));
+      for (uint32_t k = n > kLag ? n - kLag : 0; ok && k < n; ++k)
+        if (pending >> (k & 31) & 1) arrived(k);
     }
     if (!ok && lane == 0) tc::report_timeout(p.status, kStatusProducerTimeout);
   } else {
@@ -412,14 +567,14 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tcgen05_kernel(const __
         }
         __syncwarp();
       };
-      auto outputs = [&](int i, uint32_t k, bool more) {    // O_i (+)= P_i V
-        const uint32_t b = tc::desc_lo_mn_sw128(stage(k), kHalf);
+      auto outputs = [&](int i, uint32_t k, int half, bool more, bool last) {    // O_i (+)= P_i V, 64 of the keys
+        const uint32_t b = tc::desc_lo_mn_sw128(stage(k), kHalf) + half * (64 * 128 >> 4);
         if (leader) {
 #pragma unroll
-          for (int s = 0; s < kTile / 16; ++s)
-            tc::mma_f16_ts(tmem + (2 + i) * kTile, tmem + i * kTile + s * 8,
+          for (int s = 0; s < 4; ++s)
+            tc::mma_f16_ts(tmem + (2 + i) * kTile, tmem + i * kTile + kTile / 2 + half * 32 + s * 8,
                            tc::smem_desc_from_words(b + s * (16 * 128 >> 4), tc::kDescHiSw128), i_pv, more || s > 0);
-          tc::mma_commit(&bars.o_full[i]);
+          if (last) tc::mma_commit(&bars.o_full[i]);
         }
         __syncwarp();
       };
@@ -427,12 +582,13 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tcgen05_kernel(const __
         if (leader) tc::mma_commit(&bars.kv_free[k % S]);
         __syncwarp();
       };
-      while (ok && it.next(p)) {
-        const int count[2] = {tile_count(p, it, 0), tile_count(p, it, 1)};
-        const int units = max(count[0], count[1]);
+      while (const Piece *piece = take()) {
+        const int count[2] = {piece->count[0], piece->count[1]}, units = max(count[0], count[1]);
+        give_back();
         for (int i = 0; i < 2 && ok; ++i)
           if (count[i] > 0) ok = tc::warp_wait(smem_u32(&bars.q_full[i]), n_q[i]++ & 1);
-        if (!ok || units == 0) continue;
+        if (!ok) break;
+        if (units == 0) continue;
         if (!(ok = full(n))) break;
         tc::fence_after_sync();
         for (int i = 0; i < 2; ++i)
@@ -446,9 +602,12 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tcgen05_kernel(const __
           bool have_k = false;
           for (int i = 0; i < 2; ++i) {
             if (j < count[i]) {
+              if (!(ok = tc::warp_wait(smem_u32(&bars.p_half[i]), n_p[i] & 1))) break;
+              tc::fence_after_sync();
+              outputs(i, v, 1, j > 0, false);
               if (!(ok = tc::warp_wait(smem_u32(&bars.p_full[i]), n_p[i]++ & 1))) break;
               tc::fence_after_sync();
-              outputs(i, v, j > 0);
+              outputs(i, v, 0, true, true);
             }
             if (j + 1 < count[i]) {
               if (!have_k && !(ok = full(k))) break;
@@ -461,11 +620,30 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tcgen05_kernel(const __
           release(v);
           if (more) release(k);
         }
+        if (!ok) break;
         n += 2 * units;
       }
       // the last arrival that the tensor core owes this CTA
       if (ok && n > 0) ok = tc::warp_wait(smem_u32(&bars.kv_free[(n - 1) % S]), ((n - 1) / S) & 1);
       if (!ok && lane == 0) tc::report_timeout(p.status, kStatusMmaTimeout);
+    } else if (warp == 13) {
+      // ---- the walk -----------------------------------------------------------------------------------------------
+      Walk it(range);
+      for (bool more = true; more && ok;) {
+        more = it.next(p);
+        const uint32_t i = n_piece % kPieces;
+        if (n_piece >= kPieces && !(ok = tc::warp_wait(smem_u32(&bars.piece_free[i]), (n_piece / kPieces - 1) & 1))) break;
+        if (lane == 0) {
+          Piece &q = pieces[i];
+          q.seq = it.seq, q.b = more ? it.b : -1, q.tile = it.tile, q.head = it.head, q.unit0 = it.unit0, q.n_units = it.n_units;
+          q.r0 = it.r0, q.n_rows = it.n_rows, q.first_piece = it.first_piece, q.whole = it.whole;
+          if (more) q.last_cta = it.last_cta(), q.count[0] = tile_count(p, it, 0), q.count[1] = tile_count(p, it, 1);
+        }
+        __syncwarp();
+        tc::arrive_if(lane == 0, smem_u32(&bars.piece_full[i]));
+        ++n_piece;
+      }
+      if (!ok && lane == 0) tc::report_timeout(p.status, kStatusProducerTimeout);
     }
   }
   // every product has been waited for by the rows that read it; tensor memory goes back
@@ -477,22 +655,36 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tcgen05_kernel(const __
   }
 }
 
+// The cache as a tensor (column, slot, head, page) with a box of 64 columns of `box` slots.  Strides that a tensor map cannot
+// hold (none, or of 2^40 bytes) leave the row copies.
+template <typename T>
+bool page_map(CUtensorMap *map, const AttnParams &p, const void *base, const int64_t (&strides)[3], int box) {
+  const uint64_t dims[4] = {(uint64_t)p.d, (uint64_t)p.page, (uint64_t)p.hkv, (uint64_t)p.num_pages};
+  uint64_t bytes[3];
+  for (int i = 0; i < 3; ++i) {
+    if (dims[i + 1] > 1 && (strides[i] <= 0 || strides[i] >= (int64_t)1 << 38)) return false;
+    bytes[i] = dims[i + 1] > 1 ? (uint64_t)strides[i] * 2 : (uint64_t)p.d * 2;    // (of one: never used)
+  }
+  const uint32_t shape[4] = {64, (uint32_t)box, 1, 1};
+  return make_tensor_map(map, base, __is_same(T, __half) ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, dims,
+                         bytes, shape, true) == ZT_SUCCESS;
+}
+
 template <typename T, bool E4M3, int DP>
 int launch(const AttnParams &p, const AttnPlan &plan, cudaStream_t st) {
   constexpr int smem = Smem<DP>::kBytes + 1024;
-  static PerDeviceOnce once, checked;
+  static PerDeviceOnce once;
   auto kern = attention_tcgen05_kernel<T, E4M3, DP>;
-  int rc = allow_dynamic_smem(once, kern, smem);
+  const int rc = allow_dynamic_smem(once, kern, smem);
   if (rc != ZT_SUCCESS) return rc;
-  int dev = 0;
-  ZT_CUDA_OK(cudaGetDevice(&dev));
-  if (!checked.done[dev]) {     // the register split counts on the launch holding 128 per thread
-    cudaFuncAttributes attr;
-    ZT_CUDA_OK(cudaFuncGetAttributes(&attr, kern));
-    ZT_REQUIRE(attr.numRegs >= 128, ZT_UNSUPPORTED, "attention_tcgen05_kernel: built with %d registers, 128 expected", attr.numRegs);
-    checked.done[dev] = true;
+  CUtensorMap k_map{}, v_map{};
+  int box = 0;
+  if (!E4M3 && p.page_shift >= 3 && p.num_pages > 0) {
+    box = p.page < kBoxSlots ? p.page : kBoxSlots;
+    const int64_t ks[3] = {p.k_ss, p.k_sh, p.k_sp}, vs[3] = {p.v_ss, p.v_sh, p.v_sp};
+    if (!page_map<T>(&k_map, p, p.k, ks, box) || !page_map<T>(&v_map, p, p.v, vs, box)) box = 0;
   }
-  ZT_CUDA_OK(launch_overlapped(kern, dim3(plan.grid), dim3(kThreads), (size_t)smem, st, p));
+  ZT_CUDA_OK(launch_overlapped(kern, dim3(plan.grid), dim3(kThreads), (size_t)smem, st, p, k_map, v_map, box));
   return launch_status("attention_tcgen05_kernel");
 }
 
