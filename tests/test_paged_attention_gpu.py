@@ -115,6 +115,14 @@ def test_long_contexts_are_cut_between_ctas(capi, algo, cache):
 
 
 @pytest.mark.parametrize("algo", ALGOS)
+@pytest.mark.parametrize("cache", ["same", "e4m3"])
+def test_sequences_that_see_nothing_between_others(capi, algo, cache):
+    """Many items without any keys after one whose last tile is copied row by row: none may wait for another."""
+    c = make_batch([(3, 50)] + [(2, 0)] * 2000 + [(40, 70)] + [(1, 0)] * 7, 4, 2, 64, 16, BF16, E4M3 if cache == "e4m3" else BF16, seed=25)
+    check(capi, c, algo)
+
+
+@pytest.mark.parametrize("algo", ALGOS)
 def test_many_sequences(capi, algo):
     c = make_batch([(1, 1 + (37 * i) % 211) for i in range(300)], 4, 2, 64, 16, BF16, seed=12)
     check(capi, c, algo)

@@ -20,44 +20,44 @@ __global__ void __launch_bounds__(kCombineWarps * 32) attention_combine_kernel(c
   grid_dependency_wait();
   const int4 item = p.meta[blockIdx.x];
   if (item.x < 0) return;
-  const SeqInfo seq = load_seq(p, item.x);
-  const int r0 = item.y * R, rows = seq.n * p.group;
   const int row = blockIdx.y * kCombineWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (row >= R || r0 + row >= rows) return;
+  if (row >= item.z % 512) return;
   const int first = blockIdx.x, count = item.w - first + 1;
-  auto slot = [&](int i) { return (int64_t)(2 * (first + i) + (i == 0 ? 1 : 0)) * R + row; };
-  float top = -INFINITY;
-  for (int i = lane; i < count; i += 32) top = fmaxf(top, p.part_ml[slot(i)].x);
+  constexpr int V = DP / 32, BATCH = 8;
+  using Vec = std::conditional_t<V == 4, float4, float2>;
+  float acc[V] = {}, sum = 0.f, top = -INFINITY;
+  for (int i = 0; i < count; i += BATCH) {
+    float2 ml[BATCH];
+    Vec x[BATCH];
+    float to = top;
 #pragma unroll
-  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  constexpr int V = DP / 32;
-  float acc[V] = {}, sum = 0.f;
-  for (int base = 0; base < count; base += 32) {
-    float f = 0.f, l = 0.f;
-    if (base + lane < count) {
-      const float2 ml = p.part_ml[slot(base + lane)];
-      f = ml.x == -INFINITY ? 0.f : exp2_fast(ml.x - top);
-      l = ml.y * f;
-    }
-    const int n = min(32, count - base);
-#pragma unroll 4
-    for (int i = 0; i < n; ++i) {
-      const float fi = __shfl_sync(0xffffffffu, f, i);
-      sum += __shfl_sync(0xffffffffu, l, i);
-      const float *src = p.part_o + slot(base + i) * DP + lane * V;
-      if constexpr (V == 4) {
-        const float4 x = *reinterpret_cast<const float4 *>(src);
-        acc[0] = fmaf(fi, x.x, acc[0]), acc[1] = fmaf(fi, x.y, acc[1]), acc[2] = fmaf(fi, x.z, acc[2]), acc[3] = fmaf(fi, x.w, acc[3]);
-      } else {
-        const float2 x = *reinterpret_cast<const float2 *>(src);
-        acc[0] = fmaf(fi, x.x, acc[0]), acc[1] = fmaf(fi, x.y, acc[1]);
+    for (int u = 0; u < BATCH; ++u) {
+      ml[u] = make_float2(-INFINITY, 0.f), x[u] = Vec{};
+      if (i + u < count) {
+        const int64_t at = (int64_t)(2 * (first + i + u) + (i + u == 0 ? 1 : 0)) * R + row;
+        ml[u] = p.part_ml[at];
+        x[u] = *reinterpret_cast<const Vec *>(p.part_o + at * DP + lane * V);
       }
     }
+#pragma unroll
+    for (int u = 0; u < BATCH; ++u) to = fmaxf(to, ml[u].x);
+    const float f_old = top == -INFINITY ? 0.f : exp2_fast(top - to);
+    sum *= f_old;
+#pragma unroll
+    for (int v = 0; v < V; ++v) acc[v] *= f_old;
+#pragma unroll
+    for (int u = 0; u < BATCH; ++u) {
+      const float f = ml[u].x == -INFINITY ? 0.f : exp2_fast(ml[u].x - to);
+      sum += ml[u].y * f;
+#pragma unroll
+      for (int v = 0; v < V; ++v) acc[v] = fmaf(f, reinterpret_cast<const float *>(&x[u])[v], acc[v]);
+    }
+    top = to;
   }
   if (lane * V >= p.d) return;
   const float f = top == -INFINITY ? 0.f : 1.f / sum;
-  const int tok = (r0 + row) / p.group, qh = item.z * p.group + (r0 + row) % p.group;
-  char *dst = reinterpret_cast<char *>(p.out) + ((seq.q0 + tok) * p.o_st + qh * p.o_sh + lane * V) * 2;
+  const int r = item.y + row, tok = r / p.group, qh = item.z / 512 * p.group + r % p.group;
+  char *dst = reinterpret_cast<char *>(p.out) + ((item.x + tok) * p.o_st + qh * p.o_sh + lane * V) * 2;
   if constexpr (V == 4)
     *reinterpret_cast<uint2 *>(dst) = make_uint2(pack2(acc[0] * f, acc[1] * f, T(0.f)), pack2(acc[2] * f, acc[3] * f, T(0.f)));
   else
@@ -71,10 +71,9 @@ __global__ void __launch_bounds__(DP * 2) attention_combine_rows_kernel(const __
   grid_dependency_wait();
   const int4 item = p.meta[blockIdx.x];
   if (item.x < 0) return;
-  const SeqInfo seq = load_seq(p, item.x);
   const int row = blockIdx.y * 32 + (threadIdx.x & 31), c0 = (threadIdx.x >> 5) * 16;
-  const int first = blockIdx.x, count = item.w - first + 1, r = item.y * R + row;
-  if (r >= seq.n * p.group || c0 >= p.d) return;
+  const int first = blockIdx.x, count = item.w - first + 1;
+  if (row >= item.z % 512 || c0 >= p.d) return;
   auto slot = [&](int i) { return (int64_t)(2 * (first + i) + (i == 0 ? 1 : 0)); };
   float acc[16] = {}, sum = 0.f, top = -INFINITY;
   for (int i = 0; i < count; ++i) {
@@ -94,8 +93,8 @@ __global__ void __launch_bounds__(DP * 2) attention_combine_rows_kernel(const __
     }
   }
   const float f = top == -INFINITY ? 0.f : 1.f / sum;
-  const int tok = r / p.group, qh = item.z * p.group + r % p.group;
-  uint4 *dst = reinterpret_cast<uint4 *>(reinterpret_cast<char *>(p.out) + ((seq.q0 + tok) * p.o_st + qh * p.o_sh + c0) * 2);
+  const int r = item.y + row, tok = r / p.group, qh = item.z / 512 * p.group + r % p.group;
+  uint4 *dst = reinterpret_cast<uint4 *>(reinterpret_cast<char *>(p.out) + ((item.x + tok) * p.o_st + qh * p.o_sh + c0) * 2);
 #pragma unroll
   for (int q = 0; q < 2; ++q)
     if (c0 + 8 * q < p.d)
@@ -127,7 +126,11 @@ AttnPlan make_plan(const zt_paged_attention_args_t &a) {
   plan.tcgen05 = a.algo == ZT_ALGO_TCGEN05 || (a.algo == ZT_ALGO_AUTO && rows > kMaxStreamRows);
   plan.dp = a.head_dim <= 64 ? 64 : 128;
   plan.rows = plan.tcgen05 ? 256 : rows <= 16 ? 16 : 32;
-  plan.grid = plan.tcgen05 ? sm_count() : attention_stream_grid();
+  plan.grid = plan.tcgen05 ? sm_count() : attention_stream_grid(plan.rows);
+  plan.few = rows <= 4 * plan.rows;
+  // units of the whole call at most (an item has up to three beside those of its keys)
+  const int64_t unit = plan.tcgen05 ? 128 : 64, tiles = a.tokens * group / plan.rows + a.batch;
+  plan.most_units = (double)tiles * a.kv_heads * (double)((int64_t)a.page_size * a.max_blocks / unit + 4);
   plan.meta_bytes = align256((size_t)plan.grid * sizeof(int4));
   plan.ml_bytes = align256((size_t)2 * plan.grid * plan.rows * sizeof(float2));
   plan.o_bytes = align256((size_t)2 * plan.grid * plan.rows * plan.dp * sizeof(float));
@@ -185,6 +188,7 @@ extern "C" int zt_paged_attention(const zt_paged_attention_args_t *a, void *stre
   ZT_REQUIRE(a->num_pages == 0 || (aligned(a->k_cache, a->k_cache_stride, 3, es) && aligned(a->v_cache, a->v_cache_stride, 3, es)),
              ZT_INVALID_ARGUMENT, "zt_paged_attention: rows of the caches must be 16-byte aligned");
   const AttnPlan plan = make_plan(*a);
+  ZT_REQUIRE(plan.most_units < 2147483648.0, ZT_UNSUPPORTED, "zt_paged_attention: more work than one call can number");
   ZT_REQUIRE(a->workspace && a->workspace_bytes >= plan.total(), ZT_WORKSPACE_TOO_SMALL,
              "zt_paged_attention: workspace of %zu bytes is smaller than the %zu required", a->workspace_bytes, plan.total());
   ZT_REQUIRE((reinterpret_cast<uintptr_t>(a->workspace) & 255) == 0, ZT_INVALID_ARGUMENT,
@@ -204,7 +208,7 @@ extern "C" int zt_paged_attention(const zt_paged_attention_args_t *a, void *stre
   p.page_shift = -1;
   for (int s = 0; s < 31; ++s)
     if (a->page_size == 1 << s) p.page_shift = s;
-  p.causal = a->causal != 0, p.window = a->window, p.scale_log2 = a->scale * 1.4426950408889634f, p.zero_tail = a->zero_tail != 0;
+  p.causal = a->causal != 0, p.window = a->window, p.scale_log2 = a->scale * 1.4426950408889634f, p.zero_tail = a->zero_tail != 0, p.few = plan.few;
   char *ws = reinterpret_cast<char *>(a->workspace);
   p.meta = reinterpret_cast<int4 *>(ws);
   p.part_ml = reinterpret_cast<float2 *>(ws + plan.meta_bytes);

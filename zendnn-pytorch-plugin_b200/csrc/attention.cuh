@@ -34,23 +34,26 @@ struct AttnParams {
   int page, page_shift, max_blocks, num_pages;  // page_shift: log2 of the page size, or -1
   int causal, window;                           // window 0: none
   float scale_log2;                             // softmax scale times log2(e)
+  int few;                                      // no sequence can have more than a few tiles of rows
   int zero_tail;                                // rows behind the last sequence are zeroed
   float *part_o;                                // [2 * grid][R][DP]
   float2 *part_ml;                              // [2 * grid][R]: maximum (log2 units), sum
-  int4 *meta;                                   // [grid]: the item cut at the end of a CTA's range (b, tile, head) and the last CTA of it, or -1
+  int4 *meta;                                   // [grid]: the item cut at the end of a CTA's range: first new token of its sequence
+                                                // or -1, first row, head * 512 + rows, last CTA
   int *status;
 };
 
 struct AttnPlan {         // of one call, on the host
-  bool tcgen05;
+  bool tcgen05, few;
   int rows, dp, grid;     // rows per item, padded head, CTAs
+  double most_units;
   size_t meta_bytes, ml_bytes, o_bytes;
   size_t total() const { return meta_bytes + ml_bytes + o_bytes; }
 };
 
 int attention_stream_launch(const AttnParams &p, const AttnPlan &plan, int dtype, int cache_dtype, cudaStream_t st);
 int attention_tcgen05_launch(const AttnParams &p, const AttnPlan &plan, int dtype, int cache_dtype, cudaStream_t st);
-int attention_stream_grid();
+int attention_stream_grid(int rows);
 
 #ifdef __CUDACC__
 constexpr float kLazyRescale = 8.f;   // log2 units that a running maximum may lag behind before sums are rescaled
@@ -75,6 +78,17 @@ __device__ __forceinline__ SeqInfo load_seq(const AttnParams &p, int b) {
 __device__ __forceinline__ bool lengths_fit(const AttnParams &p, int b) {
   const int q0 = p.cu[b], q1 = p.cu[b + 1], len = p.lens[b];
   return q0 >= 0 && q1 >= q0 && q1 <= p.tokens && len >= 0 && len <= (int64_t)p.max_blocks * p.page;
+}
+
+// The sequence of tile t, from the tiles before each sequence: the last with prefix <= t.
+__device__ __forceinline__ int first_tile_owner(const AttnParams &p, const int *prefix, int t) {
+  int lo = 0, hi = p.batch;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (prefix[mid] <= t) lo = mid;
+    else hi = mid;
+  }
+  return lo;
 }
 
 // Keys [lo, hi) that new token `i` of a sequence sees.
@@ -102,104 +116,103 @@ __device__ __forceinline__ TileUnits tile_units(const AttnParams &p, const SeqIn
   return {lo / UK, (hi + UK - 1) / UK - lo / UK};
 }
 
-// Sum over the block, and the sum over the threads before this one.  `scratch`: 33 long longs of shared memory, free on entry.
+// Sum over the block, and the sum over the threads before this one.  `scratch`: 32 ints of shared memory, free on entry.
 template <int NT>
-__device__ __forceinline__ long long block_scan(long long v, long long *scratch, long long &total) {
+__device__ __forceinline__ int block_scan(int v, int *scratch, int &total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  long long x = v;
+  int x = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long y = __shfl_up_sync(0xffffffffu, x, o);
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
     if (lane >= o) x += y;
   }
   if (lane == 31) scratch[warp] = x;
   __syncthreads();
-  if (warp == 0) {
-    long long w = lane < NT / 32 ? scratch[lane] : 0;
+  int w = lane < NT / 32 ? scratch[lane] : 0, before = 0;      // every warp adds the warps' sums for itself
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long y = __shfl_up_sync(0xffffffffu, w, o);
-      if (lane >= o) w += y;
-    }
-    scratch[lane] = w;
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, w, o);
+    if (lane >= o) w += y;
   }
-  __syncthreads();
-  total = scratch[NT / 32 - 1];
-  const long long before = warp ? scratch[warp - 1] : 0;
-  __syncthreads();
-  return before + x - v;
+  total = __shfl_sync(0xffffffffu, w, NT / 32 - 1);
+  before = __shfl_sync(0xffffffffu, w, warp > 0 ? warp - 1 : 0);
+  return (warp ? before : 0) + x - v;
 }
 
-// Where a CTA's range begins: units [w0, w1) of all, the first of them `offset` units into sequence b, tile `tile` (over its kv
-// heads).  `per` units per CTA.
+// Where a CTA's range begins: units [w0, w1) of all, w0 within the tile whose first unit (over its kv heads) is number `item0`.
+// `per` units per CTA.  The host has checked that all units fit an int.
 struct AttnRange {
-  long long w0, w1, per, item0;   // item0: number of the first unit of (b, tile)
+  int w0, w1, per, item0;
   int b, tile;
 };
+struct AttnScratch {
+  int scan[2][32], found[3];
+};
 
-// Whole-block call.  `prefix`: batch + 1 ints of shared memory; `scratch`: 40 long longs.
+// Whole-block call.  `prefix`: batch + 1 ints of shared memory.  `few`: no sequence has more than a handful of tiles, and a thread
+// goes through those of its sequences; else the tiles of all sequences are shared out evenly first.
 template <int R, int UK, int EXTRA, int NT>
-__device__ AttnRange attention_range(const AttnParams &p, int min_units, int *prefix, long long *scratch) {
-  // tiles of the sequences before each sequence
+__device__ AttnRange attention_range(const AttnParams &p, int *prefix, AttnScratch &scratch) {
   const int chunk = (p.batch + NT - 1) / NT;
   const int b0 = min((int)threadIdx.x * chunk, p.batch), b1 = min(b0 + chunk, p.batch);
-  long long mine = 0;
-  for (int b = b0; b < b1; ++b) {
-    if (blockIdx.x == 0 && !lengths_fit(p, b)) tc::report_timeout(p.status, kStatusBadIndex);
-    mine += row_tiles<R>(p, load_seq(p, b));
-  }
-  long long tiles;
-  long long at = block_scan<NT>(mine, scratch, tiles);
-  for (int b = b0; b < b1; ++b) {
-    prefix[b] = (int)at;
-    at += row_tiles<R>(p, load_seq(p, b));
-  }
-  if (threadIdx.x == 0) prefix[p.batch] = (int)tiles;
-  __syncthreads();
-  // units of the tiles before each thread's tiles
-  const int tchunk = (int)((tiles + NT - 1) / NT);
-  const int t0 = min((long long)threadIdx.x * tchunk, tiles), t1 = min((long long)t0 + tchunk, tiles);
-  int b = 0;
-  mine = 0;
-  if (t0 < t1) {
-    int lo = 0, hi = p.batch;           // the sequence of tile t0: the last with prefix <= t0
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (prefix[mid] <= t0) lo = mid;
-      else hi = mid;
+  int mine = 0, total, t0 = 0, t1 = 0, at;
+  if (p.few) {
+    for (int b = b0; b < b1; ++b) {
+      if (blockIdx.x == 0 && !lengths_fit(p, b)) tc::report_timeout(p.status, kStatusBadIndex);
+      const SeqInfo s = load_seq(p, b);
+      const int n = row_tiles<R>(p, s);
+      for (int t = 0; t < n; ++t) mine += (tile_units<R, UK>(p, s, t).count + EXTRA) * p.hkv;
     }
-    b = lo;
-    int bb = b;
-    SeqInfo s = load_seq(p, bb);
-    for (int t = t0; t < t1; ++t) {
-      while (t >= prefix[bb + 1]) s = load_seq(p, ++bb);
-      mine += (long long)(tile_units<R, UK>(p, s, t - prefix[bb]).count + EXTRA) * p.hkv;
+  } else {
+    // tiles of the sequences before each sequence
+    for (int b = b0; b < b1; ++b) {
+      if (blockIdx.x == 0 && !lengths_fit(p, b)) tc::report_timeout(p.status, kStatusBadIndex);
+      mine += row_tiles<R>(p, load_seq(p, b));
     }
-  }
-  long long total;
-  at = block_scan<NT>(mine, scratch, total);
-  AttnRange r;
-  r.per = (total + gridDim.x - 1) / gridDim.x;
-  if (r.per < min_units) r.per = min_units;
-  r.w0 = min(r.per * blockIdx.x, total), r.w1 = min(r.w0 + r.per, total);
-  r.b = 0, r.tile = 0, r.item0 = 0;
-  if (r.w0 < r.w1) {
-    if (r.w0 >= at && r.w0 < at + mine) {      // exactly one thread
+    int tiles;
+    at = block_scan<NT>(mine, scratch.scan[0], tiles);
+    for (int b = b0; b < b1; ++b) {
+      prefix[b] = at;
+      at += row_tiles<R>(p, load_seq(p, b));
+    }
+    if (threadIdx.x == 0) prefix[p.batch] = tiles;
+    __syncthreads();
+    // units of each thread's tiles
+    const int tchunk = (tiles + NT - 1) / NT;
+    t0 = min((int)threadIdx.x * tchunk, tiles), t1 = min(t0 + tchunk, tiles);
+    mine = 0;
+    if (t0 < t1) {
+      int b = first_tile_owner(p, prefix, t0);
       SeqInfo s = load_seq(p, b);
       for (int t = t0; t < t1; ++t) {
         while (t >= prefix[b + 1]) s = load_seq(p, ++b);
-        const long long u = (long long)(tile_units<R, UK>(p, s, t - prefix[b]).count + EXTRA) * p.hkv;
-        if (r.w0 < at + u) {
-          scratch[36] = at, scratch[37] = b, scratch[38] = t - prefix[b];
+        mine += (tile_units<R, UK>(p, s, t - prefix[b]).count + EXTRA) * p.hkv;
+      }
+    }
+  }
+  at = block_scan<NT>(mine, scratch.scan[1], total);
+  AttnRange r;
+  r.per = max((total + (int)gridDim.x - 1) / (int)gridDim.x, 1);
+  r.w0 = (int)min((long long)r.per * blockIdx.x, (long long)total), r.w1 = min(r.w0 + r.per, total);
+  r.b = 0, r.tile = 0, r.item0 = 0;
+  if (r.w0 < r.w1) {
+    // (lengths that contradict one another can add up to more than an int: the walk checks what it goes by)
+    if (r.w0 >= at && r.w0 < at + mine) {      // one thread
+      int b = p.few ? b0 : first_tile_owner(p, prefix, t0);
+      SeqInfo s = load_seq(p, b);
+      for (int t = p.few ? 0 : t0 - prefix[b];; ++t) {
+        while (t >= row_tiles<R>(p, s) && b + 1 < p.batch) s = load_seq(p, ++b), t = 0;
+        const int u = (tile_units<R, UK>(p, s, t).count + EXTRA) * p.hkv;
+        if (r.w0 < at + u || t >= row_tiles<R>(p, s)) {
+          scratch.found[0] = at, scratch.found[1] = b, scratch.found[2] = t;
           break;
         }
         at += u;
       }
     }
     __syncthreads();
-    r.item0 = scratch[36], r.b = (int)scratch[37], r.tile = (int)scratch[38];
+    r.item0 = scratch.found[0], r.b = scratch.found[1], r.tile = scratch.found[2];
   }
-  __syncthreads();
   return r;
 }
 
@@ -217,19 +230,23 @@ struct AttnWalk {
         w_end_(r.w0), w1_(r.w1), per_(r.per), item0_(r.item0), h1_(-1), started_(false) {}
   __device__ bool next(const AttnParams &p) {
     for (;;) {
-      const long long w = w_end_;
+      const int w = w_end_;
       if (w >= w1_) return false;
       if (!started_) seq = load_seq(p, b);
       else if (w == h1_ && head == p.hkv - 1) ++tile, item0_ = h1_;
       started_ = true;
-      while (tile >= row_tiles<R>(p, seq)) seq = load_seq(p, ++b), tile = 0;   // (sequences without new tokens have no tiles)
+      while (tile >= row_tiles<R>(p, seq)) {             // (sequences without new tokens have no tiles)
+        if (++b >= p.batch) return false;
+        seq = load_seq(p, b), tile = 0;
+      }
       const TileUnits u = tile_units<R, UK>(p, seq, tile);
       const int cost = u.count + EXTRA;
-      head = (int)(w - item0_) / cost;                   // units of a tile over its kv heads fit 32 bits
-      const long long h0 = item0_ + (long long)head * cost;
+      head = (w - item0_) / cost;
+      if ((unsigned)head >= (unsigned)p.hkv) return false;
+      const int h0 = item0_ + head * cost;
       h1_ = h0 + cost;
-      w_end_ = h1_ < w1_ ? h1_ : w1_;
-      const int from = max((int)(w - h0) - EXTRA, 0), to = (int)(w_end_ - h0) - EXTRA;
+      w_end_ = min(h1_, w1_);
+      const int from = max(w - h0 - EXTRA, 0), to = w_end_ - h0 - EXTRA;
       if (to <= from) continue;                          // the range ends before the item's first unit
       n_units = to - from, unit0 = u.first + from;
       r0 = tile * R, n_rows = min(seq.n * p.group - r0, R);
@@ -237,12 +254,13 @@ struct AttnWalk {
       return true;
     }
   }
-  __device__ int last_cta() const { return (int)((h1_ - 1) / per_); }   // where the item ends
+  // For the kernel that joins the pieces of this item.
+  __device__ int4 cut() const { return make_int4(seq.q0, r0, head * 512 + n_rows, (h1_ - 1) / per_); }
   __device__ int token(const AttnParams &p, int row) const { return (r0 + row) / p.group; }
   __device__ int q_head(const AttnParams &p, int row) const { return head * p.group + (r0 + row) % p.group; }
 
  private:
-  long long w_end_, w1_, per_, item0_, h1_;
+  int w_end_, w1_, per_, item0_, h1_;
   bool started_;
 };
 
@@ -277,10 +295,10 @@ __device__ __forceinline__ float2 unpack2(uint32_t w, __half) { return __half22f
 __device__ __forceinline__ int row_exponent(float top) {
   return top > 0.f && top < __int_as_float(0x7f800000) ? min(max(ilogbf(top), -126), 126) : 0;
 }
-// Two e4m3 values (the low 16 bits) as halves; exact.
-__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two) {
-  uint32_t r;
-  asm("{.reg .b16 h; cvt.u16.u32 h, %1; cvt.rn.f16x2.e4m3x2 %0, h;}" : "=r"(r) : "r"(two));
+// Four e4m3 values as halves, in order; exact.
+__device__ __forceinline__ uint2 e4m3x4_to_f16x4(uint32_t four) {
+  uint2 r;
+  asm("{.reg .b16 l, h; mov.b32 {l, h}, %2; cvt.rn.f16x2.e4m3x2 %0, l; cvt.rn.f16x2.e4m3x2 %1, h;}" : "=r"(r.x), "=r"(r.y) : "r"(four));
   return r;
 }
 #endif

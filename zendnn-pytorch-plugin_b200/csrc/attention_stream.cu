@@ -4,8 +4,8 @@
 // A CTA of four warps takes units of 64 keys of an item; each warp streams its own 16 keys of every unit through a private ring
 // in shared memory (16-byte asynchronous copies, whose zero fill also blanks slots past the visible keys, so stale contents of a
 // page never meet the arithmetic) and keeps its own maxima, sums and output rows in registers: no barrier between warps until
-// the item ends, where the four are added through shared memory.  Two CTAs share an SM, so that one streams while the other is
-// in such an end.  Rows are the 16-row (or twice 16) operand of mma.sync.m16n8k16, keys its columns; the accumulator layout of
+// the item ends, where the four are added through shared memory.  Two or three CTAs share an SM, so that others stream while one
+// is in such an end.  Rows are the 16-row (or twice 16) operand of mma.sync.m16n8k16, keys its columns; the accumulator layout of
 // the scores is the operand layout of the probabilities.  e4m3 keys and values become halves in registers, which is exact; the
 // products then run in fp16 with query rows brought to a maximum below 2 by a power of two (what that takes from an element is
 // below 2^-25 of its row's largest).  Probabilities are rounded to the type of the product (half a step of 2^-8 or 2^-11 of
@@ -20,15 +20,18 @@ constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kKeys = 16;                  // of a warp per unit
 constexpr int kUnit = kWarps * kKeys;
-constexpr int kCtasPerSm = 2;
 constexpr int kExtra = 2;                  // units that an item costs beside its own
 
+// Three CTAs share an SM where their rows leave the registers (16 rows; 64 kept keys ahead per CTA), else two.  Decode of 64
+// sequences of 500 - 8000 keys: 191 us with two, 182 with three; an e4m3 cache of 4 x 110000 keys: 220 and 202.
+template <int MT>
+__host__ __device__ constexpr int ctas_per_sm() { return MT == 1 ? 3 : 2; }
 template <int DP, bool E4M3>
 __host__ __device__ constexpr int stage_bytes() { return 2 * kKeys * DP * (E4M3 ? 1 : 2); }
-template <bool E4M3>
-__host__ __device__ constexpr int stages() { return E4M3 ? 6 : 3; }
-template <int DP, bool E4M3>
-__host__ __device__ constexpr int ring_bytes() { return kWarps * stages<E4M3>() * stage_bytes<DP, E4M3>(); }
+template <bool E4M3, int MT>
+__host__ __device__ constexpr int stages() { return (E4M3 ? 2 : 1) * (MT == 1 ? 2 : 3); }
+template <int DP, bool E4M3, int MT>
+__host__ __device__ constexpr int ring_bytes() { return kWarps * stages<E4M3, MT>() * stage_bytes<DP, E4M3>(); }
 template <int R, int DP>
 __host__ __device__ constexpr int merge_bytes() { return kWarps * R * (DP + 8) * 4 + kWarps * R * 8; }
 
@@ -63,20 +66,20 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
 }
 
 template <typename T, bool E4M3, int DP, int MT>
-__global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_stream_kernel(const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(kThreads, ctas_per_sm<MT>()) attention_stream_kernel(const __grid_constant__ AttnParams p) {
   using M = std::conditional_t<E4M3, __half, T>;
-  constexpr int R = 16 * MT, S = stages<E4M3>(), SB = stage_bytes<DP, E4M3>();
+  constexpr int R = 16 * MT, S = stages<E4M3, MT>(), SB = stage_bytes<DP, E4M3>();
   constexpr int ES = E4M3 ? 1 : 2;
   constexpr int CH = DP * ES / 16;            // 16-byte chunks of a key's row
   constexpr int KS = DP / 16;                 // 16-element steps of the score product
   constexpr int NT = DP / 8;                  // 8-column tiles of the output
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ long long s_scan[40];
+  __shared__ AttnScratch s_scan;
   grid_launch_dependents();
   grid_dependency_wait();
   const int lane = threadIdx.x & 31, warp = tc::uniform_warp();
   const int g = lane >> 2, t4 = lane & 3;
-  const AttnRange range = attention_range<R, kUnit, kExtra, kThreads>(p, 1, reinterpret_cast<int *>(smem), s_scan);
+  const AttnRange range = attention_range<R, kUnit, kExtra, kThreads>(p, reinterpret_cast<int *>(smem), s_scan);
   zero_tail_rows<T>(p, kThreads);
   unsigned char *ring = smem + warp * S * SB;
   const uint32_t ring_addr = smem_u32(ring);
@@ -93,11 +96,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_stream_kernel(
     const int k_begin = max(key_lo(p, seq, tok0), unit0 * kUnit);
     const int k_end = min((long long)key_hi(p, seq, tok1), ((long long)unit0 + n_units) * kUnit);
 
-    // ---- query rows as operand fragments ------------------------------------------------------------------
+    // ---- query rows as operand fragments (their loads go out before those of the keys wait for the page table) ----
     uint32_t qf[MT][KS][4];
     int lo[MT][2], hi[MT][2];
-    float mul[MT][2];
-    const float head_scale = p.scale_log2 * (E4M3 ? fabsf(p.k_scale[head]) : 1.f);
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
 #pragma unroll
@@ -108,35 +109,13 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_stream_kernel(
         lo[m][half] = live ? key_lo(p, seq, tok) : 0;
         hi[m][half] = live ? key_hi(p, seq, tok) : 0;
         const char *src = reinterpret_cast<const char *>(p.q) + ((seq.q0 + tok) * p.q_st + qh * p.q_sh) * 2;
-        float top = 0.f;
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
 #pragma unroll
           for (int part = 0; part < 2; ++part) {
             // e4m3: a lane's four bytes of a key are elements 4t..4t+3 of a step, whichever column of the product they are
             const int e = 16 * s + (E4M3 ? 4 * t4 + 2 * part : 8 * part + 2 * t4);
-            const uint32_t x = live && e < p.d ? *reinterpret_cast<const uint32_t *>(src + e * 2) : 0u;
-            qf[m][s][2 * part + half] = x;
-            if constexpr (E4M3) {
-              const float2 f = unpack2(x, T(0.f));
-              top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
-            }
-          }
-        }
-        mul[m][half] = head_scale;
-        if constexpr (E4M3) {
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-          const int ex = row_exponent(top);
-          const float down = copysignf(ldexpf(1.f, -ex), p.k_scale[head]);
-          mul[m][half] = head_scale * ldexpf(1.f, ex);
-#pragma unroll
-          for (int s = 0; s < KS; ++s) {
-#pragma unroll
-            for (int part = 0; part < 2; ++part) {
-              const float2 f = unpack2(qf[m][s][2 * part + half], T(0.f));
-              qf[m][s][2 * part + half] = pack2(f.x * down, f.y * down, M(0.f));
-            }
+            qf[m][s][2 * part + half] = live && e < p.d ? *reinterpret_cast<const uint32_t *>(src + e * 2) : 0u;
           }
         }
       }
@@ -149,43 +128,95 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_stream_kernel(
     const char *vb = reinterpret_cast<const char *>(p.v) + head * p.v_sh * ES;
     const int32_t *pages = p.table + b * p.table_stride;
     const int key0 = unit0 * kUnit + warp * kKeys;
-    // the page of this lane's key (lanes 0-15) one piece ahead of its copies
+    // Pages of a power of two of at least 16 slots hold a warp's 16 keys in one: every lane has their page and the slot of the
+    // first.  Else lane 0-15 have the page and slot of a key each.  The lookup is one stage ahead of the copies.
+    const bool one_page = p.page_shift >= 4;
     auto page_id = [&](int i) -> int {
-      const int key = key0 + i * kUnit + (lane & 15);
-      if (i >= n_units || key < k_begin || key >= k_end) return -1;
+      const int first = key0 + i * kUnit, key = first + (one_page ? 0 : lane & 15);
+      if (i >= n_units || (one_page ? first + kKeys : key + 1) <= k_begin || key >= k_end) return -1;
       const int id = pages[page_of(p, key)];
       if (id >= 0 && id < p.num_pages) return id;
       tc::report_timeout(p.status, kStatusBadIndex);
       return -1;
     };
-    int ahead = page_id(0);
+    int ids[S];
+#pragma unroll
+    for (int i = 0; i < S; ++i) ids[i] = page_id(i);      // lookups of the first stages at once
+    int ahead = ids[0];
     auto issue = [&](int i) {
       const int id = ahead;
-      ahead = page_id(i + 1);
+      ahead = i + 1 < S ? ids[i + 1] : page_id(i + 1);
       if (i < n_units) {
-        const int key = key0 + i * kUnit + (lane & 15);
-        const int slot = key - page_of(p, key) * p.page;
-        const uint32_t dst = ring_addr + (i % S) * SB;
+        const int first = key0 + i * kUnit;
         constexpr int RP = 32 / CH;            // rows per pass of the warp
-        const int c = lane % CH;
+        const int c = lane % CH, sub = lane / CH;
         const int bytes = min(max(p.d * ES - c * 16, 0), 16);
-#pragma unroll
-        for (int j = 0; j < kKeys / RP; ++j) {
-          const int row = j * RP + lane / CH;
-          const int rid = __shfl_sync(0xffffffffu, id, row), rslot = __shfl_sync(0xffffffffu, slot, row);
-          const bool live = rid >= 0 && bytes > 0;
-          const int64_t ko = live ? (rid * p.k_sp + rslot * p.k_ss) * ES + c * 16 : 0;
-          const int64_t vo = live ? (rid * p.v_sp + rslot * p.v_ss) * ES + c * 16 : 0;
+        const uint32_t dst = ring_addr + (i % S) * SB;
+        auto copy = [&](int row, bool live, const char *k, const char *v) {
           const int sw = CH == 4 ? (c ^ ((row >> 1) & 3)) : (c ^ (row & 7));
-          const uint32_t at = row * (CH * 16) + sw * 16;
-          cp_async16(dst + at, live ? kb + ko : kb, live ? bytes : 0);
-          cp_async16(dst + SB / 2 + at, live ? vb + vo : vb, live ? bytes : 0);
+          const uint32_t at = dst + row * (CH * 16) + sw * 16;
+          cp_async16(at, live ? k : kb, live ? bytes : 0);
+          cp_async16(at + SB / 2, live ? v : vb, live ? bytes : 0);
+        };
+        if (one_page) {
+          const int slot = (first & (p.page - 1)) + sub;
+          const char *k = kb + ((int64_t)id * p.k_sp + slot * p.k_ss) * ES + c * 16, *v = vb + ((int64_t)id * p.v_sp + slot * p.v_ss) * ES + c * 16;
+          const int64_t k_step = p.k_ss * (RP * ES), v_step = p.v_ss * (RP * ES);
+          const bool any = id >= 0 && bytes > 0;
+#pragma unroll
+          for (int j = 0; j < kKeys / RP; ++j) {
+            const int row = j * RP + sub;
+            copy(row, any && first + row >= k_begin && first + row < k_end, k, v);
+            k += k_step, v += v_step;
+          }
+        } else {
+          const int key = first + (lane & 15), slot = key - page_of(p, key) * p.page;
+#pragma unroll
+          for (int j = 0; j < kKeys / RP; ++j) {
+            const int row = j * RP + sub;
+            const int rid = __shfl_sync(0xffffffffu, id, row), rslot = __shfl_sync(0xffffffffu, slot, row);
+            copy(row, rid >= 0 && bytes > 0, kb + (rid * p.k_sp + rslot * p.k_ss) * ES + c * 16, vb + (rid * p.v_sp + rslot * p.v_ss) * ES + c * 16);
+          }
         }
       }
       cp_async_commit();
     };
 #pragma unroll
     for (int i = 0; i < S - 1; ++i) issue(i);
+
+    float mul[MT][2];
+    const float head_scale = p.scale_log2 * (E4M3 ? fabsf(p.k_scale[head]) : 1.f);
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        mul[m][half] = head_scale;
+        if constexpr (E4M3) {
+          float top = 0.f;
+#pragma unroll
+          for (int s = 0; s < KS; ++s) {
+#pragma unroll
+            for (int part = 0; part < 2; ++part) {
+              const float2 f = unpack2(qf[m][s][2 * part + half], T(0.f));
+              top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+            }
+          }
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          const int ex = row_exponent(top);
+          const float down = copysignf(ldexpf(1.f, -ex), p.k_scale[head]);
+          mul[m][half] = fmaxf(head_scale * ldexpf(1.f, ex), 1e-30f);   // (a scale of zero: masked scores stay minus infinity)
+#pragma unroll
+          for (int s = 0; s < KS; ++s) {
+#pragma unroll
+            for (int part = 0; part < 2; ++part) {
+              const float2 f = unpack2(qf[m][s][2 * part + half], T(0.f));
+              qf[m][s][2 * part + half] = pack2(f.x * down, f.y * down, M(0.f));
+            }
+          }
+        }
+      }
+    }
 
     // ---- one pass over the keys -------------------------------------------------------------------------------
     float o[MT][NT][4], top[MT][2], sum[MT][2];
@@ -229,12 +260,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_stream_kernel(
           ldmatrix4(kf, frag_addr(ks, (lane & 7) + (((lane >> 3) & 1) << 3), s + (lane >> 4)));
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const uint32_t a0 = e4m3x2_to_f16x2(kf[2 * h]), a1 = e4m3x2_to_f16x2(kf[2 * h] >> 16);
-            const uint32_t b0 = e4m3x2_to_f16x2(kf[2 * h + 1]), b1 = e4m3x2_to_f16x2(kf[2 * h + 1] >> 16);
+            const uint2 x = e4m3x4_to_f16x4(kf[2 * h]), y = e4m3x4_to_f16x4(kf[2 * h + 1]);
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
-              mma16816(sc[m][0], qf[m][s + h], a0, a1, M(0.f));
-              mma16816(sc[m][1], qf[m][s + h], b0, b1, M(0.f));
+              mma16816(sc[m][0], qf[m][s + h], x.x, x.y, M(0.f));
+              mma16816(sc[m][1], qf[m][s + h], y.x, y.y, M(0.f));
             }
           }
         }
@@ -245,33 +275,39 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_stream_kernel(
       uint32_t pf[MT][4];
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
+        float mx[2];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          float x[4] = {sc[m][0][2 * half] * mul[m][half], sc[m][0][2 * half + 1] * mul[m][half],
-                        sc[m][1][2 * half] * mul[m][half], sc[m][1][2 * half + 1] * mul[m][half]};
           if (!inside) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int key = kbase + (e >> 1) * 8 + 2 * t4 + (e & 1);
-              if (key < max(lo[m][half], k_begin) || key >= min(hi[m][half], k_end)) x[e] = -INFINITY;
+              if (key < max(lo[m][half], k_begin) || key >= min(hi[m][half], k_end)) sc[m][e >> 1][2 * half + (e & 1)] = -INFINITY;
             }
           }
-          float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-          // the reference of the exponents follows the maximum only when it has fallen far behind
-          if (__any_sync(0xffffffffu, mx > top[m][half] + kLazyRescale)) {
-            const float to = fmaxf(top[m][half], mx);
+          mx[half] = fmaxf(fmaxf(sc[m][0][2 * half], sc[m][0][2 * half + 1]), fmaxf(sc[m][1][2 * half], sc[m][1][2 * half + 1]));
+          mx[half] = fmaxf(mx[half], __shfl_xor_sync(0xffffffffu, mx[half], 1));
+          mx[half] = fmaxf(mx[half], __shfl_xor_sync(0xffffffffu, mx[half], 2)) * mul[m][half];
+        }
+        // the reference of the exponents follows the maximum only when it has fallen far behind
+        if (__any_sync(0xffffffffu, mx[0] > top[m][0] + kLazyRescale || mx[1] > top[m][1] + kLazyRescale)) {
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const float to = fmaxf(top[m][half], mx[half]);
             const float f = top[m][half] == -INFINITY ? 0.f : exp2_fast(top[m][half] - to);
             sum[m][half] *= f;
 #pragma unroll
             for (int n = 0; n < NT; ++n) o[m][n][2 * half] *= f, o[m][n][2 * half + 1] *= f;
             top[m][half] = to;
           }
-          const float ref = top[m][half] == -INFINITY ? 0.f : top[m][half];
+        }
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const float neg = top[m][half] == -INFINITY ? 0.f : -top[m][half];
+          float x[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            x[e] = exp2_fast(x[e] - ref);
+            x[e] = exp2_fast(fmaf(sc[m][e >> 1][2 * half + (e & 1)], mul[m][half], neg));
             sum[m][half] += x[e];
           }
           pf[m][half] = pack2(x[0], x[1], M(0.f));
@@ -297,13 +333,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_stream_kernel(
           ldmatrix4_trans(vf, frag_addr(vs, (lane & 7) + (((lane >> 3) & 1) << 3), n / 2 + (lane >> 4)));
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const uint32_t x = __byte_perm(vf[2 * h], 0, 0x3120), y = __byte_perm(vf[2 * h + 1], 0, 0x3120);
-            const uint32_t e0 = e4m3x2_to_f16x2(x), e1 = e4m3x2_to_f16x2(y);              // even columns of the chunk
-            const uint32_t d0 = e4m3x2_to_f16x2(x >> 16), d1 = e4m3x2_to_f16x2(y >> 16);   // odd columns
+            // the even and the odd columns of the chunk
+            const uint2 x = e4m3x4_to_f16x4(__byte_perm(vf[2 * h], 0, 0x3120)), y = e4m3x4_to_f16x4(__byte_perm(vf[2 * h + 1], 0, 0x3120));
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
-              mma16816(o[m][n + 2 * h], pf[m], e0, e1, M(0.f));
-              mma16816(o[m][n + 2 * h + 1], pf[m], d0, d1, M(0.f));
+              mma16816(o[m][n + 2 * h], pf[m], x.x, y.x, M(0.f));
+              mma16816(o[m][n + 2 * h + 1], pf[m], x.y, y.y, M(0.f));
             }
           }
         }
@@ -379,14 +414,14 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_stream_kernel(
         if (c == 0) p.part_ml[(int64_t)slot * R + row] = make_float2(best, l);
       }
     }
-    if (threadIdx.x == 0 && !it.whole && it.first_piece) p.meta[blockIdx.x] = make_int4(b, it.tile, head, it.last_cta());
+    if (threadIdx.x == 0 && !it.whole && it.first_piece) p.meta[blockIdx.x] = it.cut();
     __syncthreads();   // the merge area is read before the next rings fill it
   }
 }
 
 template <typename T, bool E4M3, int DP, int MT>
 int launch(const AttnParams &p, const AttnPlan &plan, cudaStream_t st) {
-  constexpr int ring = ring_bytes<DP, E4M3>(), merge = merge_bytes<16 * MT, DP>();
+  constexpr int ring = ring_bytes<DP, E4M3, MT>(), merge = merge_bytes<16 * MT, DP>();
   constexpr int fixed = ring > merge ? ring : merge;
   const int prefix = (p.batch + 1) * 4;
   const int smem = prefix > fixed ? prefix : fixed;   // the division of the batch comes before the first copy
@@ -405,7 +440,7 @@ int launch_sized(const AttnParams &p, const AttnPlan &plan, cudaStream_t st) {
 
 }  // namespace
 
-int attention_stream_grid() { return kCtasPerSm * sm_count(); }
+int attention_stream_grid(int rows) { return (rows == 16 ? ctas_per_sm<1>() : ctas_per_sm<2>()) * sm_count(); }
 
 int attention_stream_launch(const AttnParams &p, const AttnPlan &plan, int dtype, int cache_dtype, cudaStream_t st) {
   const bool e4m3 = cache_dtype == ZT_E4M3;

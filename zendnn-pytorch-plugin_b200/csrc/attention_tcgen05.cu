@@ -9,7 +9,7 @@
 //   warps 8-11       K and V tiles into a ring, 32 keys each: by TMA, in boxes of up to 32 slots of a page, where the pages hold a power
 //                    of two of at least 8 slots and all 32 keys are visible; else row by row, 16 bytes per asynchronous copy (any
 //                    page size).  Slots past the visible keys become zeros that way, so stale contents of a page never meet the
-//                    arithmetic.  e4m3 caches come through registers and are stored as halves (exact)
+//                    arithmetic.  e4m3 tiles come row by row into a ring of their own and from there as halves (exact)
 //   warp 12          issues the MMAs
 //   warp 13          walks the CTA's range and hands its pieces to the others
 //
@@ -26,17 +26,19 @@ namespace {
 constexpr int kTile = 128;                 // rows of a tile, keys of a unit
 constexpr int kRows = 2 * kTile;
 constexpr int kThreads = 512;              // four warpgroups: tile 0, tile 1, copies, MMA and walk (and two idle warps)
-constexpr int kExtra = 2;                  // units that an item costs beside its own
+constexpr int kExtra = 3;                  // units that an item costs beside its own
 constexpr int kHalf = kTile * 128;         // bytes of 64 columns of a tile: 128 rows of 128 bytes, swizzled
-constexpr int kLag = 2;                    // stages whose row copies are in flight behind the newest
 constexpr int kBoxSlots = 32;              // slots of a page per TMA box, at most
 
-template <int DP>
+template <int DP, bool E4M3>
 struct Smem {
   static constexpr int kTileBytes = kTile * DP * 2;
-  static constexpr int kStages = DP == 128 ? 5 : 8;
+  static constexpr int kStages = E4M3 ? (DP == 128 ? 3 : 6) : DP == 128 ? 5 : 8;
+  static constexpr int kLag = E4M3 ? 3 : 2;                     // stages whose row copies are in flight behind the newest
   static constexpr int kRing = 2 * kTileBytes;                  // after the two query tiles
-  static constexpr int kBytes = kRing + kStages * kTileBytes;
+  static constexpr int kRaw = kRing + kStages * kTileBytes;     // e4m3: tiles as they come, kLag + 1 of them
+  static constexpr int kRawBytes = kTile * DP;
+  static constexpr int kBytes = kRaw + (E4M3 ? (kLag + 1) * kRawBytes : 0);
 };
 
 // Registers per thread after the split; the sum over the four warpgroups is that of the launch, 4 * 128.
@@ -86,38 +88,7 @@ __device__ __forceinline__ void tma_load_4d_if(bool lane_does, uint32_t dst, con
       : "memory");
 }
 
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  float2 d;
-  asm("mul.rn.f32x2 %0, %1, %2;"
-      : "=l"(*reinterpret_cast<unsigned long long *>(&d))
-      : "l"(*reinterpret_cast<const unsigned long long *>(&a)), "l"(*reinterpret_cast<const unsigned long long *>(&b)));
-  return d;
-}
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
-
-// 2^x for x below 128 on the multiply-add pipes: 2^n 2^f with n the nearest whole number (which an addition of 1.5 2^23 leaves in
-// the low bits) and a minimax polynomial of degree 4 for 2^f on [-1/2, 1/2], fitted for this file by the exchange algorithm with
-// the relative error as its target: 2.7e-6 (2^-18.5) with fp32 coefficients and arithmetic.  Below 2^-126.5 the result is zero;
-// NaN stays NaN.
-__device__ __forceinline__ float2 exp2_poly2(float2 x) {
-  constexpr float kMagic = 12582912.f + 127.f;    // the low bits become n + 127, the exponent field of 2^n
-  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x.x));   // -127
-  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x.y));
-  const float2 r = add2(x, both(kMagic));
-  const float2 f = add2(x, mul2(add2(r, both(-kMagic)), both(-1.f)));
-  float2 y = fma2(both(0.009570102207362652f), f, both(0.05591785907745361f));
-  y = fma2(y, f, both(0.240247443318367f));
-  y = fma2(y, f, both(0.6931217908859253f));
-  y = fma2(y, f, both(0.9999992847442627f));
-  return mul2(y, make_float2(__uint_as_float(__float_as_uint(r.x) << 23), __uint_as_float(__float_as_uint(r.y) << 23)));
-}
-// Of 16 pairs of exponentials this many go that way, the others to the special-function unit, whose 4 lanes per cycle would
-// otherwise be the longest part of a row's work.
-#ifndef POLY16
-#define POLY16 5
-#endif
-constexpr int kPolyOf16 = POLY16;
-__host__ __device__ constexpr bool by_polynomial(int pair) { return (pair * kPolyOf16) / 16 != ((pair + 1) * kPolyOf16) / 16; }
 
 struct Barriers {
   uint64_t kv_full[8], kv_free[8];
@@ -129,7 +100,8 @@ struct Barriers {
 // A piece of an item, as the walk hands it out; b < 0: there are no more.
 struct Piece {
   SeqInfo seq;
-  int b, tile, head, unit0, n_units, r0, n_rows, first_piece, whole, last_cta;
+  int4 cut;          // what the joining kernel is told of the item
+  int b, head, unit0, n_units, r0, n_rows, first_piece, whole;
   int count[2];      // units that each tile works on, from the piece's first
 
   __device__ int token(const AttnParams &p, int row) const { return (r0 + row) / p.group; }
@@ -151,12 +123,12 @@ template <typename T, bool E4M3, int DP>
 __global__ void __launch_bounds__(kThreads, 1) attention_tcgen05_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUtensorMap k_map,
                                                                         const __grid_constant__ CUtensorMap v_map, int box) {
   using M = std::conditional_t<E4M3, __half, T>;
-  using L = Smem<DP>;
+  using L = Smem<DP, E4M3>;
   constexpr int S = L::kStages, CHUNKS = DP / 8;
   extern __shared__ unsigned char smem_raw[];
   __shared__ Barriers bars;
   __shared__ Piece pieces[kPieces];
-  __shared__ long long s_scan[40];
+  __shared__ AttnScratch s_scan;
   unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   const uint32_t base = smem_u32(smem);
   const int warp = tc::uniform_warp(), lane = threadIdx.x & 31;
@@ -172,7 +144,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tcgen05_kernel(const __
   if (warp == 12) tc::tmem_alloc(&bars.tmem, 512);
   grid_launch_dependents();
   grid_dependency_wait();
-  const AttnRange range = attention_range<kRows, kTile, kExtra, kThreads>(p, 1, reinterpret_cast<int *>(smem), s_scan);
+  const AttnRange range = attention_range<kRows, kTile, kExtra, kThreads>(p, reinterpret_cast<int *>(smem), s_scan);
   zero_tail_rows<T>(p, kThreads);
   if (threadIdx.x == 0) p.meta[blockIdx.x] = make_int4(-1, 0, 0, 0);
   tc::fence_before_sync();
@@ -203,8 +175,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tcgen05_kernel(const __
                    p_half = smem_u32(&bars.p_half[i]);
     uint32_t n_s = 0, n_o = 0;     // phases of s_full and o_full so far
 
-    // Rows of queries come in, and rows of the output go out, 16 lanes (8 for heads of up to 64) to a row, so that a warp's access
-    // covers whole lines; the tile of shared memory that held the queries takes the output rows in between.
+    // Rows of queries come in 16 lanes (8 for heads of up to 64) to a row, so that a warp's access covers whole lines.
     constexpr int RP = 32 / CHUNKS, PASSES = 32 / RP;    // rows per pass of the warp
     const int c = lane % CHUNKS, sub = lane / CHUNKS;
     const uint32_t tile = base + i * L::kTileBytes;
@@ -225,7 +196,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tcgen05_kernel(const __
           const bool in = o >= 0 && c * 8 < p.d;
           cp_async16(tile + tile_at(row0 + q * RP + sub, c), in ? src + (o + c * 8) * 2 : src, in ? 16 : 0);
         }
-        asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+        asm volatile("cp.async.commit_group;" ::: "memory");
       } else {
         const float k_scale = p.k_scale[it.head];
         uint4 x[PASSES];
@@ -260,15 +231,21 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tcgen05_kernel(const __
         }
         mul *= fabsf(k_scale) * ldexpf(1.f, my_ex);
       }
+      return fmaxf(mul, 1e-30f);    // a scale of zero: masked scores stay minus infinity
+    };
+    auto query_ready = [&]() {
+      if constexpr (!E4M3) asm volatile("cp.async.wait_group 0;" ::: "memory");
       fence_async_proxy();
       __syncwarp();
       tc::arrive_if(lane == 0, q_full);
-      return fmaxf(mul, 1e-30f);    // a scale of zero: masked scores stay minus infinity
     };
 
     const Piece *it = take();
     float mul = 0.f;
-    if (it && it->count[i] > 0) mul = load_query(*it);
+    if (it && it->count[i] > 0) {
+      mul = load_query(*it);
+      query_ready();
+    }
     while (it) {
       const int rows = min(max(it->n_rows - i * kTile, 0), kTile), count = it->count[i], unit0 = it->unit0;
       const bool live = row < rows;
@@ -341,8 +318,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tcgen05_kernel(const __
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
             float2 y = fma2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), mul_2, neg_2);
-            if (by_polynomial(e / 2)) y = exp2_poly2(y);
-            else y.x = exp2_fast(y.x), y.y = exp2_fast(y.y);
+            y.x = exp2_fast(y.x), y.y = exp2_fast(y.y);
             part[(e >> 1) & 1] = add2(part[(e >> 1) & 1], y);
             pk[e / 2] = pack2(y.x, y.y, M(0.f));
           }
@@ -377,14 +353,23 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tcgen05_kernel(const __
         const int r = i * kTile + row;
         out_at = (it->seq.q0 + it->token(p, r)) * p.o_st + it->q_head(p, r) * p.o_sh;
       }
-      if (threadIdx.x == 0 && !whole && it->first_piece) p.meta[blockIdx.x] = make_int4(it->b, it->tile, it->head, it->last_cta);
+      if (threadIdx.x == 0 && !whole && it->first_piece) p.meta[blockIdx.x] = it->cut;
       give_back();
+      // the next queries are on their way during the wait for the last product, and the tensor core has them before this output
+      it = take();
+      if (!ok) break;
+      const bool query = it && it->count[i] > 0;
+      if (query) mul = load_query(*it);
       if (count > 0) {
         if (!(ok = tc::warp_wait(o_full, (n_o - 1) & 1))) break;
         tc::fence_after_sync();
       }
+      if (query) query_ready();
       if (rows > 0) {
         const float f = !whole ? v_scale : sum == 0.f ? 0.f : v_scale / sum;
+        int64_t quad[4];       // this lane's four rows after the exchange below
+#pragma unroll
+        for (int r = 0; r < 4; ++r) quad[r] = __shfl_sync(0xffffffffu, out_at, (lane & ~3) + r);
 #pragma unroll 1
         for (int col = 0; col < p.d; col += 32) {
           uint32_t o[32];
@@ -396,14 +381,30 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tcgen05_kernel(const __
             for (int e = 0; e < 32; ++e) o[e] = 0;
           }
           if (whole) {
+            // 16 bytes of a row per lane would touch 32 lines at once: four lanes exchange so that each row's 64 bytes lie in a quad
+            uint32_t h[4][4];
 #pragma unroll
-            for (int e = 0; e < 32; e += 8) {
-              uint32_t h[4];
+            for (int e = 0; e < 16; ++e)
+              h[e / 4][e % 4] = pack2(__uint_as_float(o[2 * e]) * f, __uint_as_float(o[2 * e + 1]) * f, T(0.f));
 #pragma unroll
-              for (int q = 0; q < 4; ++q)
-                h[q] = pack2(__uint_as_float(o[e + 2 * q]) * f, __uint_as_float(o[e + 2 * q + 1]) * f, T(0.f));
-              if (col + e < DP) st_shared16(tile + tile_at(row, (col + e) / 8), h[0], h[1], h[2], h[3]);
+            for (int m = 1; m <= 2; m *= 2) {
+              const bool upper = lane & m;
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                if (k & m) continue;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const uint32_t got = __shfl_xor_sync(0xffffffffu, upper ? h[k][e] : h[k + m][e], m);
+                  if (upper) h[k][e] = got;
+                  else h[k + m][e] = got;
+                }
+              }
             }
+            const int at = col + (lane & 3) * 8;
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (quad[r] >= 0 && at < p.d)
+                *reinterpret_cast<uint4 *>(reinterpret_cast<char *>(p.out) + (quad[r] + at) * 2) = make_uint4(h[r][0], h[r][1], h[r][2], h[r][3]);
           } else if (live) {     // [slot][column / 4][row] in units of four columns: a warp's rows are neighbours
             float4 *dst = reinterpret_cast<float4 *>(p.part_o) + ((int64_t)slot * (DP / 4) + col / 4) * kRows + i * kTile + row;
 #pragma unroll
@@ -413,23 +414,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tcgen05_kernel(const __
                                                    __uint_as_float(o[e + 2]) * f, __uint_as_float(o[e + 3]) * f);
           }
         }
-        if (whole) {
-          __syncwarp();
-#pragma unroll
-          for (int q = 0; q < PASSES; ++q) {
-            const int64_t o = row_of(out_at, q);
-            if (o >= 0 && c * 8 < p.d)
-              *reinterpret_cast<uint4 *>(reinterpret_cast<char *>(p.out) + (o + c * 8) * 2) = ld_shared16(tile + tile_at(row0 + q * RP + sub, c));
-          }
-          __syncwarp();     // the rows are read before the next queries come
-        } else if (live) {  // (a NaN outweighs the other pieces' rows)
+        if (live && !whole)    // (a NaN outweighs the other pieces' rows)
           p.part_ml[(int64_t)slot * kRows + i * kTile + row] = make_float2(sum != sum ? INFINITY : sum == 0.f ? -INFINITY : ref, sum);
-        }
       }
       tc::fence_before_sync();   // O is read before the next piece's first product, which waits for this warp's probabilities
-      it = take();
-      if (!ok) break;
-      if (it && it->count[i] > 0) mul = load_query(*it);
     }
     if (!ok && lane == 0) tc::report_timeout(p.status, kStatusEpilogueTimeout);
   } else if (warp < 12) {
@@ -442,15 +430,39 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tcgen05_kernel(const __
     constexpr int PASSES = 32 / RP;
     const int c = lane % CH, sub = lane / CH;
     const int bytes = min(max(p.d * ES - c * 16, 0), 16);
-    uint32_t n = 0, pending = 0;              // stages begun; which of the last have row copies that were not reported yet
-    auto arrived = [&](uint32_t k) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(kLag) : "memory");
+    uint32_t n = 0, pending = 0;              // stages begun; which of the last have row copies that were not handed on yet
+    const uint32_t raw = base + L::kRaw + w4 * (L::kRawBytes / 4) + lane * 16;      // e4m3: this lane's part of a raw tile
+    // Hands stage k on; its row copies are the oldest of at most kLag + 1 groups in flight.
+    auto finish = [&](uint32_t k) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(L::kLag) : "memory");
+      if constexpr (E4M3) {
+        const uint32_t st = k % S, dst = base + L::kRing + st * L::kTileBytes;
+        if (k >= S && !(ok = tc::warp_wait(smem_u32(&bars.kv_free[st]), (k / S - 1) & 1))) return;
+#pragma unroll
+        for (int q = 0; q < PASSES; ++q) {
+          const int r = w4 * 32 + q * RP + sub;
+          const uint4 x = ld_shared16(raw + k % (L::kLag + 1) * L::kRawBytes + q * 512);
+          const uint2 h0 = e4m3x4_to_f16x4(x.x), h1 = e4m3x4_to_f16x4(x.y), h2 = e4m3x4_to_f16x4(x.z), h3 = e4m3x4_to_f16x4(x.w);
+          st_shared16(dst + tile_at(r, 2 * c), h0.x, h0.y, h1.x, h1.y);
+          st_shared16(dst + tile_at(r, 2 * c + 1), h2.x, h2.y, h3.x, h3.y);
+        }
+      }
       fence_async_proxy();
       __syncwarp();
       tc::arrive_if(lane == 0, smem_u32(&bars.kv_full[k % S]));
       pending &= ~(1u << (k & 31));
     };
-    while (const Piece *piece = take()) {
+    auto finish_all = [&]() {
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      for (uint32_t k = n > L::kLag ? n - L::kLag : 0; ok && k < n; ++k)
+        if (pending >> (k & 31) & 1) finish(k);
+    };
+    // Stages lag behind only while there are others to begin: the piece after this one may be waiting for its products.
+    auto take_or_finish = [&]() -> const Piece * {
+      if (!__all_sync(0xffffffffu, tc::mbar_test_addr(smem_u32(&bars.piece_full[n_piece % kPieces]), (n_piece / kPieces) & 1))) finish_all();
+      return ok ? take() : nullptr;
+    };
+    while (const Piece *piece = take_or_finish()) {
       const Piece &it = *piece;
       const int units = max(it.count[0], it.count[1]), head = it.head;
       const int k_begin = max(key_lo(p, it.seq, it.token(p, 0)), it.unit0 * kTile);
@@ -469,79 +481,53 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tcgen05_kernel(const __
         return -1;
       };
       auto slot_of = [&](int key) { return key - page_of(p, key) * p.page; };
-      uint4 xk[E4M3 ? PASSES : 1], xv[E4M3 ? PASSES : 1];      // e4m3: 16 bytes of PASSES rows, in flight
-      auto fetch = [&](uint4 (&x)[E4M3 ? PASSES : 1], const char *src, int64_t sp, int64_t ss, int id, int slot) {
-#pragma unroll
-        for (int q = 0; q < (E4M3 ? PASSES : 1); ++q) {
-          const int r = q * RP + sub;
-          const int rid = __shfl_sync(0xffffffffu, id, r), rslot = __shfl_sync(0xffffffffu, slot, r);
-          x[q] = rid >= 0 && bytes > 0 ? *reinterpret_cast<const uint4 *>(src + rid * sp + rslot * ss + c * 16) : make_uint4(0, 0, 0, 0);
-        }
-      };
       int ahead = page_id(0);
-      if (E4M3 && units > 0) fetch(xk, kb, p.k_sp, p.k_ss, ahead, slot_of(first));
       for (int j = 0; j < units && ok; ++j) {
         const int id = ahead, key = first + j * kTile, slot = slot_of(key);
         ahead = page_id(j + 1);
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
           const int st = n % S;
-          const uint32_t dst = base + L::kRing + st * L::kTileBytes;
           const char *src = kv ? vb : kb;
           const int64_t sp = kv ? p.v_sp : p.k_sp, ss = kv ? p.v_ss : p.k_ss;
+          bool rows = true;
           if constexpr (!E4M3) {
             if (n >= S && !(ok = tc::warp_wait(smem_u32(&bars.kv_free[st]), (n / S - 1) & 1))) break;
-            const uint32_t full = smem_u32(&bars.kv_full[st]);
             if (box > 0 && __all_sync(0xffffffffu, id >= 0)) {
               // lane l of the first (boxes x halves): box l / halves of this warp's 32 keys, 64 columns of it
               constexpr int HALVES = DP / 64;
               const int b_i = lane / HALVES, half = lane % HALVES;
               const int bid = __shfl_sync(0xffffffffu, id, b_i * box & 31), bslot = __shfl_sync(0xffffffffu, slot, b_i * box & 31);
+              const uint32_t full = smem_u32(&bars.kv_full[st]), dst = base + L::kRing + st * L::kTileBytes;
               tc::expect_tx_if(lane == 0, full, 32 * DP * 2);
               __syncwarp();
               tma_load_4d_if(b_i * box < 32, dst + half * kHalf + (w4 * 32 + b_i * box) * 128, kv ? &v_map : &k_map, full, half * 64, bslot,
                              head, bid);
-            } else {
-#pragma unroll
-              for (int q = 0; q < PASSES; ++q) {
-                const int r = q * RP + sub;
-                const int rid = __shfl_sync(0xffffffffu, id, r), rslot = __shfl_sync(0xffffffffu, slot, r);
-                const bool live = rid >= 0 && bytes > 0;
-                cp_async16(dst + tile_at(w4 * 32 + r, c), live ? src + (rid * sp + rslot * ss) * ES + c * 16 : src, live ? bytes : 0);
-              }
-              pending |= 1u << (n & 31);
+              rows = false;
             }
-            asm volatile("cp.async.commit_group;" ::: "memory");
-            // the row copies of the stage kLag behind this one have arrived
-            if (n >= kLag && (pending >> ((n - kLag) & 31) & 1)) arrived(n - kLag);
-          } else {
-            // the rows of the stage after this one go out before this one is converted
-            if (kv == 0) fetch(xv, vb, p.v_sp, p.v_ss, id, slot);
-            else if (j + 1 < units) fetch(xk, kb, p.k_sp, p.k_ss, ahead, slot_of(key + kTile));
-            if (n >= S && !(ok = tc::warp_wait(smem_u32(&bars.kv_free[st]), (n / S - 1) & 1))) break;
+          }
+          if (rows) {
 #pragma unroll
             for (int q = 0; q < PASSES; ++q) {
-              const int r = w4 * 32 + q * RP + sub;
-              const uint4 x = kv ? xv[q] : xk[q];
-              st_shared16(dst + tile_at(r, 2 * c), e4m3x2_to_f16x2(x.x), e4m3x2_to_f16x2(x.x >> 16), e4m3x2_to_f16x2(x.y),
-                          e4m3x2_to_f16x2(x.y >> 16));
-              st_shared16(dst + tile_at(r, 2 * c + 1), e4m3x2_to_f16x2(x.z), e4m3x2_to_f16x2(x.z >> 16), e4m3x2_to_f16x2(x.w),
-                          e4m3x2_to_f16x2(x.w >> 16));
+              const int r = q * RP + sub;
+              const int rid = __shfl_sync(0xffffffffu, id, r), rslot = __shfl_sync(0xffffffffu, slot, r);
+              const bool live = rid >= 0 && bytes > 0;
+              const uint32_t dst = E4M3 ? raw + n % (L::kLag + 1) * L::kRawBytes + q * 512
+                                        : base + L::kRing + st * L::kTileBytes + tile_at(w4 * 32 + r, c);
+              cp_async16(dst, live ? src + (rid * sp + rslot * ss) * ES + c * 16 : src, live ? bytes : 0);
             }
-            fence_async_proxy();
-            __syncwarp();
-            tc::arrive_if(lane == 0, smem_u32(&bars.kv_full[st]));
+            pending |= 1u << (n & 31);
           }
+          asm volatile("cp.async.commit_group;" ::: "memory");
+          if (n >= L::kLag && (pending >> ((n - L::kLag) & 31) & 1)) finish(n - L::kLag);
+          if (!ok) break;
           ++n;
         }
       }
       if (!ok) break;
     }
-    if constexpr (!E4M3) {
-      asm volatile("cp.async.wait_group 0;" ::: "memory");
-      for (uint32_t k = n > kLag ? n - kLag : 0; ok && k < n; ++k)
-        if (pending >> (k & 31) & 1) arrived(k);
-    }
+    if (ok) finish_all();
+    asm volatile("cp.async.wait_group 0;" ::: "memory");      // (none is left in flight by a wait that gave up)
     if (!ok && lane == 0) tc::report_timeout(p.status, kStatusProducerTimeout);
   } else {
     // ---- MMAs -----------------------------------------------------------------------------------------------------
@@ -635,9 +621,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tcgen05_kernel(const __
         if (n_piece >= kPieces && !(ok = tc::warp_wait(smem_u32(&bars.piece_free[i]), (n_piece / kPieces - 1) & 1))) break;
         if (lane == 0) {
           Piece &q = pieces[i];
-          q.seq = it.seq, q.b = more ? it.b : -1, q.tile = it.tile, q.head = it.head, q.unit0 = it.unit0, q.n_units = it.n_units;
+          q.seq = it.seq, q.b = more ? it.b : -1, q.head = it.head, q.unit0 = it.unit0, q.n_units = it.n_units;
           q.r0 = it.r0, q.n_rows = it.n_rows, q.first_piece = it.first_piece, q.whole = it.whole;
-          if (more) q.last_cta = it.last_cta(), q.count[0] = tile_count(p, it, 0), q.count[1] = tile_count(p, it, 1);
+          if (more) q.cut = it.cut(), q.count[0] = tile_count(p, it, 0), q.count[1] = tile_count(p, it, 1);
         }
         __syncwarp();
         tc::arrive_if(lane == 0, smem_u32(&bars.piece_full[i]));
@@ -672,7 +658,7 @@ bool page_map(CUtensorMap *map, const AttnParams &p, const void *base, const int
 
 template <typename T, bool E4M3, int DP>
 int launch(const AttnParams &p, const AttnPlan &plan, cudaStream_t st) {
-  constexpr int smem = Smem<DP>::kBytes + 1024;
+  constexpr int smem = Smem<DP, E4M3>::kBytes + 1024;
   static PerDeviceOnce once;
   auto kern = attention_tcgen05_kernel<T, E4M3, DP>;
   const int rc = allow_dynamic_smem(once, kern, smem);
