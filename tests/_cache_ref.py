@@ -142,3 +142,28 @@ def make_batch(pairs, hq, hkv, d, page, dtype=torch.bfloat16, cache=None, seed=0
                 lens=torch.tensor([kv for _, kv in pairs], dtype=torch.int32, device=device), table=table.to(device),
                 k_scale=None if ks is None else ks.to(device), v_scale=None if vs is None else vs.to(device),
                 max_q=max((n for n, _ in pairs), default=0))
+
+
+class PlainOps:
+    """The operators a decoder layer calls, evaluated plainly on the CPU (torch.ops.zentorch's names and arguments)."""
+
+    @staticmethod
+    def zentorch_rope_cache(query, key, value, positions, inv_freq, key_cache, value_cache, slot_mapping, k_scale=None, v_scale=None,
+                            interleaved=False, attention_factor=1.0):
+        q, k = (rope_ref(t, positions, inv_freq, attention_factor, interleaved)[0] for t in (query, key))
+        page = key_cache.shape[1]
+        live = slot_mapping >= 0
+        at = slot_mapping[live]
+        key_cache[at // page, at % page] = k[live].to(key_cache.dtype)
+        value_cache[at // page, at % page] = value[live].to(value_cache.dtype)
+        return q.to(query.dtype)
+
+    @staticmethod
+    def zentorch_paged_attention(query, key_cache, value_cache, cu_seqlens_q, seq_lens, block_table, max_query_len=None, scale=None,
+                                 causal=True, window=0, k_scale=None, v_scale=None):
+        return attention_ref(query, key_cache, value_cache, cu_seqlens_q, seq_lens, block_table, scale, causal, window)[0].to(query.dtype)
+
+
+def plain_copy_pages(caches, src, dst):
+    for c in caches:
+        c[dst.long()] = c[src.long()]

@@ -228,8 +228,8 @@ class DecoderLayerLinears:
         gu   = o . [Wgate | Wup]    column-parallel, fused; h = silu(gate) * up stays sharded
         down = h . Wdown            row-parallel, all-reduce
 
-    Attention itself is outside this path; `attn` is whatever buffer the caller passes (its shard of the
-    attention output).  `kind` is 'woq' or 'int8'; `full` maps a projection name to its unsharded
+    `attn` is whatever buffer the caller passes (its shard of the attention output); `DecoderLayer` below puts
+    rotary positions, the paged cache and the attention in between.  `kind` is 'woq' or 'int8'; `full` maps a projection name to its unsharded
     parameters (woq: weight [K/8, N] view, scales, zeros, bias; int8: weight [N, K], w_scales, bias).
     Every step is plain launches on the current stream plus NCCL calls, so a whole step can be captured
     in a CUDA graph and replayed without host code between the kernels."""
@@ -304,3 +304,46 @@ class DecoderLayerLinears:
                 if t is not None:
                     total += t.numel() * t.element_size()
         return total
+
+
+class DecoderLayer:
+    """A decoder layer's projections with its attention: what `DecoderLayerLinears` leaves to its caller is done by
+    `zentorch_rope_cache` (rotary positions, new keys and values into the paged cache) and `zentorch_paged_attention`:
+
+        qkv = x . [Wq | Wk | Wv];  q = rope(q), cache <- rope(k), v;  attn = attention(q, cache);  o, gate/up, down as above
+
+    `linears` are the layer's (this rank's shard), `q_heads` / `kv_heads` those of the whole layer; every rank keeps
+    its own heads' cache.  `inv_freq` and `attention_factor` come from `cache.rope_frequencies`.  A step is launches on the
+    current stream and, at more than one rank, two collectives; it can be captured in a CUDA graph (the step's tensors
+    are then the ones to refill).  `ops` replaces the operators (CPU checks); None = torch.ops.zentorch."""
+
+    def __init__(self, linears: DecoderLayerLinears, q_heads: int, kv_heads: int, head_dim: int, inv_freq: torch.Tensor,
+                 attention_factor: float = 1.0, interleaved: bool = False, window: int = 0, scale: Optional[float] = None,
+                 ops=None):
+        world = linears.world
+        if q_heads % kv_heads or kv_heads % world:
+            raise ValueError(f"{q_heads} query and {kv_heads} key/value heads do not divide over groups and {world} ranks")
+        self.linears, self.q_heads, self.kv_heads, self.head_dim = linears, q_heads // world, kv_heads // world, head_dim
+        self.inv_freq, self.attention_factor, self.interleaved = inv_freq, attention_factor, interleaved
+        self.window, self.scale, self.ops = window, scale, ops
+
+    def attention(self, qkv: torch.Tensor, cache, layer: int, step) -> torch.Tensor:
+        """The attention output [tokens, q_heads * head_dim] of a fused projection's output; the layer's cache is written."""
+        ops = self.ops if self.ops is not None else torch.ops.zentorch
+        d, sizes = self.head_dim, (self.q_heads, self.kv_heads, self.kv_heads)
+        q, k, v = (t.unflatten(-1, (-1, d)) for t in qkv.split([n * d for n in sizes], dim=-1))
+        keys, values = cache.keys(layer), cache.values(layer)
+        k_scale, v_scale = cache.scales(layer)
+        q = ops.zentorch_rope_cache(q, k, v, step.positions, self.inv_freq, keys, values, step.slots, k_scale, v_scale,
+                                    interleaved=self.interleaved, attention_factor=self.attention_factor)
+        out = ops.zentorch_paged_attention(q, keys, values, step.cu_seqlens_q, step.seq_lens, step.block_table, step.max_query_len,
+                                           scale=self.scale, window=self.window, k_scale=k_scale, v_scale=v_scale)
+        return out.flatten(1)
+
+    def __call__(self, x: torch.Tensor, cache, layer: int, step) -> torch.Tensor:
+        """x [tokens, hidden]: the new tokens of `step` (cache.PagedKVCache.step); returns the down projection's output."""
+        lin = self.linears
+        attn = self.attention(lin._lin(x, lin.qkv), cache, layer, step)
+        gu = lin._lin(lin._reduce(lin._lin(attn, lin.o)), lin.gate_up)
+        half = gu.shape[-1] // 2
+        return lin._reduce(lin._lin(torch.nn.functional.silu(gu[..., :half]) * gu[..., half:], lin.down))
