@@ -6,8 +6,9 @@
 // frequency exactly enough for positions up to 2^31), reduced to half a turn there, and only the remainder goes to fp32: a table
 // in fp32 would be 0.06 radians off at position 10^6.  The angles of a token are computed once and shared by its heads.
 //
-// Bound by memory: every element is read once and written once.  A block takes one token (several where a token has few
-// vectors); its threads have their 16-byte loads in flight while the angles are computed.
+// Bound by memory: every element is read once and written once.  A block takes up to eight tokens, as many as its 256 threads have
+// angles to compute at once, and the first 16-byte loads are in flight meanwhile: with one token per block three quarters of the
+// threads waited for the others' angles, and 8192 tokens of 64 heads took 69 us.
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
@@ -26,6 +27,8 @@ struct RopeParams {
   const float *inv_freq, *k_scale, *v_scale;
   int64_t capacity;   // slots of the cache
   int tokens, hq, hkv, d, rot, page, pos64, slot64, interleaved;
+  uint32_t magic_token, magic_rot, magic_rest, magic_whole;   // divisions by the items of a token, the vectors of a head's parts
+  int block_tokens;
   float factor;
   int *status;
 };
@@ -60,16 +63,21 @@ __device__ __forceinline__ Pack<T, VEC> load_pack(const char *base, int64_t elem
     r.e[0] = reinterpret_cast<const T *>(base)[elem];
   return r;
 }
-// VEC values to `base`, as T or, divided by `scale` and saturated, as e4m3 (round to nearest even in both).
+// VEC values to `base`, as T or, times `inv_scale` and saturated, as e4m3 (round to nearest even in both).
 template <typename T, int VEC, bool E4M3>
-__device__ __forceinline__ void store_pack(char *base, int64_t elem, const float (&v)[VEC], float scale) {
-  if constexpr (E4M3) {
-    uint8_t b[VEC];
+__device__ __forceinline__ void store_pack(char *base, int64_t elem, const float (&v)[VEC], float inv_scale) {
+  if constexpr (E4M3 && VEC == 1) {
+    base[elem] = (char)__nv_cvt_float_to_fp8(v[0] * inv_scale, __NV_SATFINITE, __NV_E4M3);
+  } else if constexpr (E4M3) {
+    uint32_t w[VEC / 4];
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) b[i] = __nv_cvt_float_to_fp8(__fdiv_rn(v[i], scale), __NV_SATFINITE, __NV_E4M3);
-    if constexpr (VEC == 8) *reinterpret_cast<uint2 *>(base + elem) = *reinterpret_cast<const uint2 *>(b);
-    else if constexpr (VEC == 4) *reinterpret_cast<uint32_t *>(base + elem) = *reinterpret_cast<const uint32_t *>(b);
-    else base[elem] = (char)b[0];
+    for (int i = 0; i < VEC; i += 4) {
+      const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[i] * inv_scale, v[i + 1] * inv_scale), __NV_SATFINITE, __NV_E4M3);
+      const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[i + 2] * inv_scale, v[i + 3] * inv_scale), __NV_SATFINITE, __NV_E4M3);
+      w[i / 4] = lo | hi << 16;
+    }
+    if constexpr (VEC == 8) *reinterpret_cast<uint2 *>(base + elem) = make_uint2(w[0], w[1]);
+    else *reinterpret_cast<uint32_t *>(base + elem) = w[0];
   } else {
     Pack<T, VEC> r;
 #pragma unroll
@@ -83,140 +91,157 @@ __device__ __forceinline__ void store_pack(char *base, int64_t elem, const float
 
 constexpr int kRopeThreads = 256;
 constexpr int kMaxHalf = 128;       // rotated pairs per head
-constexpr int kMaxTokensPerBlock = 8;
+constexpr int kMaxTokens = 8;       // of a block
 
-// blockDim = (threads of a token, tokens of a block).  A work item is one pair of vectors of a rotated head, one vector of the
-// part of a head that passes through, or one vector of a value.
+// n / d for n d < 2^32, by a multiplication with `magic` = ceil(2^32 / d) (0 for d = 1).
+__device__ __forceinline__ int quotient(int n, uint32_t magic) { return magic ? (int)__umulhi((uint32_t)n, magic) : n; }
+uint32_t magic_of(int d) { return d > 1 ? (uint32_t)(((1ull << 32) + d - 1) / d) : 0u; }
+
+// An item is two vectors: the two sides of the pairs of a rotated head, or two of the part of a head that passes through or of a
+// value (of an odd number of vectors the last item has one).  Heads are counted through: queries, keys, values; items through the block's tokens.
 template <typename T, int VEC, bool CACHE, bool E4M3>
-__global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeParams p) {
-  __shared__ float2 s_turn[kMaxTokensPerBlock][kMaxHalf];
+__global__ void __launch_bounds__(kRopeThreads, 5) rope_kernel(const __grid_constant__ RopeParams p) {
+  __shared__ float2 s_turn[kMaxTokens * kMaxHalf];      // [token][element of a vector][vector]: neighbouring lanes, neighbouring words
+  __shared__ int64_t s_row[kMaxTokens][2];              // a token's row in the caches
   grid_launch_dependents();
   grid_dependency_wait();
-  const int token = blockIdx.x * blockDim.y + threadIdx.y, half = p.rot / 2;
-  const bool live = token < p.tokens;
-  const int per_head = half / VEC, rest = (p.d - p.rot) / VEC, whole = p.d / VEC;
+  const int token0 = blockIdx.x * p.block_tokens, tokens = min(p.block_tokens, p.tokens - token0), half = p.rot / 2;
+  const int per_head = half / VEC, rest = (p.d - p.rot) / VEC, whole = p.d / VEC;     // vectors
+  const int rest_items = (rest + 1) / 2, whole_items = (whole + 1) / 2;
   const int heads = p.hq + p.hkv;
-  const int n_rot = heads * per_head, n_rest = heads * rest, n = live ? n_rot + n_rest + (CACHE ? p.hkv * whole : 0) : 0;
+  const int n_rot = heads * per_head, n_rest = n_rot + heads * rest_items, n_token = n_rest + (CACHE ? p.hkv * whole_items : 0);
+  const int n = tokens * n_token;
 
-  // where the vectors of item `it` are: input, their distance, and (head, first element)
-  auto locate = [&](int it, const char *&in, int64_t &at, int &gap, int &head, int &elem) {
+  struct Item {
+    Pack<T, VEC> x0, x1;
+    int token, head;
+    int vec0, vec1;       // the vectors of the head, vec1 < 0: there is none
+    int turn;             // rotated: number of the pair's vector, else -1
+  };
+  Item item{};
+  auto load = [&](int it, Item &i) {
+    if (it >= n) return;
+    i.token = quotient(it, p.magic_token);
+    it -= i.token * n_token;
+    i.turn = -1;
     if (it < n_rot) {
-      head = it / per_head;
-      const int j = it - head * per_head;
-      elem = p.interleaved ? 2 * j * VEC : j * VEC;
-      gap = p.interleaved ? VEC : half;
-    } else if (it < n_rot + n_rest) {
-      head = (it - n_rot) / rest;
-      elem = p.rot + (it - n_rot - head * rest) * VEC;
-      gap = 0;
+      i.head = quotient(it, p.magic_rot);
+      i.turn = it - i.head * per_head;
+      i.vec0 = p.interleaved ? 2 * i.turn : i.turn;
+      i.vec1 = p.interleaved ? i.vec0 + 1 : i.vec0 + per_head;
+    } else if (!CACHE || it < n_rest) {
+      i.head = quotient(it - n_rot, p.magic_rest);
+      i.vec0 = it - n_rot - i.head * rest_items;
+      i.vec1 = i.vec0 + rest_items < rest ? i.vec0 + rest_items + 2 * per_head : -1;
+      i.vec0 += 2 * per_head;
     } else {
-      const int r = it - n_rot - n_rest;
-      head = r / whole;
-      elem = (r - head * whole) * VEC;
-      gap = 0;
-      in = p.v;
-      at = token * p.v_st + head * p.v_sh + elem;
-      head += heads;                        // heads of the values come behind those of the keys
-      return;
+      i.head = quotient(it - n_rest, p.magic_whole);
+      i.vec0 = it - n_rest - i.head * whole_items;
+      i.vec1 = i.vec0 + whole_items < whole ? i.vec0 + whole_items : -1;
+      i.head += heads;
     }
-    if (head < p.hq) in = p.q, at = token * p.q_st + head * p.q_sh + elem;
-    else in = p.k, at = token * p.k_st + (head - p.hq) * p.k_sh + elem;
+    const int64_t token = token0 + i.token;
+    const char *in;
+    int64_t at;
+    if (i.head < p.hq) in = p.q, at = token * p.q_st + i.head * p.q_sh;
+    else if (!CACHE || i.head < heads) in = p.k, at = token * p.k_st + (i.head - p.hq) * p.k_sh;
+    else in = p.v, at = token * p.v_st + (i.head - heads) * p.v_sh;
+    i.x0 = load_pack<T, VEC>(in, at + i.vec0 * VEC);
+    if (i.vec1 >= 0) i.x1 = load_pack<T, VEC>(in, at + i.vec1 * VEC);
   };
 
-  // first item's loads before the angles, so that they are in flight meanwhile
-  const char *in = nullptr;
-  int64_t at = 0;
-  int gap = 0, head = 0, elem = 0;
-  Pack<T, VEC> x0{}, x1{};
-  int it = threadIdx.x;
-  if (it < n) {
-    locate(it, in, at, gap, head, elem);
-    x0 = load_pack<T, VEC>(in, at);
-    if (gap) x1 = load_pack<T, VEC>(in, at + gap);
+  load(threadIdx.x, item);      // in flight during the angles
+  if (CACHE && threadIdx.x < tokens) {
+    const int64_t slot = load_index(p.slots, token0 + threadIdx.x, p.slot64);
+    int64_t kc = -1, vc = 0;
+    if (slot >= 0 && slot < p.capacity) {
+      const int64_t page = slot / p.page, row = slot - page * p.page;
+      kc = page * p.kc_sp + row * p.kc_ss;
+      vc = page * p.vc_sp + row * p.vc_ss;
+    } else if (slot >= p.capacity) {
+      tc::report_timeout(p.status, kStatusBadIndex);
+    }
+    s_row[threadIdx.x][0] = kc, s_row[threadIdx.x][1] = vc;
   }
-  int64_t kc = -1, vc = 0;
-  if (live) {
-    const int64_t pos = load_index(p.positions, token, p.pos64);
-    if constexpr (CACHE) {
-      const int64_t slot = load_index(p.slots, token, p.slot64);
-      if (slot >= 0 && slot < p.capacity) {
-        const int64_t page = slot / p.page, row = slot - page * p.page;
-        kc = page * p.kc_sp + row * p.kc_ss;
-        vc = page * p.vc_sp + row * p.vc_ss;
-      } else if (slot >= p.capacity && threadIdx.x == 0) {
-        tc::report_timeout(p.status, kStatusBadIndex);
-      }
-    }
-    for (int i = threadIdx.x; i < half; i += blockDim.x) {
-      const double turns = (double)pos * ((double)p.inv_freq[i] * 0.15915494309189535);   // 1 / (2 pi)
-      float s, c;
-      sincospif(2.f * (float)(turns - rint(turns)), &s, &c);
-      s_turn[threadIdx.y][i] = make_float2(c * p.factor, s * p.factor);
-    }
+  for (int i = threadIdx.x; i < tokens * half; i += kRopeThreads) {
+    const int t = i / half, pair = i - t * half;
+    const double pos = (double)load_index(p.positions, token0 + t, p.pos64);
+    const double turns = pos * ((double)p.inv_freq[pair] * 0.15915494309189535);   // 1 / (2 pi)
+    float s, c;
+    sincospif(2.f * (float)(turns - rint(turns)), &s, &c);
+    s_turn[t * half + pair % VEC * per_head + pair / VEC] = make_float2(c * p.factor, s * p.factor);
   }
   __syncthreads();
-  while (it < n) {
-    const int next = it + blockDim.x;
+
+  auto process = [&](const Item &i) {
     float a[VEC], b[VEC];
-    const bool rotated = gap != 0;
-    if (rotated) {
+    if (i.turn >= 0) {
       float u[2 * VEC];
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) u[i] = to_f32<T>(x0.e[i]), u[VEC + i] = to_f32<T>(x1.e[i]);
-      const int pair = p.interleaved ? elem / 2 : elem;
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const float2 t = s_turn[threadIdx.y][pair + i];
-        const float first = p.interleaved ? u[2 * i] : u[i], second = p.interleaved ? u[2 * i + 1] : u[VEC + i];
-        a[i] = first * t.x - second * t.y;
-        b[i] = second * t.x + first * t.y;
-      }
+      for (int e = 0; e < VEC; ++e) u[e] = to_f32<T>(i.x0.e[e]), u[VEC + e] = to_f32<T>(i.x1.e[e]);
+      const float2 *turn = s_turn + i.token * half + i.turn;
       if (p.interleaved) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) u[2 * i] = a[i], u[2 * i + 1] = b[i];
+        for (int e = 0; e < VEC; ++e) {
+          const float2 t = turn[e * per_head];
+          const float first = u[2 * e], second = u[2 * e + 1];
+          u[2 * e] = first * t.x - second * t.y, u[2 * e + 1] = second * t.x + first * t.y;
+        }
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) a[i] = u[i], b[i] = u[VEC + i];
+        for (int e = 0; e < VEC; ++e) a[e] = u[e], b[e] = u[VEC + e];
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const float2 t = turn[e * per_head];
+          a[e] = u[e] * t.x - u[VEC + e] * t.y, b[e] = u[VEC + e] * t.x + u[e] * t.y;
+        }
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) a[i] = to_f32<T>(x0.e[i]);
+      for (int e = 0; e < VEC; ++e) a[e] = to_f32<T>(i.x0.e[e]), b[e] = to_f32<T>(i.x1.e[e]);
     }
-    const int this_head = head, this_elem = elem, this_gap = gap;
-    if (next < n) {
-      locate(next, in, at, gap, head, elem);
-      x0 = load_pack<T, VEC>(in, at);
-      if (gap) x1 = load_pack<T, VEC>(in, at + gap);
-    }
-    if (this_head < p.hq) {
-      const int64_t o = token * p.qo_st + this_head * p.qo_sh + this_elem;
-      store_pack<T, VEC, false>(p.q_out, o, a, 1.f);
-      if (rotated) store_pack<T, VEC, false>(p.q_out, o + this_gap, b, 1.f);
+    const int e0 = i.vec0 * VEC, e1 = i.vec1 * VEC;
+    const int64_t token = token0 + i.token;
+    if (i.head < p.hq) {
+      const int64_t o = token * p.qo_st + i.head * p.qo_sh;
+      store_pack<T, VEC, false>(p.q_out, o + e0, a, 1.f);
+      if (e1 >= 0) store_pack<T, VEC, false>(p.q_out, o + e1, b, 1.f);
     } else if constexpr (CACHE) {
-      if (kc >= 0) {
-        const int h = this_head < heads ? this_head - p.hq : this_head - heads;
-        const bool value = this_head >= heads;
-        const int64_t o = (value ? vc + h * p.vc_sh : kc + h * p.kc_sh) + this_elem;
-        const float scale = E4M3 ? (value ? p.v_scale[h] : p.k_scale[h]) : 1.f;
+      const bool value = i.head >= heads;
+      const int64_t row = s_row[i.token][value];
+      if (s_row[i.token][0] >= 0) {
+        const int h = i.head - (value ? heads : p.hq);
+        const int64_t o = row + h * (value ? p.vc_sh : p.kc_sh);
+        const float inv_scale = E4M3 ? __frcp_rn(value ? p.v_scale[h] : p.k_scale[h]) : 1.f;
         char *base = value ? p.v_cache : p.k_cache;
-        store_pack<T, VEC, E4M3>(base, o, a, scale);
-        if (rotated) store_pack<T, VEC, E4M3>(base, o + this_gap, b, scale);
+        store_pack<T, VEC, E4M3>(base, o + e0, a, inv_scale);
+        if (e1 >= 0) store_pack<T, VEC, E4M3>(base, o + e1, b, inv_scale);
       }
     } else {
-      const int64_t o = token * p.ko_st + (this_head - p.hq) * p.ko_sh + this_elem;
-      store_pack<T, VEC, false>(p.k_out, o, a, 1.f);
-      if (rotated) store_pack<T, VEC, false>(p.k_out, o + this_gap, b, 1.f);
+      const int64_t o = token * p.ko_st + (i.head - p.hq) * p.ko_sh;
+      store_pack<T, VEC, false>(p.k_out, o + e0, a, 1.f);
+      if (e1 >= 0) store_pack<T, VEC, false>(p.k_out, o + e1, b, 1.f);
     }
-    it = next;
+  };
+  for (int it = threadIdx.x; it < n; it += kRopeThreads) {
+    process(item);
+    load(it + kRopeThreads, item);
   }
 }
 
 template <typename T, int VEC>
-cudaError_t launch_rope(const RopeParams &p, int cache, cudaStream_t st) {   // cache: 0 none, 1 of the inputs' type, 2 e4m3
-  const int items = (p.hq + p.hkv) * (p.rot / 2 / VEC + (p.d - p.rot) / VEC) + (cache ? p.hkv * (p.d / VEC) : 0);
-  int tx = 32;
-  while (tx < kRopeThreads && tx < items) tx *= 2;
-  const int ty = kRopeThreads / tx;
-  const dim3 grid((unsigned)ceil_div(p.tokens, ty)), block(tx, ty);
+cudaError_t launch_rope(RopeParams p, int cache, cudaStream_t st) {   // cache: 0 none, 1 of the inputs' type, 2 e4m3
+  const int rot = p.rot / 2 / VEC, rest = ((p.d - p.rot) / VEC + 1) / 2, whole = (p.d / VEC + 1) / 2;      // items of a head
+  p.magic_rot = magic_of(rot), p.magic_rest = magic_of(rest), p.magic_whole = magic_of(whole);
+  const int items = (p.hq + p.hkv) * (rot + rest) + (cache ? p.hkv * whole : 0);
+  p.magic_token = magic_of(items);
+  // as many tokens as give every thread an angle, or (tokens of few items) an item; fewer where that leaves SMs without a block
+  const int by_angles = p.rot > 0 ? kRopeThreads / (p.rot / 2) : kMaxTokens, by_items = ceil_div(kRopeThreads, items);
+  int t = by_angles > by_items ? by_angles : by_items;
+  const int spread = ceil_div(p.tokens, 2 * sm_count());
+  if (t > spread) t = spread;
+  p.block_tokens = t < 1 ? 1 : t > kMaxTokens ? kMaxTokens : t;
+  const dim3 grid((unsigned)ceil_div(p.tokens, p.block_tokens)), block(kRopeThreads);
   if (cache == 0) return launch_overlapped(rope_kernel<T, VEC, false, false>, grid, block, (size_t)0, st, p);
   if (cache == 1) return launch_overlapped(rope_kernel<T, VEC, true, false>, grid, block, (size_t)0, st, p);
   return launch_overlapped(rope_kernel<T, VEC, true, true>, grid, block, (size_t)0, st, p);
