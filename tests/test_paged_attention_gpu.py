@@ -204,6 +204,40 @@ def test_nan_in_a_key_reaches_the_rows_that_see_it(capi, algo):
     assert torch.equal(got[:2], clean[:2]) and got[2:].isnan().all()
 
 
+@pytest.mark.parametrize("algo", ALGOS)
+@pytest.mark.parametrize("cache", ["same", "e4m3"])
+@pytest.mark.parametrize("dtype,d", [(BF16, 64), (F16, 128)])
+@pytest.mark.parametrize("n,kv,window", [(4, 40, 0), (30, 300, 100), (200, 400, 0), (300, 300, 7)])
+def test_values_that_are_not_finite_reach_only_rows_that_see_them(capi, algo, cache, dtype, d, n, kv, window):
+    """NaN and infinities in values of keys that some rows of a tile see and others do not: the latter keep their results, the former
+    get them in their columns and nowhere else.  What is finite is held to the bound of every other test (rows that the tensor
+    cores spoilt are summed again in another order, so bits may differ); the streaming kernel leaves even the bits."""
+    c = make_batch([(1, 20), (n, kv), (3, 9)], 4, 2, d, 16, dtype, E4M3 if cache == "e4m3" else dtype, seed=26)
+    clean = run(capi, c, algo, window=window)
+    raw = c["v_cache"].view(torch.uint8) if cache == "e4m3" else c["v_cache"]
+    special = [(kv - 2, 0, 3, float("nan")), (kv - n // 2, 1, 17, float("inf")), (kv - n // 2, 1, d - 1, float("-inf")),
+               (max(kv - n - 1, 0), 0, 30, float("nan")), (kv - 1, 1, 8, float("inf")), (kv - 1, 1, 17, float("-inf"))]
+    want = clean.double()
+    pos = torch.arange(kv - n, kv, device="cuda")
+    for key, h, col, value in special:
+        if cache == "e4m3":
+            value = float("nan")                                # the type has no infinities
+        raw[c["table"][1, key // 16].long(), key % 16, h, col] = 0x7f if cache == "e4m3" else value
+        sees = (pos >= key) & ((pos - window < key) if window else True)
+        want[1:1 + n, 2 * h:2 * h + 2, col] += torch.where(sees, value, 0.0).unsqueeze(1)
+    got = run(capi, c, algo, window=window)
+    fine = torch.isfinite(want)
+    assert not fine.all()
+    if algo == "skinny":
+        assert torch.equal(got[fine], clean[fine])
+    ref, bound = attention_ref(c["q"], c["k_cache"], c["v_cache"], c["cu"], c["lens"], c["table"], window=window, k_scale=c["k_scale"],
+                               v_scale=c["v_scale"])
+    keep = fine.cpu()
+    assert torch.equal(torch.isfinite(ref), keep)
+    assert bool(((got.double().cpu() - ref).abs()[keep] <= bound[keep]).all())
+    assert torch.equal(got.double()[~fine].nan_to_num(5e4, 6e4, 7e4), want[~fine].nan_to_num(5e4, 6e4, 7e4))
+
+
 def test_bad_pages_and_lengths_are_reported(capi):
     c = make_batch([(1, 60), (1, 100)], 4, 2, 64, 16, BF16, seed=20)
     good = run(capi, c)

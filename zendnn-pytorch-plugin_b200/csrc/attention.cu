@@ -18,7 +18,7 @@ template <typename T, int DP>
 __global__ void __launch_bounds__(kCombineWarps * 32) attention_combine_kernel(const __grid_constant__ AttnParams p, int R) {
   grid_launch_dependents();
   grid_dependency_wait();
-  const int4 item = p.meta[blockIdx.x];
+  const int4 item = p.meta[blockIdx.x].cut;
   if (item.x < 0) return;
   const int row = blockIdx.y * kCombineWarps + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (row >= item.z % 512) return;
@@ -64,50 +64,145 @@ __global__ void __launch_bounds__(kCombineWarps * 32) attention_combine_kernel(c
     *reinterpret_cast<uint32_t *>(dst) = pack2(acc[0] * f, acc[1] * f, T(0.f));
 }
 
+// One element of a cache.
+template <typename T, bool E4M3>
+__device__ __forceinline__ float cache_value(const void *base, int64_t at) {
+  if constexpr (E4M3) {
+    const uint2 h = e4m3x4_to_f16x4(reinterpret_cast<const uint8_t *>(base)[at]);
+    return unpack2(h.x, __half(0.f)).x;
+  } else {
+    return (float)reinterpret_cast<const T *>(base)[at];
+  }
+}
+
+// Goes through a row of the output again, by one warp, where it is not finite: unless every such column has a value that is not
+// finite among the keys that the row sees, the row is computed from those keys alone.
+template <typename T, bool E4M3>
+__device__ __noinline__ void redo_row(const AttnParams &p, int b, const SeqInfo &seq, int head, int r) {
+  constexpr int V = 4;                                   // columns of a lane
+  const int lane = threadIdx.x & 31, tok = r / p.group, qh = head * p.group + r % p.group;
+  const int lo = key_lo(p, seq, tok), hi = key_hi(p, seq, tok);
+  T *out = reinterpret_cast<T *>(p.out) + (seq.q0 + tok) * p.o_st + qh * p.o_sh;
+  const T *q = reinterpret_cast<const T *>(p.q) + (seq.q0 + tok) * p.q_st + qh * p.q_sh;
+  auto row_of = [&](int key, int64_t sp, int64_t ss, int64_t sh) -> int64_t {      // -1: no such page
+    const int id = p.table[b * p.table_stride + page_of(p, key)];
+    return id >= 0 && id < p.num_pages ? id * sp + (key - page_of(p, key) * p.page) * ss + head * sh : -1;
+  };
+  uint32_t open = 0;                                     // this lane's columns that want an explanation
+#pragma unroll
+  for (int e = 0; e < V; ++e)
+    if (lane * V + e < p.d && !isfinite((float)out[lane * V + e])) open |= 1u << e;
+  if (!__any_sync(0xffffffffu, open != 0)) return;
+  for (int key = hi - 1; key >= lo && __any_sync(0xffffffffu, open != 0); --key) {
+    const int64_t at = row_of(key, p.v_sp, p.v_ss, p.v_sh);
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      if (at >= 0 && (open >> e & 1) && !isfinite(cache_value<T, E4M3>(p.v, at + lane * V + e))) open &= ~(1u << e);
+  }
+  if (!__any_sync(0xffffffffu, open != 0)) return;
+  const float mul = p.scale_log2 * (E4M3 ? p.k_scale[head] : 1.f);
+  float acc[V] = {}, top = -INFINITY, sum = 0.f;
+  for (int first = lo; first < hi; first += 32) {        // a key per lane, then its value by all lanes
+    const int key = first + lane;
+    float s = -INFINITY;
+    if (key < hi) {
+      const int64_t at = row_of(key, p.k_sp, p.k_ss, p.k_sh);
+      s = 0.f;
+      if (at >= 0)
+        for (int e = 0; e < p.d; ++e) s = fmaf((float)q[e], cache_value<T, E4M3>(p.k, at + e), s);
+      s *= mul;
+    }
+    float to = s;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) to = fmaxf(to, __shfl_xor_sync(0xffffffffu, to, o));
+    to = fmaxf(to, top);
+    const float f = top == -INFINITY ? 0.f : exp2_fast(top - to), x = key < hi ? exp2_fast(s - (to == -INFINITY ? 0.f : to)) : 0.f;
+    top = to;
+    sum = sum * f + x;
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[e] *= f;
+    for (int i = 0; i < min(32, hi - first); ++i) {
+      const float xi = __shfl_sync(0xffffffffu, x, i);
+      const int64_t at = row_of(first + i, p.v_sp, p.v_ss, p.v_sh);
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (at >= 0 && lane * V + e < p.d) acc[e] = fmaf(xi, cache_value<T, E4M3>(p.v, at + lane * V + e), acc[e]);
+    }
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  const float f = sum == 0.f ? 0.f : (E4M3 ? p.v_scale[head] : 1.f) / sum;
+#pragma unroll
+  for (int e = 0; e < V; ++e)
+    if (lane * V + e < p.d) out[lane * V + e] = (T)(acc[e] * f);
+}
+
 // The same for the pieces of the tcgen05 kernel, whose rows are neighbours in the workspace: a lane per row, a warp per 16 columns.
-template <typename T, int DP>
+// A block whose CTA found outputs that are not finite goes through the rows of its items again.
+template <typename T, bool E4M3, int DP>
 __global__ void __launch_bounds__(DP * 2) attention_combine_rows_kernel(const __grid_constant__ AttnParams p, int R) {
   grid_launch_dependents();
   grid_dependency_wait();
-  const int4 item = p.meta[blockIdx.x];
-  if (item.x < 0) return;
-  const int row = blockIdx.y * 32 + (threadIdx.x & 31), c0 = (threadIdx.x >> 5) * 16;
-  const int first = blockIdx.x, count = item.w - first + 1;
-  if (row >= item.z % 512 || c0 >= p.d) return;
-  auto slot = [&](int i) { return (int64_t)(2 * (first + i) + (i == 0 ? 1 : 0)); };
-  float acc[16] = {}, sum = 0.f, top = -INFINITY;
-  for (int i = 0; i < count; ++i) {
-    const float2 ml = p.part_ml[slot(i) * R + row];
-    const float4 *src = reinterpret_cast<const float4 *>(p.part_o) + (slot(i) * (DP / 4) + c0 / 4) * R + row;
-    float4 x[4];
+  const AttnMeta &meta = p.meta[blockIdx.x];
+  const int4 item = meta.cut;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = blockIdx.y * 32 + lane, c0 = warp * 16;
+  bool redo = meta.not_finite;
+  if (item.x >= 0) {
+    const int first = blockIdx.x, count = item.w - first + 1, n_rows = item.z % 512;
+    if (row < n_rows && c0 < p.d) {
+      auto slot = [&](int i) { return (int64_t)(2 * (first + i) + (i == 0 ? 1 : 0)); };
+      float acc[16] = {}, sum = 0.f, top = -INFINITY;
+      for (int i = 0; i < count; ++i) {
+        const float2 ml = p.part_ml[slot(i) * R + row];
+        const float4 *src = reinterpret_cast<const float4 *>(p.part_o) + (slot(i) * (DP / 4) + c0 / 4) * R + row;
+        float4 x[4];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) x[q] = src[(int64_t)q * R];
-    const float to = fmaxf(top, ml.x);
-    const float f_old = top == -INFINITY ? 0.f : exp2_fast(top - to), f = ml.x == -INFINITY ? 0.f : exp2_fast(ml.x - to);
-    top = to;
-    sum = sum * f_old + ml.y * f;
+        for (int q = 0; q < 4; ++q) x[q] = src[(int64_t)q * R];
+        const float to = fmaxf(top, ml.x);
+        const float f_old = top == -INFINITY ? 0.f : exp2_fast(top - to), f = ml.x == -INFINITY ? 0.f : exp2_fast(ml.x - to);
+        top = to;
+        sum = sum * f_old + ml.y * f;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      acc[4 * q] = acc[4 * q] * f_old + x[q].x * f, acc[4 * q + 1] = acc[4 * q + 1] * f_old + x[q].y * f;
-      acc[4 * q + 2] = acc[4 * q + 2] * f_old + x[q].z * f, acc[4 * q + 3] = acc[4 * q + 3] * f_old + x[q].w * f;
+        for (int q = 0; q < 4; ++q) {
+          acc[4 * q] = acc[4 * q] * f_old + x[q].x * f, acc[4 * q + 1] = acc[4 * q + 1] * f_old + x[q].y * f;
+          acc[4 * q + 2] = acc[4 * q + 2] * f_old + x[q].z * f, acc[4 * q + 3] = acc[4 * q + 3] * f_old + x[q].w * f;
+        }
+      }
+      const float f = top == -INFINITY ? 0.f : 1.f / sum;
+      const int r = item.y + row, tok = r / p.group, qh = item.z / 512 * p.group + r % p.group;
+      uint4 *dst = reinterpret_cast<uint4 *>(reinterpret_cast<char *>(p.out) + ((item.x + tok) * p.o_st + qh * p.o_sh + c0) * 2);
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+        if (c0 + 8 * q < p.d)
+          dst[q] = make_uint4(pack2(acc[8 * q] * f, acc[8 * q + 1] * f, T(0.f)), pack2(acc[8 * q + 2] * f, acc[8 * q + 3] * f, T(0.f)),
+                              pack2(acc[8 * q + 4] * f, acc[8 * q + 5] * f, T(0.f)), pack2(acc[8 * q + 6] * f, acc[8 * q + 7] * f, T(0.f)));
     }
+    int others = 0;       // any CTA that worked on the cut item
+    for (int i = 1 + lane; i < count; i += 32) others |= p.meta[first + i].not_finite;
+    redo |= __any_sync(0xffffffffu, others) != 0;
   }
-  const float f = top == -INFINITY ? 0.f : 1.f / sum;
-  const int r = item.y + row, tok = r / p.group, qh = item.z / 512 * p.group + r % p.group;
-  uint4 *dst = reinterpret_cast<uint4 *>(reinterpret_cast<char *>(p.out) + ((item.x + tok) * p.o_st + qh * p.o_sh + c0) * 2);
-#pragma unroll
-  for (int q = 0; q < 2; ++q)
-    if (c0 + 8 * q < p.d)
-      dst[q] = make_uint4(pack2(acc[8 * q] * f, acc[8 * q + 1] * f, T(0.f)), pack2(acc[8 * q + 2] * f, acc[8 * q + 3] * f, T(0.f)),
-                          pack2(acc[8 * q + 4] * f, acc[8 * q + 5] * f, T(0.f)), pack2(acc[8 * q + 6] * f, acc[8 * q + 7] * f, T(0.f)));
+  if (!redo) return;
+  __syncthreads();        // this block's part of the cut item is written
+  if (item.x >= 0) {
+    const SeqInfo seq = load_seq(p, meta.cut_b);
+    for (int i = warp; i < 32; i += DP * 2 / 32)
+      if (blockIdx.y * 32 + i < item.z % 512) redo_row<T, E4M3>(p, meta.cut_b, seq, item.z / 512, item.y + blockIdx.y * 32 + i);
+  }
+  if (!meta.not_finite) return;
+  AttnWalk<kTcgen05Rows, kTcgen05Unit, kTcgen05Extra> it(meta.range);
+  while (it.next(p)) {
+    if (!it.whole) continue;      // (the block of the item's first CTA has it)
+    for (int i = warp; i < 32; i += DP * 2 / 32)
+      if (blockIdx.y * 32 + i < it.n_rows) redo_row<T, E4M3>(p, it.b, it.seq, it.head, it.r0 + blockIdx.y * 32 + i);
+  }
 }
 
-template <typename T>
+template <typename T, bool E4M3>
 cudaError_t launch_combine(const AttnParams &p, const AttnPlan &plan, cudaStream_t st) {
   if (plan.tcgen05) {
     const dim3 grid((unsigned)plan.grid, (unsigned)(plan.rows / 32)), block((unsigned)plan.dp * 2);
-    return plan.dp == 64 ? launch_overlapped(attention_combine_rows_kernel<T, 64>, grid, block, (size_t)0, st, p, plan.rows)
-                         : launch_overlapped(attention_combine_rows_kernel<T, 128>, grid, block, (size_t)0, st, p, plan.rows);
+    return plan.dp == 64 ? launch_overlapped(attention_combine_rows_kernel<T, E4M3, 64>, grid, block, (size_t)0, st, p, plan.rows)
+                         : launch_overlapped(attention_combine_rows_kernel<T, E4M3, 128>, grid, block, (size_t)0, st, p, plan.rows);
   }
   const dim3 grid((unsigned)plan.grid, (unsigned)ceil_div(plan.rows, kCombineWarps)), block(kCombineWarps * 32);
   return plan.dp == 64 ? launch_overlapped(attention_combine_kernel<T, 64>, grid, block, (size_t)0, st, p, plan.rows)
@@ -125,13 +220,13 @@ AttnPlan make_plan(const zt_paged_attention_args_t &a) {
   const int64_t rows = longest * group;
   plan.tcgen05 = a.algo == ZT_ALGO_TCGEN05 || (a.algo == ZT_ALGO_AUTO && rows > kMaxStreamRows);
   plan.dp = a.head_dim <= 64 ? 64 : 128;
-  plan.rows = plan.tcgen05 ? 256 : rows <= 16 ? 16 : 32;
+  plan.rows = plan.tcgen05 ? kTcgen05Rows : rows <= 16 ? 16 : 32;
   plan.grid = plan.tcgen05 ? sm_count() : attention_stream_grid(plan.rows);
   plan.few = rows <= 4 * plan.rows;
   // units of the whole call at most (an item has up to three beside those of its keys)
   const int64_t unit = plan.tcgen05 ? 128 : 64, tiles = a.tokens * group / plan.rows + a.batch;
   plan.most_units = (double)tiles * a.kv_heads * (double)((int64_t)a.page_size * a.max_blocks / unit + 4);
-  plan.meta_bytes = align256((size_t)plan.grid * sizeof(int4));
+  plan.meta_bytes = align256((size_t)plan.grid * sizeof(AttnMeta));
   plan.ml_bytes = align256((size_t)2 * plan.grid * plan.rows * sizeof(float2));
   plan.o_bytes = align256((size_t)2 * plan.grid * plan.rows * plan.dp * sizeof(float));
   return plan;
@@ -210,7 +305,7 @@ extern "C" int zt_paged_attention(const zt_paged_attention_args_t *a, void *stre
     if (a->page_size == 1 << s) p.page_shift = s;
   p.causal = a->causal != 0, p.window = a->window, p.scale_log2 = a->scale * 1.4426950408889634f, p.zero_tail = a->zero_tail != 0, p.few = plan.few;
   char *ws = reinterpret_cast<char *>(a->workspace);
-  p.meta = reinterpret_cast<int4 *>(ws);
+  p.meta = reinterpret_cast<AttnMeta *>(ws);
   p.part_ml = reinterpret_cast<float2 *>(ws + plan.meta_bytes);
   p.part_o = reinterpret_cast<float *>(ws + plan.meta_bytes + plan.ml_bytes);
   p.status = status;
@@ -219,6 +314,7 @@ extern "C" int zt_paged_attention(const zt_paged_attention_args_t *a, void *stre
   const int rc = plan.tcgen05 ? attention_tcgen05_launch(p, plan, a->dtype, a->cache_dtype, st)
                               : attention_stream_launch(p, plan, a->dtype, a->cache_dtype, st);
   if (rc != ZT_SUCCESS) return rc;
-  ZT_CUDA_OK(a->dtype == ZT_BF16 ? launch_combine<__nv_bfloat16>(p, plan, st) : launch_combine<__half>(p, plan, st));
+  ZT_CUDA_OK(a->dtype == ZT_BF16 ? (e4m3 ? launch_combine<__nv_bfloat16, true>(p, plan, st) : launch_combine<__nv_bfloat16, false>(p, plan, st))
+                                 : (e4m3 ? launch_combine<__half, true>(p, plan, st) : launch_combine<__half, false>(p, plan, st)));
   return launch_status("attention_combine_kernel");
 }

@@ -38,9 +38,22 @@ struct AttnParams {
   int zero_tail;                                // rows behind the last sequence are zeroed
   float *part_o;                                // [2 * grid][R][DP]
   float2 *part_ml;                              // [2 * grid][R]: maximum (log2 units), sum
-  int4 *meta;                                   // [grid]: the item cut at the end of a CTA's range: first new token of its sequence
-                                                // or -1, first row, head * 512 + rows, last CTA
+  struct AttnMeta *meta;                        // [grid]
   int *status;
+};
+
+// Where a CTA's range begins: units [w0, w1) of all, w0 within the tile whose first unit (over its kv heads) is number `item0`.
+// `per` units per CTA.  The host has checked that all units fit an int.
+struct AttnRange {
+  int w0, w1, per, item0;
+  int b, tile;
+};
+// What a CTA leaves for the kernel that joins the cut items.
+struct AttnMeta {
+  int4 cut;           // the item cut at the end of its range: first new token of its sequence or -1, first row, head * 512 + rows, last CTA
+  int cut_b;          // that item's sequence (tcgen05 kernel, as the rest)
+  AttnRange range;
+  int not_finite;     // some output of an item whose rows see different keys is not finite
 };
 
 struct AttnPlan {         // of one call, on the host
@@ -56,6 +69,8 @@ int attention_tcgen05_launch(const AttnParams &p, const AttnPlan &plan, int dtyp
 int attention_stream_grid(int rows);
 
 #ifdef __CUDACC__
+constexpr int kTcgen05Rows = 256, kTcgen05Unit = 128, kTcgen05Extra = 3;   // rows of an item, keys of a unit, units that an item costs beside its own
+
 constexpr float kLazyRescale = 8.f;   // log2 units that a running maximum may lag behind before sums are rescaled
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -139,12 +154,6 @@ __device__ __forceinline__ int block_scan(int v, int *scratch, int &total) {
   return (warp ? before : 0) + x - v;
 }
 
-// Where a CTA's range begins: units [w0, w1) of all, w0 within the tile whose first unit (over its kv heads) is number `item0`.
-// `per` units per CTA.  The host has checked that all units fit an int.
-struct AttnRange {
-  int w0, w1, per, item0;
-  int b, tile;
-};
 struct AttnScratch {
   int scan[2][32], found[3];
 };
@@ -295,6 +304,31 @@ __device__ __forceinline__ float2 unpack2(uint32_t w, __half) { return __half22f
 __device__ __forceinline__ int row_exponent(float top) {
   return top > 0.f && top < __int_as_float(0x7f800000) ? min(max(ilogbf(top), -126), 126) : 0;
 }
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, int bytes) {   // the rest of the 16 is zero
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void st_shared16(uint32_t dst, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ uint4 ld_shared16(uint32_t src) {
+  uint4 x;
+  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(src) : "memory");
+  return x;
+}
+
+// Values that are not finite.  A probability of zero times such a value would reach rows that do not see its key, so where the rows
+// of a tile see different keys those values are taken out of the product and added to the rows that do see them.
+// Mask over the bits of the elements of `w` that are not finite: two of M, or four e4m3.
+__device__ __forceinline__ uint32_t not_finite_mask(uint32_t w, __nv_bfloat16) {
+  return (((w & 0x7f807f80u) + 0x00800080u) >> 15 & 0x00010001u) * 0xffffu;
+}
+__device__ __forceinline__ uint32_t not_finite_mask(uint32_t w, __half) {
+  return (((w & 0x7c007c00u) + 0x04000400u) >> 15 & 0x00010001u) * 0xffffu;
+}
+__device__ __forceinline__ uint32_t not_finite_mask_e4m3(uint32_t w) {
+  return (((w & 0x7f7f7f7fu) + 0x01010101u) >> 7 & 0x01010101u) * 0xffu;
+}
+
 // Four e4m3 values as halves, in order; exact.
 __device__ __forceinline__ uint2 e4m3x4_to_f16x4(uint32_t four) {
   uint2 r;

@@ -35,13 +35,15 @@ __host__ __device__ constexpr int ring_bytes() { return kWarps * stages<E4M3, MT
 template <int R, int DP>
 __host__ __device__ constexpr int merge_bytes() { return kWarps * R * (DP + 8) * 4 + kWarps * R * 8; }
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, int bytes) {   // the rest of the 16 is zero
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
+__device__ __forceinline__ uint32_t ld_shared4(uint32_t src) {
+  uint32_t x;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(x) : "r"(src) : "memory");
+  return x;
+}
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -85,7 +87,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<MT>()) attention_stream_
   const uint32_t ring_addr = smem_u32(ring);
   float *merge_o = reinterpret_cast<float *>(smem);                                   // [warp][R][DP + 8]
   float2 *merge_ml = reinterpret_cast<float2 *>(smem + kWarps * R * (DP + 8) * 4);    // [warp][R]
-  if (threadIdx.x == 0) p.meta[blockIdx.x] = make_int4(-1, 0, 0, 0);
+  if (threadIdx.x == 0) p.meta[blockIdx.x].cut.x = -1;
 
   AttnWalk<R, kUnit, kExtra> it(range);
   while (it.next(p)) {
@@ -314,6 +316,49 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<MT>()) attention_stream_
           pf[m][2 + half] = pack2(x[2], x[3], M(0.f));
         }
       }
+      if (!inside && tok0 != tok1) {     // rows that see different keys: values that are not finite apart
+        auto bad = [&](uint32_t w) { return E4M3 ? not_finite_mask_e4m3(w) : not_finite_mask(w, M(0.f)); };
+        constexpr int PER_LANE = kKeys * CH / 32;
+        uint32_t any = 0;
+#pragma unroll
+        for (int q = 0; q < PER_LANE; ++q) {
+          const uint4 x = ld_shared16(vs + (q * 32 + lane) * 16);
+          any |= bad(x.x) | bad(x.y) | bad(x.z) | bad(x.w);
+        }
+        if (__any_sync(0xffffffffu, any != 0)) {
+#pragma unroll 1
+          for (int r = 0; r < kKeys; ++r) {
+            const int key = kbase + r;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {       // this lane's two columns of tile n
+              const uint32_t w = ld_shared4(frag_addr(vs, r, E4M3 ? n / 2 : n) + t4 * 4), x = w & bad(w);
+              float2 f;
+              if constexpr (E4M3) {
+                const uint2 h = e4m3x4_to_f16x4(__byte_perm(x, 0, 0x3120));
+                f = unpack2(n & 1 ? h.y : h.x, M(0.f));
+              } else {
+                f = unpack2(x, M(0.f));
+              }
+#pragma unroll
+              for (int m = 0; m < MT; ++m) {
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                  if (key < max(lo[m][half], k_begin) || key >= min(hi[m][half], k_end)) continue;
+                  o[m][n][2 * half] += f.x, o[m][n][2 * half + 1] += f.y;
+                }
+              }
+            }
+          }
+          __syncwarp();
+#pragma unroll
+          for (int q = 0; q < PER_LANE; ++q) {
+            const uint32_t at = vs + (q * 32 + lane) * 16;
+            const uint4 x = ld_shared16(at);
+            st_shared16(at, x.x & ~bad(x.x), x.y & ~bad(x.y), x.z & ~bad(x.z), x.w & ~bad(x.w));
+          }
+          __syncwarp();
+        }
+      }
       // output rows
       if constexpr (!E4M3) {
 #pragma unroll
@@ -414,7 +459,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<MT>()) attention_stream_
         if (c == 0) p.part_ml[(int64_t)slot * R + row] = make_float2(best, l);
       }
     }
-    if (threadIdx.x == 0 && !it.whole && it.first_piece) p.meta[blockIdx.x] = it.cut();
+    if (threadIdx.x == 0 && !it.whole && it.first_piece) p.meta[blockIdx.x].cut = it.cut();
     __syncthreads();   // the merge area is read before the next rings fill it
   }
 }

@@ -13,6 +13,11 @@
 //   warp 12          issues the MMAs
 //   warp 13          walks the CTA's range and hands its pieces to the others
 //
+// Where the rows of an item see different keys, a probability of zero meets the values of the others, and one that is not finite
+// spoils rows that do not see it.  The rows look at their output, which costs next to nothing, and note a CTA that found some not
+// finite; the kernel after this one, which joins the cut items, goes through those rows again (taking such values out of the
+// products here cost 10 - 40 %, by the size of the code alone).
+//
 // The reference of the exponents follows the row maximum only when that has run 8 (log2) ahead of it, so the rows of O are
 // rescaled a few times at the start and hardly ever after; the thread that finds it does it itself.  Probabilities are rounded
 // to the products' type; their sum is of the unrounded fp32 values.  e4m3: fp16 products, query rows brought below 2 by a power of
@@ -23,10 +28,10 @@ namespace zt {
 
 namespace {
 
-constexpr int kTile = 128;                 // rows of a tile, keys of a unit
-constexpr int kRows = 2 * kTile;
+constexpr int kTile = kTcgen05Unit;         // rows of a tile, keys of a unit
+constexpr int kRows = kTcgen05Rows;
 constexpr int kThreads = 512;              // four warpgroups: tile 0, tile 1, copies, MMA and walk (and two idle warps)
-constexpr int kExtra = 3;                  // units that an item costs beside its own
+constexpr int kExtra = kTcgen05Extra;
 constexpr int kHalf = kTile * 128;         // bytes of 64 columns of a tile: 128 rows of 128 bytes, swizzled
 constexpr int kBoxSlots = 32;              // slots of a page per TMA box, at most
 
@@ -45,17 +50,6 @@ struct Smem {
 constexpr int kRegsRows = 152, kRegsCopy = 104, kRegsMma = 104;
 static_assert(2 * kRegsRows + kRegsCopy + kRegsMma <= 4 * 128, "register split above the launch's registers");
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, int bytes) {   // the rest of the 16 is zero
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void st_shared16(uint32_t dst, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
-}
-__device__ __forceinline__ uint4 ld_shared16(uint32_t src) {
-  uint4 x;
-  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(src) : "memory");
-  return x;
-}
 __device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // Byte offset of 16-byte chunk `c` of row `row` in a tile.
@@ -94,6 +88,7 @@ struct Barriers {
   uint64_t kv_full[8], kv_free[8];
   uint64_t q_full[2], s_full[2], p_half[2], p_full[2], o_full[2];
   uint64_t piece_full[4], piece_free[4];
+  uint32_t not_finite;           // some output that may be another row's doing
   uint32_t tmem;
 };
 
@@ -139,6 +134,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tcgen05_kernel(const __
       tc::mbar_init(&bars.s_full[i], 1), tc::mbar_init(&bars.o_full[i], 1);
     }
     for (int i = 0; i < kPieces; ++i) tc::mbar_init(&bars.piece_full[i], 1), tc::mbar_init(&bars.piece_free[i], kPieceReaders);
+    bars.not_finite = 0;
     tc::mbar_fence_init();
   }
   if (warp == 12) tc::tmem_alloc(&bars.tmem, 512);
@@ -146,7 +142,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tcgen05_kernel(const __
   grid_dependency_wait();
   const AttnRange range = attention_range<kRows, kTile, kExtra, kThreads>(p, reinterpret_cast<int *>(smem), s_scan);
   zero_tail_rows<T>(p, kThreads);
-  if (threadIdx.x == 0) p.meta[blockIdx.x] = make_int4(-1, 0, 0, 0);
+  if (threadIdx.x == 0) p.meta[blockIdx.x].cut.x = -1, p.meta[blockIdx.x].range = range;
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
@@ -345,7 +341,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tcgen05_kernel(const __
         ++n_o;
       }
       if (!ok) break;
-      const bool whole = it->whole;
+      const bool whole = it->whole, watch = all_lo > unit0 * kTile || all_hi < (unit0 + count) * kTile;
       const float v_scale = E4M3 ? p.v_scale[it->head] : 1.f;
       const int slot = 2 * blockIdx.x + (it->first_piece ? 1 : 0);
       int64_t out_at = -1;
@@ -353,7 +349,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tcgen05_kernel(const __
         const int r = i * kTile + row;
         out_at = (it->seq.q0 + it->token(p, r)) * p.o_st + it->q_head(p, r) * p.o_sh;
       }
-      if (threadIdx.x == 0 && !whole && it->first_piece) p.meta[blockIdx.x] = it->cut;
+      if (threadIdx.x == 0 && !whole && it->first_piece) p.meta[blockIdx.x].cut = it->cut, p.meta[blockIdx.x].cut_b = it->b;
       give_back();
       // the next queries are on their way during the wait for the last product, and the tensor core has them before this output
       it = take();
@@ -367,6 +363,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tcgen05_kernel(const __
       if (query) query_ready();
       if (rows > 0) {
         const float f = !whole ? v_scale : sum == 0.f ? 0.f : v_scale / sum;
+        float2 zeros = both(0.f);        // not, where an output is not finite
         int64_t quad[4];       // this lane's four rows after the exchange below
 #pragma unroll
         for (int r = 0; r < 4; ++r) quad[r] = __shfl_sync(0xffffffffu, out_at, (lane & ~3) + r);
@@ -376,6 +373,11 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tcgen05_kernel(const __
           if (count > 0) {
             tc::tmem_ld_32x32b_x32(o_tmem + col, o);
             tc::tmem_ld_wait();
+            if (watch) {
+#pragma unroll
+              for (int e = 0; e < 32; e += 2)
+                if (col + e < p.d) zeros = fma2(make_float2(__uint_as_float(o[e]), __uint_as_float(o[e + 1])), both(0.f), zeros);
+            }
           } else {
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] = 0;
@@ -414,6 +416,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tcgen05_kernel(const __
                                                    __uint_as_float(o[e + 2]) * f, __uint_as_float(o[e + 3]) * f);
           }
         }
+        // (a row whose sum is not finite has it from its own scores)
+        if (live && isfinite(sum) && !(zeros.x + zeros.y == 0.f)) *(volatile uint32_t *)&bars.not_finite = 1;
         if (live && !whole)    // (a NaN outweighs the other pieces' rows)
           p.part_ml[(int64_t)slot * kRows + i * kTile + row] = make_float2(sum != sum ? INFINITY : sum == 0.f ? -INFINITY : ref, sum);
       }
@@ -635,6 +639,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tcgen05_kernel(const __
   // every product has been waited for by the rows that read it; tensor memory goes back
   tc::fence_before_sync();
   __syncthreads();
+  if (threadIdx.x == 0) p.meta[blockIdx.x].not_finite = (int)*(volatile uint32_t *)&bars.not_finite;
   if (warp == 12) {
     tc::fence_after_sync();
     tc::tmem_dealloc(tmem, 512);
