@@ -29,7 +29,8 @@ def freq(rot, theta=10000.0):
 @pytest.mark.parametrize("interleaved", [False, True])
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
 @pytest.mark.parametrize("t,hq,hkv,d,rot", [(1, 1, 1, 64, 64), (33, 8, 2, 128, 128), (5, 5, 1, 80, 32), (300, 3, 3, 96, 96), (7, 2, 1, 20, 6),
-                                            (4, 4, 2, 256, 256), (3, 2, 2, 64, 0), (0, 4, 2, 64, 64), (9, 2, 1, 7, 2)])
+                                            (4, 4, 2, 256, 256), (3, 2, 2, 64, 0), (0, 4, 2, 64, 64), (9, 2, 1, 7, 2),
+                                             (600, 128, 128, 128, 128), (40, 300, 200, 66, 64)])
 def test_rope(ops, interleaved, dtype, t, hq, hkv, d, rot):
     q, k, _ = qkv(t, hq, hkv, d, dtype, seed=t)
     pos = torch.randint(0, 5000, (t,), generator=torch.Generator().manual_seed(1)).cuda()
@@ -213,6 +214,8 @@ def test_refusals(ops):
     refused("rotates 128 elements", lambda: ops.zentorch_rope(q, k, pos, freq(128)))
     refused("1D float32", lambda: ops.zentorch_rope(q, k, pos, f.double()))
     refused("input's device", lambda: ops.zentorch_rope(q, k, pos.cpu(), f))
+    many = torch.zeros(1, 2000, 67, dtype=BF16, device="cuda")
+    refused("too many", lambda: ops.zentorch_rope(many, many, pos[:1], freq(64)))
     refused("shape and dtype of the key", lambda: ops.zentorch_rope_cache(q, k, v[:2], pos, f, kc, vc, pos))
     refused("caches must be", lambda: ops.zentorch_rope_cache(q, k, v, pos, f, kc.half(), vc.half(), pos))
     refused("needs k_scale", lambda: ops.zentorch_rope_cache(q, k, v, pos, f, kc.to(E4M3), vc.to(E4M3), pos))

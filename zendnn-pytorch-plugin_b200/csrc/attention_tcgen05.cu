@@ -511,7 +511,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tcgen05_kernel(const __
             }
           }
           if (rows) {
-#pragma unroll
+#pragma unroll(E4M3 ? PASSES : 2)
             for (int q = 0; q < PASSES; ++q) {
               const int r = q * RP + sub;
               const int rid = __shfl_sync(0xffffffffu, id, r), rslot = __shfl_sync(0xffffffffu, slot, r);

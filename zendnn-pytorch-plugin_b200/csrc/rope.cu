@@ -240,7 +240,9 @@ cudaError_t launch_rope(RopeParams p, int cache, cudaStream_t st) {   // cache: 
   int t = by_angles > by_items ? by_angles : by_items;
   const int spread = ceil_div(p.tokens, 2 * sm_count());
   if (t > spread) t = spread;
-  p.block_tokens = t < 1 ? 1 : t > kMaxTokens ? kMaxTokens : t;
+  t = t < 1 ? 1 : t > kMaxTokens ? kMaxTokens : t;
+  while (t > 1 && (int64_t)items * items * t >= (int64_t)1 << 32) --t;      // quotient() is exact up to there
+  p.block_tokens = t;
   const dim3 grid((unsigned)ceil_div(p.tokens, p.block_tokens)), block(kRopeThreads);
   if (cache == 0) return launch_overlapped(rope_kernel<T, VEC, false, false>, grid, block, (size_t)0, st, p);
   if (cache == 1) return launch_overlapped(rope_kernel<T, VEC, true, false>, grid, block, (size_t)0, st, p);
@@ -309,6 +311,9 @@ extern "C" int zt_rope(const zt_rope_args_t *a, void *stream) {
   // least as wide as the cache's (an e4m3 vector of the same elements has 8 or 4 bytes)
   const bool wide = (a->rot_dim / 2) % vec == 0 && a->head_dim % vec == 0 && strides % vec == 0 && bits % 16 == 0;
   const int form = !cache ? 0 : e4m3 ? 2 : 1;
+  const int per = wide ? vec : 1, head_items = (a->rot_dim / 2 / per) + ((a->head_dim - a->rot_dim) / per + 1) / 2;
+  ZT_REQUIRE((int64_t)(a->q_heads + a->kv_heads) * head_items + (cache ? (int64_t)a->kv_heads * ((a->head_dim / per + 1) / 2) : 0) < 65536,
+             ZT_UNSUPPORTED, "zt_rope: %d heads of %d elements per token are too many", a->q_heads + a->kv_heads, a->head_dim);
   cudaStream_t st = (cudaStream_t)stream;
   cudaError_t e;
   if (a->dtype == ZT_BF16)
