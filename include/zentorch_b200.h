@@ -489,7 +489,8 @@ typedef struct {
   int32_t zero_tail;
   void *workspace;
   size_t workspace_bytes;
-  int32_t algo; /* zt_algo_t: ZT_ALGO_AUTO, ZT_ALGO_SKINNY (streaming kernel), ZT_ALGO_TCGEN05 */
+  int32_t algo; /* zt_algo_t: ZT_ALGO_AUTO, ZT_ALGO_SKINNY (streaming kernel), ZT_ALGO_TCGEN05.  Streaming kernel, as a tile hint:
+                   1 = the work dealt out evenly and joined by a second kernel, 1 + s = s CTAs per sequence and kv head (s up to 8) */
 } zt_paged_attention_args_t;
 
 ZT_API size_t zt_paged_attention_workspace_bytes(const zt_paged_attention_args_t *args);

@@ -270,7 +270,10 @@ def test_c_entry_points_refuse_before_device_work(zt):
     refused(lib.zt_paged_attention(C.byref(p), None), 1, b"caches must be 16-byte aligned")
     p.v_cache_stride[:] = (16 * 4 * 64, 4 * 64, 64)
     refused(lib.zt_paged_attention(C.byref(p), None), 4, b"workspace of 0 bytes")
+    assert lib.zt_paged_attention_workspace_bytes(C.byref(p)) <= 4096         # short contexts: nothing is divided and joined
+    blocks, p.max_blocks = p.max_blocks, 1024
     assert lib.zt_paged_attention_workspace_bytes(C.byref(p)) >= 2 * 2 * 148 * 16 * 64 * 4
+    p.max_blocks = blocks
     p.tokens = 0
     assert lib.zt_paged_attention(C.byref(p), None) == 0
 

@@ -8,7 +8,7 @@ from _cache_ref import assert_attention, attention_ref, make_batch
 pytestmark = pytest.mark.gpu
 
 BF16, F16, E4M3 = torch.bfloat16, torch.float16, torch.float8_e4m3fn
-ALGOS = ["skinny", "tcgen05"]
+ALGOS = ["dealt", "slices1", "slices3", "slices8", "tcgen05"]
 
 
 @pytest.fixture(scope="module")
@@ -23,7 +23,10 @@ def run(capi, c, algo=None, **kw):
     if algo is None:
         return torch.ops.zentorch.zentorch_paged_attention(c["q"], c["k_cache"], c["v_cache"], c["cu"], c["lens"], c["table"],
                                                            c["max_q"], **scales, **kw)
-    code = {"skinny": capi.ZT_ALGO_SKINNY, "tcgen05": capi.ZT_ALGO_TCGEN05}[algo]
+    if algo == "tcgen05":
+        code = capi.ZT_ALGO_TCGEN05
+    else:
+        code = capi.ZT_ALGO_SKINNY | (1 if algo == "dealt" else 1 + int(algo[6:])) << 8
     return capi.paged_attention(c["q"], c["k_cache"], c["v_cache"], c["cu"], c["lens"], c["table"], c["max_q"], algo=code,
                                 **scales, **kw)
 
@@ -228,7 +231,7 @@ def test_values_that_are_not_finite_reach_only_rows_that_see_them(capi, algo, ca
     got = run(capi, c, algo, window=window)
     fine = torch.isfinite(want)
     assert not fine.all()
-    if algo == "skinny":
+    if algo != "tcgen05":
         assert torch.equal(got[fine], clean[fine])
     ref, bound = attention_ref(c["q"], c["k_cache"], c["v_cache"], c["cu"], c["lens"], c["table"], window=window, k_scale=c["k_scale"],
                                v_scale=c["v_scale"])

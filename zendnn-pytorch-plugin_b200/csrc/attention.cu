@@ -211,6 +211,16 @@ cudaError_t launch_combine(const AttnParams &p, const AttnPlan &plan, cudaStream
 
 size_t align256(size_t v) { return (v + 255) / 256 * 256; }
 
+// CTAs per sequence and kv head where block_table has room for `keys` keys each, 0: the units are dealt out.  A CTA takes about
+// 1 us for 64 keys, dealing and joining about 4 us, and clusters of 512 and more CTAs take longer to place than they save.  Direct
+// against dealt, ragged lengths of keys / 10 to keys, in us: 16 items of 2048 keys 9.9 / 12.9 (8 CTAs each), 128 of 512 11.7 / 11.9
+// (2), 128 of 1024 16.6 / 15.3, 512 of 256 14.8 / 18.1 (1), 512 of 512 21.3 / 23.1, 512 of 1024 38.4 / 35.0.
+int direct_slices(int64_t keys, int64_t items) {
+  int s = 8;
+  while (s > 1 && (items * s > 256 || keys <= 64 * s)) s /= 2;
+  return keys <= 320 * s ? s : 0;
+}
+
 AttnPlan make_plan(const zt_paged_attention_args_t &a) {
   AttnPlan plan{};
   const int group = a.kv_heads > 0 ? a.q_heads / a.kv_heads : 1;
@@ -218,11 +228,19 @@ AttnPlan make_plan(const zt_paged_attention_args_t &a) {
   const int64_t bound = a.tokens - a.batch + 1 > 1 ? a.tokens - a.batch + 1 : 1;
   const int64_t longest = a.max_query_len > 0 && a.max_query_len < bound ? a.max_query_len : bound;
   const int64_t rows = longest * group;
-  plan.tcgen05 = a.algo == ZT_ALGO_TCGEN05 || (a.algo == ZT_ALGO_AUTO && rows > kMaxStreamRows);
+  const int algo = a.algo & 0xff, hint = (a.algo >> 8) & 0xffff;
+  plan.tcgen05 = algo == ZT_ALGO_TCGEN05 || (algo == ZT_ALGO_AUTO && rows > kMaxStreamRows);
   plan.dp = a.head_dim <= 64 ? 64 : 128;
   plan.rows = plan.tcgen05 ? kTcgen05Rows : rows <= 16 ? 16 : 32;
   plan.grid = plan.tcgen05 ? sm_count() : attention_stream_grid(plan.rows);
   plan.few = rows <= 4 * plan.rows;
+  const int64_t keys = (int64_t)a.page_size * a.max_blocks, items = (int64_t)a.batch * a.kv_heads;
+  if (!plan.tcgen05 && items > 0) plan.slices = hint ? (hint == 1 ? 0 : hint - 1) : direct_slices(keys, items);
+  if (plan.slices > 0) {
+    plan.grid = 0;
+    plan.meta_bytes = 256;      // (nothing is kept there)
+    return plan;
+  }
   // units of the whole call at most (an item has up to three beside those of its keys)
   const int64_t unit = plan.tcgen05 ? 128 : 64, tiles = a.tokens * group / plan.rows + a.batch;
   plan.most_units = (double)tiles * a.kv_heads * (double)((int64_t)a.page_size * a.max_blocks / unit + 4);
@@ -270,7 +288,8 @@ extern "C" int zt_paged_attention(const zt_paged_attention_args_t *a, void *stre
   ZT_REQUIRE(std::isfinite(a->scale) && a->scale > 0.f, ZT_INVALID_ARGUMENT, "zt_paged_attention: the scale must be positive and finite");
   ZT_REQUIRE(!e4m3 || (a->k_scale && a->v_scale), ZT_INVALID_ARGUMENT,
              "zt_paged_attention: a float8_e4m3 cache needs k_scale and v_scale");
-  ZT_REQUIRE(a->algo == ZT_ALGO_AUTO || a->algo == ZT_ALGO_SKINNY || a->algo == ZT_ALGO_TCGEN05, ZT_INVALID_ARGUMENT,
+  const int algo = a->algo & 0xff, hint = (a->algo >> 8) & 0xffff;
+  ZT_REQUIRE((algo == ZT_ALGO_AUTO || algo == ZT_ALGO_SKINNY || algo == ZT_ALGO_TCGEN05) && a->algo >> 24 == 0 && hint <= 9, ZT_INVALID_ARGUMENT,
              "zt_paged_attention: unknown algo %d", a->algo);
   if (a->tokens == 0) return ZT_SUCCESS;
   ZT_REQUIRE(a->q && a->out && a->cu_seqlens_q, ZT_INVALID_ARGUMENT, "zt_paged_attention: null tensor pointer");
@@ -303,7 +322,7 @@ extern "C" int zt_paged_attention(const zt_paged_attention_args_t *a, void *stre
   p.page_shift = -1;
   for (int s = 0; s < 31; ++s)
     if (a->page_size == 1 << s) p.page_shift = s;
-  p.causal = a->causal != 0, p.window = a->window, p.scale_log2 = a->scale * 1.4426950408889634f, p.zero_tail = a->zero_tail != 0, p.few = plan.few;
+  p.causal = a->causal != 0, p.window = a->window, p.scale_log2 = a->scale * 1.4426950408889634f, p.zero_tail = a->zero_tail != 0, p.few = plan.few, p.slices = plan.slices;
   char *ws = reinterpret_cast<char *>(a->workspace);
   p.meta = reinterpret_cast<AttnMeta *>(ws);
   p.part_ml = reinterpret_cast<float2 *>(ws + plan.meta_bytes);
@@ -313,7 +332,7 @@ extern "C" int zt_paged_attention(const zt_paged_attention_args_t *a, void *stre
   cudaStream_t st = (cudaStream_t)stream;
   const int rc = plan.tcgen05 ? attention_tcgen05_launch(p, plan, a->dtype, a->cache_dtype, st)
                               : attention_stream_launch(p, plan, a->dtype, a->cache_dtype, st);
-  if (rc != ZT_SUCCESS) return rc;
+  if (rc != ZT_SUCCESS || plan.slices > 0) return rc;
   ZT_CUDA_OK(a->dtype == ZT_BF16 ? (e4m3 ? launch_combine<__nv_bfloat16, true>(p, plan, st) : launch_combine<__nv_bfloat16, false>(p, plan, st))
                                  : (e4m3 ? launch_combine<__half, true>(p, plan, st) : launch_combine<__half, false>(p, plan, st)));
   return launch_status("attention_combine_kernel");

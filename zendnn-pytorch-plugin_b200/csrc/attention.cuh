@@ -34,6 +34,7 @@ struct AttnParams {
   int page, page_shift, max_blocks, num_pages;  // page_shift: log2 of the page size, or -1
   int causal, window;                           // window 0: none
   float scale_log2;                             // softmax scale times log2(e)
+  int slices;                                   // streaming kernel: CTAs per sequence and kv head (0: all units are dealt out)
   int few;                                      // no sequence can have more than a few tiles of rows
   int zero_tail;                                // rows behind the last sequence are zeroed
   float *part_o;                                // [2 * grid][R][DP]
@@ -59,6 +60,7 @@ struct AttnMeta {
 struct AttnPlan {         // of one call, on the host
   bool tcgen05, few;
   int rows, dp, grid;     // rows per item, padded head, CTAs
+  int slices;             // see AttnParams
   double most_units;
   size_t meta_bytes, ml_bytes, o_bytes;
   size_t total() const { return meta_bytes + ml_bytes + o_bytes; }

@@ -33,7 +33,7 @@ __host__ __device__ constexpr int stages() { return (E4M3 ? 2 : 1) * (MT == 1 ? 
 template <int DP, bool E4M3, int MT>
 __host__ __device__ constexpr int ring_bytes() { return kWarps * stages<E4M3, MT>() * stage_bytes<DP, E4M3>(); }
 template <int R, int DP>
-__host__ __device__ constexpr int merge_bytes() { return kWarps * R * (DP + 8) * 4 + kWarps * R * 8; }
+__host__ __device__ constexpr int merge_bytes() { return kWarps * R * (DP + 8) * 4 + kWarps * R * 8 + R * 8 + R * DP * 4; }
 
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -67,7 +67,24 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-template <typename T, bool E4M3, int DP, int MT>
+__device__ __forceinline__ float4 ld_cluster16(uint32_t addr) {
+  float4 x;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(addr) : "memory");
+  return x;
+}
+
+// An item, or a slice of its keys, of a CTA that belongs to one sequence and kv head.
+struct DirectPiece {
+  SeqInfo seq;
+  int b, head, unit0, n_units, n_rows, r0;
+  __device__ int token(const AttnParams &p, int row) const { return (r0 + row) / p.group; }
+  __device__ int q_head(const AttnParams &p, int row) const { return head * p.group + (r0 + row) % p.group; }
+};
+
+// DIRECT: for short contexts, where dividing the batch and joining the pieces (two dependent steps of about 2 us and a launch) cost
+// more than they even out: a cluster of p.slices CTAs per sequence and kv head, which add their rows through shared memory.  (64
+// keys take a CTA 1 us, by the length of its chain of instructions: a ring of five stages instead of two changed nothing.)
+template <typename T, bool E4M3, int DP, int MT, bool DIRECT>
 __global__ void __launch_bounds__(kThreads, ctas_per_sm<MT>()) attention_stream_kernel(const __grid_constant__ AttnParams p) {
   using M = std::conditional_t<E4M3, __half, T>;
   constexpr int R = 16 * MT, S = stages<E4M3, MT>(), SB = stage_bytes<DP, E4M3>();
@@ -81,16 +98,14 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<MT>()) attention_stream_
   grid_dependency_wait();
   const int lane = threadIdx.x & 31, warp = tc::uniform_warp();
   const int g = lane >> 2, t4 = lane & 3;
-  const AttnRange range = attention_range<R, kUnit, kExtra, kThreads>(p, reinterpret_cast<int *>(smem), s_scan);
   zero_tail_rows<T>(p, kThreads);
   unsigned char *ring = smem + warp * S * SB;
   const uint32_t ring_addr = smem_u32(ring);
   float *merge_o = reinterpret_cast<float *>(smem);                                   // [warp][R][DP + 8]
   float2 *merge_ml = reinterpret_cast<float2 *>(smem + kWarps * R * (DP + 8) * 4);    // [warp][R]
-  if (threadIdx.x == 0) p.meta[blockIdx.x].cut.x = -1;
-
-  AttnWalk<R, kUnit, kExtra> it(range);
-  while (it.next(p)) {
+  float2 *slice_ml = merge_ml + kWarps * R;                                           // DIRECT: [R], and the rows of this slice [R][DP]
+  float *slice_o = reinterpret_cast<float *>(slice_ml + R);
+  auto work = [&](const auto &it) {
     const SeqInfo seq = it.seq;
     const int b = it.b, head = it.head, n_units = it.n_units, unit0 = it.unit0, n_rows = it.n_rows;
     const int tok0 = it.token(p, 0), tok1 = it.token(p, n_rows - 1);
@@ -428,8 +443,12 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<MT>()) attention_stream_
       }
     }
     __syncthreads();
-    const int slot = 2 * blockIdx.x + (it.first_piece ? 1 : 0);
     const float v_scale = E4M3 ? p.v_scale[head] : 1.f;
+    auto write_row = [&](int row, int c, float4 acc, float f) {
+      const int tok = it.token(p, row), qh = it.q_head(p, row);
+      char *dst = reinterpret_cast<char *>(p.out) + ((seq.q0 + tok) * p.o_st + qh * p.o_sh + c) * 2;
+      *reinterpret_cast<uint2 *>(dst) = make_uint2(pack2(acc.x * f, acc.y * f, T(0.f)), pack2(acc.z * f, acc.w * f, T(0.f)));
+    };
     for (int idx = threadIdx.x; idx < n_rows * (DP / 4); idx += kThreads) {
       const int row = idx / (DP / 4), c = (idx % (DP / 4)) * 4;
       float best = -INFINITY, l = 0.f;
@@ -446,36 +465,86 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<MT>()) attention_stream_
         const float4 x = *reinterpret_cast<const float4 *>(merge_o + (v * R + row) * (DP + 8) + c);
         acc.x += x.x, acc.y += x.y, acc.z += x.z, acc.w += x.w;
       }
-      if (it.whole) {
-        if (c < p.d) {
-          const float f = best == -INFINITY ? 0.f : v_scale / l;
-          const int tok = it.token(p, row), qh = it.q_head(p, row);
-          char *dst = reinterpret_cast<char *>(p.out) + ((seq.q0 + tok) * p.o_st + qh * p.o_sh + c) * 2;
-          *reinterpret_cast<uint2 *>(dst) = make_uint2(pack2(acc.x * f, acc.y * f, T(0.f)), pack2(acc.z * f, acc.w * f, T(0.f)));
-        }
+      bool whole;
+      if constexpr (DIRECT) whole = p.slices == 1;
+      else whole = it.whole;
+      if (whole) {
+        if (c < p.d) write_row(row, c, acc, best == -INFINITY ? 0.f : v_scale / l);
+      } else if constexpr (DIRECT) {
+        *reinterpret_cast<float4 *>(slice_o + row * DP + c) = acc;
+        if (c == 0) slice_ml[row] = make_float2(best, l);
       } else {
+        const int slot = 2 * blockIdx.x + (it.first_piece ? 1 : 0);
         *reinterpret_cast<float4 *>(p.part_o + ((int64_t)slot * R + row) * DP + c) =
             make_float4(acc.x * v_scale, acc.y * v_scale, acc.z * v_scale, acc.w * v_scale);
         if (c == 0) p.part_ml[(int64_t)slot * R + row] = make_float2(best, l);
       }
     }
-    if (threadIdx.x == 0 && !it.whole && it.first_piece) p.meta[blockIdx.x].cut = it.cut();
+    if constexpr (DIRECT) {
+      if (p.slices > 1) {          // each CTA of the cluster finishes a share of the rows
+        tc::cluster_sync();
+        const uint32_t o_at = smem_u32(slice_o), ml_at = smem_u32(slice_ml);
+        for (int idx = (blockIdx.x % p.slices) * kThreads + threadIdx.x; idx < n_rows * (DP / 4); idx += p.slices * kThreads) {
+          const int row = idx / (DP / 4), c = (idx % (DP / 4)) * 4;
+          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+          float best = -INFINITY, l = 0.f;
+          for (int r = 0; r < p.slices; ++r) {
+            const float top = tc::load_cluster_f32(tc::map_to_rank(ml_at + row * 8, r)), part = tc::load_cluster_f32(tc::map_to_rank(ml_at + row * 8 + 4, r));
+            const float4 x = ld_cluster16(tc::map_to_rank(o_at + (row * DP + c) * 4, r));
+            const float to = fmaxf(best, top), f_old = best == -INFINITY ? 0.f : exp2_fast(best - to), f = top == -INFINITY ? 0.f : exp2_fast(top - to);
+            best = to, l = l * f_old + part * f;
+            acc.x = acc.x * f_old + x.x * f, acc.y = acc.y * f_old + x.y * f, acc.z = acc.z * f_old + x.z * f, acc.w = acc.w * f_old + x.w * f;
+          }
+          if (c < p.d) write_row(row, c, acc, best == -INFINITY ? 0.f : v_scale / l);
+        }
+        tc::cluster_sync();        // the other CTAs have read this one's rows
+      }
+    } else if (threadIdx.x == 0 && !it.whole && it.first_piece) {
+      p.meta[blockIdx.x].cut = it.cut();
+    }
     __syncthreads();   // the merge area is read before the next rings fill it
+  };
+
+  if constexpr (DIRECT) {
+    DirectPiece it;
+    const int item = blockIdx.x / p.slices, slice = blockIdx.x % p.slices;
+    it.b = item / p.hkv, it.head = item % p.hkv;
+    if (it.head == 0 && slice == 0 && threadIdx.x == 0 && !lengths_fit(p, it.b)) tc::report_timeout(p.status, kStatusBadIndex);
+    it.seq = load_seq(p, it.b);
+    const int tiles = row_tiles<R>(p, it.seq);
+    for (int tile = 0; tile < tiles; ++tile) {
+      const TileUnits u = tile_units<R, kUnit>(p, it.seq, tile);
+      const int from = u.count * slice / p.slices, to = u.count * (slice + 1) / p.slices;
+      it.unit0 = u.first + from, it.n_units = to - from;
+      it.r0 = tile * R, it.n_rows = min(it.seq.n * p.group - it.r0, R);
+      work(it);
+    }
+  } else {
+    const AttnRange range = attention_range<R, kUnit, kExtra, kThreads>(p, reinterpret_cast<int *>(smem), s_scan);
+    if (threadIdx.x == 0) p.meta[blockIdx.x].cut.x = -1;
+    AttnWalk<R, kUnit, kExtra> it(range);
+    while (it.next(p)) work(it);
   }
 }
 
-template <typename T, bool E4M3, int DP, int MT>
-int launch(const AttnParams &p, const AttnPlan &plan, cudaStream_t st) {
+template <typename T, bool E4M3, int DP, int MT, bool DIRECT>
+int launch_mode(const AttnParams &p, dim3 grid, size_t prefix, cudaStream_t st) {
   constexpr int ring = ring_bytes<DP, E4M3, MT>(), merge = merge_bytes<16 * MT, DP>();
   constexpr int fixed = ring > merge ? ring : merge;
-  const int prefix = (p.batch + 1) * 4;
-  const int smem = prefix > fixed ? prefix : fixed;   // the division of the batch comes before the first copy
+  const size_t smem = prefix > fixed ? prefix : fixed;
   static PerDeviceOnce once;
-  auto kern = attention_stream_kernel<T, E4M3, DP, MT>;
+  auto kern = attention_stream_kernel<T, E4M3, DP, MT, DIRECT>;
   const int rc = allow_dynamic_smem(once, kern, 110 * 1024);
   if (rc != ZT_SUCCESS) return rc;
-  ZT_CUDA_OK(launch_overlapped(kern, dim3(plan.grid), dim3(kThreads), (size_t)smem, st, p));
+  if (!DIRECT || p.slices == 1) ZT_CUDA_OK(launch_overlapped(kern, grid, dim3(kThreads), smem, st, p));
+  else ZT_CUDA_OK(launch_overlapped_cluster(kern, grid, dim3(kThreads), smem, st, dim3((unsigned)p.slices), p));
   return launch_status("attention_stream_kernel");
+}
+template <typename T, bool E4M3, int DP, int MT>
+int launch(const AttnParams &p, const AttnPlan &plan, cudaStream_t st) {
+  // (the division of the batch comes before the first copy and has the shared memory to itself)
+  if (plan.slices == 0) return launch_mode<T, E4M3, DP, MT, false>(p, dim3(plan.grid), (size_t)(p.batch + 1) * 4, st);
+  return launch_mode<T, E4M3, DP, MT, true>(p, dim3((unsigned)(p.batch * p.hkv * plan.slices)), 0, st);
 }
 template <typename T, bool E4M3>
 int launch_sized(const AttnParams &p, const AttnPlan &plan, cudaStream_t st) {
