@@ -100,6 +100,21 @@ def test_masks(capi, algo, causal, window):
 
 
 @pytest.mark.parametrize("algo", ALGOS)
+@pytest.mark.parametrize("causal", [True, False])
+def test_the_largest_window_is_none(capi, algo, causal):
+    """Also where a sequence has more new tokens than keys, whose positions begin below zero."""
+    c = make_batch([(1, 333), (9, 4), (5, 0), (40, 40)], 6, 2, 64, 16, BF16, seed=31)
+    assert torch.equal(run(capi, c, algo, causal=causal, window=2 ** 31 - 1), run(capi, c, algo, causal=causal))
+
+
+@pytest.mark.parametrize("max_q", [None, 1, 10 ** 6])
+def test_most_new_tokens_need_not_be_exact(capi, max_q):
+    """max_query_len only chooses the kernel: one that is too small, too large or unknown gives every row all the same."""
+    c = make_batch([(1, 333), (150, 300), (0, 9), (1, 1)], 8, 2, 64, 16, BF16, seed=32)
+    check(capi, dict(c, max_q=max_q), None)
+
+
+@pytest.mark.parametrize("algo", ALGOS)
 def test_pages_behind_a_window_may_be_gone(capi, algo):
     """Pages that no new token sees any more are not read: their table entries may be anything."""
     c = make_batch([(3, 500)], 4, 2, 64, 16, BF16, seed=9)
@@ -166,6 +181,9 @@ def test_tail_rows(capi, algo):
     torch.ops.zentorch.zentorch_paged_attention.out(mine, c["q"], c["k_cache"], c["v_cache"], c["cu"], c["lens"], c["table"], 3)
     assert_attention(mine[:5], ref[:5], bound[:5])
     assert (mine[5:] == 7).all()
+    c = make_batch([(2, 30)], 5, 1, 72, 16, BF16, seed=15, tail=700)      # a tail wider than the grid, heads of 144 bytes
+    got = run(capi, c, algo)
+    assert (got[2:] == 0).all() and (got[:2] != 0).any()
 
 
 def test_unaligned_query_and_output(capi):
@@ -196,6 +214,23 @@ def test_nan_and_infinite_queries_stay_in_their_rows(capi, algo):
     keep = torch.ones(6, 4, dtype=torch.bool, device="cuda")
     keep[2, 1] = keep[3, 2] = False
     assert torch.equal(got[keep], clean[keep])
+
+
+@pytest.mark.parametrize("algo", ALGOS)
+@pytest.mark.parametrize("cache", ["same", "e4m3"])
+def test_a_key_of_nan_among_tiles_of_rows(capi, algo, cache):
+    """Rows of several tiles, some of which see the key: NaN in all their columns, the bound of every other row."""
+    n, kv, key = 200, 300, 180
+    c = make_batch([(n, kv), (1, 20)], 4, 2, 64, 16, BF16, E4M3 if cache == "e4m3" else BF16, seed=33)
+    ref, bound = attention_ref(c["q"], c["k_cache"], c["v_cache"], c["cu"], c["lens"], c["table"], k_scale=c["k_scale"],
+                               v_scale=c["v_scale"])
+    raw = c["k_cache"].view(torch.uint8) if cache == "e4m3" else c["k_cache"]
+    raw[c["table"][0, key // 16].long(), key % 16, 1, 9] = 0x7f if cache == "e4m3" else float("nan")
+    got = run(capi, c, algo)
+    hit = torch.zeros(n + 1, 4, dtype=torch.bool)
+    hit[key - (kv - n):n, 2:] = True
+    assert got.cpu()[hit].isnan().all()
+    assert bool(((got.double().cpu() - ref).abs()[~hit] <= bound[~hit]).all())
 
 
 @pytest.mark.parametrize("algo", ALGOS)
@@ -319,6 +354,11 @@ def test_refusals(capi):
     refused("window must not be negative", window=-1)
     refused("scale must be positive", scale=0.0)
     refused("belongs to a float8", k_scale=torch.ones(2, device="cuda"))
+    into = torch.ops.zentorch.zentorch_paged_attention.out
+    with pytest.raises(RuntimeError, match="share memory with query"):
+        into(c["q"][:, :4], *args)
+    with pytest.raises(RuntimeError, match="hold an element twice"):
+        into(torch.zeros(1, 1, 64, dtype=BF16, device="cuda").expand(1, 4, 64), *args)
     refused("16-byte aligned", 1, torch.zeros(c["k_cache"].shape[0], 16, 2, 65, dtype=BF16, device="cuda")[..., 1:])
     e = c["k_cache"].nan_to_num().to(E4M3)
     with pytest.raises(RuntimeError, match="needs k_scale"):

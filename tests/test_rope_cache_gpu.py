@@ -188,6 +188,39 @@ def test_copy_pages_of_views(ops):
     assert torch.equal(both, want) and torch.equal(heads, want_heads)
 
 
+def test_copy_pages_skips_caches_without_elements(ops):
+    x = torch.arange(8 * 6, device="cuda").view(8, 6)
+    y = x.clone()
+    ops.zentorch_cache_copy_pages([x[:, :0], x], torch.tensor([5]).cuda(), torch.tensor([2]).cuda())
+    y[2] = y[5]
+    assert torch.equal(x, y)
+
+
+def test_two_calls_at_once(ops):
+    """Appends to different rows of one cache on two streams, while a third copies pages that neither touches."""
+    kc, vc = caches(6, 4, 2, 64, BF16, "joined")
+    f, pos = freq(64), torch.arange(4).cuda()
+    src, dst = torch.tensor([4]).cuda(), torch.tensor([5]).cuda()
+    batches = [qkv(4, 4, 2, 64, BF16, seed=s) for s in (1, 2)]
+    slots = [torch.arange(4).cuda(), torch.arange(8, 12).cuda()]
+    kc[4], vc[4] = 1.5, 2.5
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    outs = [None, None]
+    for _ in range(5):
+        for i in (0, 1):
+            with torch.cuda.stream(streams[i]):
+                outs[i] = ops.zentorch_rope_cache(*batches[i], pos, f, kc, vc, slots[i])
+        with torch.cuda.stream(streams[2]):
+            ops.zentorch_cache_copy_pages([kc, vc], src, dst)
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        assert_rope(outs[i], batches[i][0], pos, f, 1.0, False)
+        assert_rope(kc.reshape(24, 2, 64)[slots[i]], batches[i][1], pos, f, 1.0, False)
+        assert torch.equal(vc.reshape(24, 2, 64)[slots[i]], batches[i][2])
+    assert (kc[5] == 1.5).all() and (vc[5] == 2.5).all()
+
+
 def test_copy_pages_past_the_cache_are_reported(ops, zt):
     from zentorch_b200 import _capi
     x = torch.randn(4, 64, device="cuda")
@@ -219,6 +252,7 @@ def test_refusals(ops):
     refused("shape and dtype of the key", lambda: ops.zentorch_rope_cache(q, k, v[:2], pos, f, kc, vc, pos))
     refused("caches must be", lambda: ops.zentorch_rope_cache(q, k, v, pos, f, kc.half(), vc.half(), pos))
     refused("needs k_scale", lambda: ops.zentorch_rope_cache(q, k, v, pos, f, kc.to(E4M3), vc.to(E4M3), pos))
+    refused("hold an element twice", lambda: ops.zentorch_rope_cache(q, k, v, pos, f, kc[:1].expand_as(kc), vc, pos))
     refused("heads, the key", lambda: ops.zentorch_rope_cache(q, q, q, pos, f, kc, vc, pos))
     refused("one block of memory", lambda: ops.zentorch_cache_copy_pages([kc[..., :32]], pos[:1], pos[1:2]))
     refused("one number of pages", lambda: ops.zentorch_cache_copy_pages([kc, vc[:1]], pos[:1], pos[1:2]))

@@ -75,8 +75,8 @@ __device__ __forceinline__ float cache_value(const void *base, int64_t at) {
   }
 }
 
-// Goes through a row of the output again, by one warp, where it is not finite: unless every such column has a value that is not
-// finite among the keys that the row sees, the row is computed from those keys alone.
+// Goes through a row of the output again, by one warp, where it is not finite: unless its query or a key that it sees holds a NaN,
+// or every such column has a value that is not finite among the keys that the row sees, the row is computed from those keys alone.
 template <typename T, bool E4M3>
 __device__ __noinline__ void redo_row(const AttnParams &p, int b, const SeqInfo &seq, int head, int r) {
   constexpr int V = 4;                                   // columns of a lane
@@ -93,11 +93,20 @@ __device__ __noinline__ void redo_row(const AttnParams &p, int b, const SeqInfo 
   for (int e = 0; e < V; ++e)
     if (lane * V + e < p.d && !isfinite((float)out[lane * V + e])) open |= 1u << e;
   if (!__any_sync(0xffffffffu, open != 0)) return;
-  for (int key = hi - 1; key >= lo && __any_sync(0xffffffffu, open != 0); --key) {
-    const int64_t at = row_of(key, p.v_sp, p.v_ss, p.v_sh);
+  bool nan = false;
 #pragma unroll
-    for (int e = 0; e < V; ++e)
-      if (at >= 0 && (open >> e & 1) && !isfinite(cache_value<T, E4M3>(p.v, at + lane * V + e))) open &= ~(1u << e);
+  for (int e = 0; e < V; ++e)
+    if (lane * V + e < p.d) nan |= isnan((float)q[lane * V + e]);
+  if (hi > lo && __any_sync(0xffffffffu, nan)) return;
+  for (int key = hi - 1; key >= lo && __any_sync(0xffffffffu, open != 0); --key) {
+    const int64_t at = row_of(key, p.v_sp, p.v_ss, p.v_sh), k_at = row_of(key, p.k_sp, p.k_ss, p.k_sh);
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      if (at < 0 || lane * V + e >= p.d) continue;
+      if ((open >> e & 1) && !isfinite(cache_value<T, E4M3>(p.v, at + lane * V + e))) open &= ~(1u << e);
+      nan |= isnan(cache_value<T, E4M3>(p.k, k_at + lane * V + e));
+    }
+    if (__any_sync(0xffffffffu, nan)) return;
   }
   if (!__any_sync(0xffffffffu, open != 0)) return;
   const float mul = p.scale_log2 * (E4M3 ? p.k_scale[head] : 1.f);
@@ -322,7 +331,7 @@ extern "C" int zt_paged_attention(const zt_paged_attention_args_t *a, void *stre
   p.page_shift = -1;
   for (int s = 0; s < 31; ++s)
     if (a->page_size == 1 << s) p.page_shift = s;
-  p.causal = a->causal != 0, p.window = a->window, p.scale_log2 = a->scale * 1.4426950408889634f, p.zero_tail = a->zero_tail != 0, p.few = plan.few, p.slices = plan.slices;
+  p.causal = a->causal != 0, p.window = a->window < 1 << 30 ? a->window : 1 << 30 /* no context is longer */, p.scale_log2 = a->scale * 1.4426950408889634f, p.zero_tail = a->zero_tail != 0, p.few = plan.few, p.slices = plan.slices;
   char *ws = reinterpret_cast<char *>(a->workspace);
   p.meta = reinterpret_cast<AttnMeta *>(ws);
   p.part_ml = reinterpret_cast<float2 *>(ws + plan.meta_bytes);

@@ -206,8 +206,11 @@ __device__ AttnRange attention_range(const AttnParams &p, int *prefix, AttnScrat
   r.per = max((total + (int)gridDim.x - 1) / (int)gridDim.x, 1);
   r.w0 = (int)min((long long)r.per * blockIdx.x, (long long)total), r.w1 = min(r.w0 + r.per, total);
   r.b = 0, r.tile = 0, r.item0 = 0;
+  if (threadIdx.x == 0) scratch.found[0] = scratch.found[1] = scratch.found[2] = 0;
+  __syncthreads();
   if (r.w0 < r.w1) {
-    // (lengths that contradict one another can add up to more than an int: the walk checks what it goes by)
+    // (lengths that contradict one another can add up to more than an int, and then no thread may find w0: the walk checks what it
+    // goes by, and `cut` where it ends)
     if (r.w0 >= at && r.w0 < at + mine) {      // one thread
       int b = p.few ? b0 : first_tile_owner(p, prefix, t0);
       SeqInfo s = load_seq(p, b);
@@ -266,7 +269,7 @@ struct AttnWalk {
     }
   }
   // For the kernel that joins the pieces of this item.
-  __device__ int4 cut() const { return make_int4(seq.q0, r0, head * 512 + n_rows, (h1_ - 1) / per_); }
+  __device__ int4 cut() const { return make_int4(seq.q0, r0, head * 512 + n_rows, min((h1_ - 1) / per_, (int)gridDim.x - 1)); }
   __device__ int token(const AttnParams &p, int row) const { return (r0 + row) / p.group; }
   __device__ int q_head(const AttnParams &p, int row) const { return head * p.group + (r0 + row) % p.group; }
 
@@ -283,10 +286,12 @@ template <typename T>
 __device__ __forceinline__ void zero_tail_rows(const AttnParams &p, int threads) {
   if (!p.zero_tail) return;
   const int end = min(max(p.cu[p.batch], 0), p.tokens);
-  const int64_t per = (int64_t)p.hq * p.d, n = (p.tokens - end) * per;
+  const int vecs = p.d / 8, per = p.hq * vecs;      // (rows are whole 16-byte vectors)
+  const int64_t n = (int64_t)(p.tokens - end) * per;
   for (int64_t i = (int64_t)blockIdx.x * threads + threadIdx.x; i < n; i += (int64_t)gridDim.x * threads) {
-    const int64_t t = end + i / per, c = i % per;
-    reinterpret_cast<T *>(p.out)[t * p.o_st + (c / p.d) * p.o_sh + c % p.d] = T(0.f);
+    const int64_t t = end + i / per;
+    const int c = (int)(i % per);
+    *reinterpret_cast<uint4 *>(reinterpret_cast<T *>(p.out) + t * p.o_st + (c / vecs) * p.o_sh + c % vecs * 8) = make_uint4(0, 0, 0, 0);
   }
 }
 

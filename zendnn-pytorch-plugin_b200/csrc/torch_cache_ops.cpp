@@ -1,6 +1,7 @@
 // PyTorch boundary of the operators between a decoder layer's linears: rotary positions, the paged key/value cache and the
 // attention that reads it.  The reference leaves them to its host framework, so the schemas are this library's own.  Like the
 // linears' boundary (torch_ops.cpp) this only checks and marshals tensors into the C ABI on the current stream.
+#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/record_function.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -37,6 +38,16 @@ void check_lengths(const at::Tensor &t, const at::Tensor &input, const char *op,
   check_on_device(t, input, op, name);
   TORCH_CHECK(t.scalar_type() == at::kInt, op, ": ", name, " must be int32, got ", t.scalar_type());
   TORCH_CHECK(t.dim() == dim, op, ": ", name, " must be ", dim, "D, got ", t.dim(), "D");
+}
+
+// Nothing is written twice, or while the same call still reads it.
+void check_written(const at::Tensor &t, const char *op, const char *name) {
+  TORCH_CHECK(at::has_internal_overlap(t) != at::MemOverlap::Yes, op, ": ", name, " is written and must not hold an element twice");
+}
+void check_apart(const at::Tensor &t, const at::Tensor &other, const char *op, const char *name, const char *other_name) {
+  const auto status = at::get_overlap_status(t, other);
+  TORCH_CHECK(status != at::MemOverlapStatus::Full && status != at::MemOverlapStatus::Partial, op, ": ", name,
+              " is written and must not share memory with ", other_name);
 }
 
 // A pair of caches [pages, page_size, heads, head_dim] of one shape and type; for `input` of `head_dim`.
@@ -129,6 +140,7 @@ at::Tensor rope_cache(const at::Tensor &query, const at::Tensor &key, const at::
   check_index(slots, q, op, "slot_mapping", q.size(0));
   check_caches(key_cache, value_cache, q, q.size(2), op);
   TORCH_CHECK(key_cache.size(2) == k.size(1), op, ": the caches have ", key_cache.size(2), " heads, the key ", k.size(1));
+  check_written(key_cache, op, "key_cache"), check_written(value_cache, op, "value_cache");
   a.k_scale = cache_scale(k_scale, key_cache, q, op, "k_scale");
   a.v_scale = cache_scale(v_scale, value_cache, q, op, "v_scale");
   c10::cuda::CUDAGuard device_guard(q.device());
@@ -171,27 +183,25 @@ void cache_copy_pages(at::TensorList caches, const at::Tensor &src, const at::Te
   check_index(dst, src, op, "dst", src.size(0));
   TORCH_CHECK(src.scalar_type() == dst.scalar_type(), op, ": src and dst must have one dtype");
   if (caches.empty()) return;
-  const size_t n = caches.size();
-  std::vector<void *> base(n);
-  std::vector<int64_t> stride(n), bytes(n);
-  for (size_t i = 0; i < n; ++i) {
-    const at::Tensor &t = caches[i];
+  std::vector<void *> base;
+  std::vector<int64_t> stride, bytes;
+  for (const at::Tensor &t : caches) {
     check_on_device(t, src, op, "every cache");
     TORCH_CHECK(t.dim() >= 2, op, ": a cache must be [pages, ...], got ", t.dim(), "D");
     TORCH_CHECK(t.size(0) == caches[0].size(0), op, ": the caches must have one number of pages");
     TORCH_CHECK(t.size(0) < (int64_t)1 << 31, op, ": pages of the cache out of range");
-    if (t.numel() > 0)
-      TORCH_CHECK(dense_pages(t), op, ": a page of a cache must be one block of memory; got strides ", t.strides(), " for ", t.sizes());
+    if (t.numel() == 0) continue;
+    TORCH_CHECK(dense_pages(t), op, ": a page of a cache must be one block of memory; got strides ", t.strides(), " for ", t.sizes());
     const int64_t es = (int64_t)t.element_size();
-    base[i] = t.data_ptr();
-    bytes[i] = t.size(0) == 0 ? 0 : t.numel() / t.size(0) * es;
-    stride[i] = t.size(0) <= 1 ? bytes[i] : t.stride(0) * es;
+    base.push_back(t.data_ptr());
+    bytes.push_back(t.numel() / t.size(0) * es);
+    stride.push_back(t.size(0) <= 1 ? bytes.back() : t.stride(0) * es);
   }
-  if (caches[0].numel() == 0 || src.size(0) == 0) return;
+  if (base.empty() || src.size(0) == 0) return;
   c10::cuda::CUDAGuard device_guard(src.device());
   const at::Tensor s = src.contiguous(), d = dst.contiguous();
   zt_cache_copy_args_t a{};
-  a.n_caches = (int32_t)n;
+  a.n_caches = (int32_t)base.size();
   a.caches = base.data(), a.page_stride_bytes = stride.data(), a.page_bytes = bytes.data();
   a.num_pages = (int32_t)caches[0].size(0);
   a.n_pairs = s.size(0);
@@ -230,6 +240,10 @@ void paged_attention_into(at::Tensor &out, const at::Tensor &query, const at::Te
   check_on_device(out, query, op, "out");
   TORCH_CHECK(out.sizes() == query.sizes() && out.scalar_type() == query.scalar_type(), op,
               ": out must have the shape and dtype of the query");
+  if (!zero_tail) {      // (else it was made for this call)
+    check_written(out, op, "out");
+    check_apart(out, query, op, "out", "query"), check_apart(out, key_cache, op, "out", "key_cache"), check_apart(out, value_cache, op, "out", "value_cache");
+  }
   zt_paged_attention_args_t a{};
   a.k_scale = cache_scale(k_scale, key_cache, query, op, "k_scale");
   a.v_scale = cache_scale(v_scale, value_cache, query, op, "v_scale");
