@@ -6,8 +6,8 @@
 // one is in its exponentials while the tensor core works for the other.
 //
 //   warps 0-3, 4-7   a row of tile 0 / 1 each thread: query rows to shared memory, running maximum and sum, probabilities, output
-//   warps 8-11       K and V tiles into a ring, 32 keys each: by TMA, in boxes of up to 32 slots of a page, where the pages hold a power
-//                    of two of at least 8 slots and all 32 keys are visible; else row by row, 16 bytes per asynchronous copy (any
+//   warps 8-11       K and V tiles into a ring, 32 keys each: by TMA, in boxes of 8, 16 or 32 slots of a page, where a page is whole
+//                    boxes and all 32 keys are visible; else row by row, 16 bytes per asynchronous copy (any
 //                    page size).  Slots past the visible keys become zeros that way, so stale contents of a page never meet the
 //                    arithmetic.  e4m3 tiles come row by row into a ring of their own and from there as halves (exact)
 //   warp 12          issues the MMAs
@@ -22,6 +22,8 @@
 // rescaled a few times at the start and hardly ever after; the thread that finds it does it itself.  Probabilities are rounded
 // to the products' type; their sum is of the unrounded fp32 values.  e4m3: fp16 products, query rows brought below 2 by a power of
 // two as in the streaming kernel.
+#include <algorithm>
+
 #include "attention.cuh"
 
 namespace zt {
@@ -670,8 +672,8 @@ int launch(const AttnParams &p, const AttnPlan &plan, cudaStream_t st) {
   if (rc != ZT_SUCCESS) return rc;
   CUtensorMap k_map{}, v_map{};
   int box = 0;
-  if (!E4M3 && p.page_shift >= 3 && p.num_pages > 0) {
-    box = p.page < kBoxSlots ? p.page : kBoxSlots;
+  if (!E4M3 && p.page % 8 == 0 && p.num_pages > 0) {
+    box = std::min(p.page & -p.page, kBoxSlots);      // divides the page, so that no box of aligned keys spans two
     const int64_t ks[3] = {p.k_ss, p.k_sh, p.k_sp}, vs[3] = {p.v_ss, p.v_sh, p.v_sp};
     if (!page_map<T>(&k_map, p, p.k, ks, box) || !page_map<T>(&v_map, p, p.v, vs, box)) box = 0;
   }
