@@ -8,7 +8,8 @@ from _cache_ref import assert_attention, attention_ref, make_batch
 pytestmark = pytest.mark.gpu
 
 BF16, F16, E4M3 = torch.bfloat16, torch.float16, torch.float8_e4m3fn
-ALGOS = ["dealt", "slices1", "slices3", "slices8", "tcgen05"]
+ROWS = {"rows8": 8, "rows16": 16}                  # the streaming kernel for so many rows per kv head; "dealt": 32 in most tests
+ALGOS = ["dealt", *ROWS, "slices1", "slices3", "slices8", "tcgen05"]
 
 
 @pytest.fixture(scope="module")
@@ -26,9 +27,11 @@ def run(capi, c, algo=None, **kw):
     if algo == "tcgen05":
         code = capi.ZT_ALGO_TCGEN05
     else:
-        code = capi.ZT_ALGO_SKINNY | (1 if algo == "dealt" else 1 + int(algo[6:])) << 8
-    return capi.paged_attention(c["q"], c["k_cache"], c["v_cache"], c["cu"], c["lens"], c["table"], c["max_q"], algo=code,
-                                **scales, **kw)
+        code = capi.ZT_ALGO_SKINNY | (1 if algo in ROWS or algo == "dealt" else 1 + int(algo[6:])) << 8
+    max_q = c["max_q"]
+    if algo in ROWS:      # (it need not be exact)
+        max_q = max(1, ROWS[algo] * c["k_cache"].shape[2] // c["q"].shape[1])
+    return capi.paged_attention(c["q"], c["k_cache"], c["v_cache"], c["cu"], c["lens"], c["table"], max_q, algo=code, **scales, **kw)
 
 
 def check(capi, c, algo=None, what="", **kw):

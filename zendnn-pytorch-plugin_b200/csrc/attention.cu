@@ -240,7 +240,7 @@ AttnPlan make_plan(const zt_paged_attention_args_t &a) {
   const int algo = a.algo & 0xff, hint = (a.algo >> 8) & 0xffff;
   plan.tcgen05 = algo == ZT_ALGO_TCGEN05 || (algo == ZT_ALGO_AUTO && rows > kMaxStreamRows);
   plan.dp = a.head_dim <= 64 ? 64 : 128;
-  plan.rows = plan.tcgen05 ? kTcgen05Rows : rows <= 16 ? 16 : 32;
+  plan.rows = plan.tcgen05 ? kTcgen05Rows : rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
   plan.grid = plan.tcgen05 ? sm_count() : attention_stream_grid(plan.rows);
   plan.few = rows <= 4 * plan.rows;
   const int64_t keys = (int64_t)a.page_size * a.max_blocks, items = (int64_t)a.batch * a.kv_heads;

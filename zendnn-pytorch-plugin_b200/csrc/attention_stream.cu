@@ -24,14 +24,14 @@ constexpr int kExtra = 2;                  // units that an item costs beside it
 
 // Three CTAs share an SM where their rows leave the registers (16 rows; 64 kept keys ahead per CTA), else two.  Decode of 64
 // sequences of 500 - 8000 keys: 191 us with two, 182 with three; an e4m3 cache of 4 x 110000 keys: 220 and 202.
-template <int MT>
-__host__ __device__ constexpr int ctas_per_sm() { return MT == 1 ? 3 : 2; }
+template <int R>
+__host__ __device__ constexpr int ctas_per_sm() { return R <= 16 ? 3 : 2; }
 template <int DP, bool E4M3>
 __host__ __device__ constexpr int stage_bytes() { return 2 * kKeys * DP * (E4M3 ? 1 : 2); }
-template <bool E4M3, int MT>
-__host__ __device__ constexpr int stages() { return (E4M3 ? 2 : 1) * (MT == 1 ? 2 : 3); }
-template <int DP, bool E4M3, int MT>
-__host__ __device__ constexpr int ring_bytes() { return kWarps * stages<E4M3, MT>() * stage_bytes<DP, E4M3>(); }
+template <bool E4M3, int R>
+__host__ __device__ constexpr int stages() { return (E4M3 ? 2 : 1) * (R <= 16 ? 2 : 3); }
+template <int DP, bool E4M3, int R>
+__host__ __device__ constexpr int ring_bytes() { return kWarps * stages<E4M3, R>() * stage_bytes<DP, E4M3>(); }
 template <int R, int DP>
 __host__ __device__ constexpr int merge_bytes() { return kWarps * R * (DP + 8) * 4 + kWarps * R * 8 + R * 8 + R * DP * 4; }
 
@@ -43,6 +43,17 @@ __device__ __forceinline__ uint32_t ld_shared4(uint32_t src) {
   uint32_t x;
   asm volatile("ld.shared.b32 %0, [%1];" : "=r"(x) : "r"(src) : "memory");
   return x;
+}
+__device__ __forceinline__ uint32_t ld_shared2(uint32_t src) {
+  uint16_t x;
+  asm volatile("ld.shared.b16 %0, [%1];" : "=h"(x) : "r"(src) : "memory");
+  return x;
+}
+// Of an 8x8 matrix of 16-bit elements, two neighbours of a row in each lane.
+__device__ __forceinline__ uint32_t transposed8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -84,17 +95,18 @@ struct DirectPiece {
 // DIRECT: for short contexts, where dividing the batch and joining the pieces (two dependent steps of about 2 us and a launch) cost
 // more than they even out: a cluster of p.slices CTAs per sequence and kv head, which add their rows through shared memory.  (64
 // keys take a CTA 1 us, by the length of its chain of instructions: a ring of five stages instead of two changed nothing.)
-template <typename T, bool E4M3, int DP, int MT, bool DIRECT>
-__global__ void __launch_bounds__(kThreads, ctas_per_sm<MT>()) attention_stream_kernel(const __grid_constant__ AttnParams p) {
+template <typename T, bool E4M3, int DP, int R, bool DIRECT>
+__global__ void __launch_bounds__(kThreads, ctas_per_sm<R>()) attention_stream_kernel(const __grid_constant__ AttnParams p) {
   using M = std::conditional_t<E4M3, __half, T>;
-  constexpr int R = 16 * MT, S = stages<E4M3, MT>(), SB = stage_bytes<DP, E4M3>();
+  constexpr bool NARROW = R == 8;          // the transposed form
+  constexpr int MT = NARROW ? 1 : R / 16, S = stages<E4M3, R>(), SB = stage_bytes<DP, E4M3>();
   constexpr int ES = E4M3 ? 1 : 2;
   constexpr int CH = DP * ES / 16;            // 16-byte chunks of a key's row
   constexpr int KS = DP / 16;                 // 16-element steps of the score product
   constexpr int NT = DP / 8;                  // 8-column tiles of the output
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ AttnScratch s_scan;
-  grid_launch_dependents();
+  if constexpr (DIRECT) grid_launch_dependents();
   grid_dependency_wait();
   const int lane = threadIdx.x & 31, warp = tc::uniform_warp();
   const int g = lane >> 2, t4 = lane & 3;
@@ -114,17 +126,24 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<MT>()) attention_stream_
     const int k_end = min((long long)key_hi(p, seq, tok1), ((long long)unit0 + n_units) * kUnit);
 
     // ---- query rows as operand fragments (their loads go out before those of the keys wait for the page table) ----
-    uint32_t qf[MT][KS][4];
-    int lo[MT][2], hi[MT][2];
+    constexpr int HALVES = NARROW ? 1 : 2;          // of 8 rows in a fragment
+    uint32_t qf[MT][KS][2 * HALVES];
+    int lo[MT][2], hi[MT][2];                       // keys that the two rows of this lane's scores see
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
+        const int row = NARROW ? 2 * t4 + half : m * 16 + half * 8 + g;
+        const bool live = row < n_rows;
+        const int tok = it.token(p, live ? row : 0);
+        lo[m][half] = live ? key_lo(p, seq, tok) : 0;
+        hi[m][half] = live ? key_hi(p, seq, tok) : 0;
+      }
+#pragma unroll
+      for (int half = 0; half < HALVES; ++half) {
         const int row = m * 16 + half * 8 + g;
         const bool live = row < n_rows;
         const int tok = it.token(p, live ? row : 0), qh = it.q_head(p, live ? row : 0);
-        lo[m][half] = live ? key_lo(p, seq, tok) : 0;
-        hi[m][half] = live ? key_hi(p, seq, tok) : 0;
         const char *src = reinterpret_cast<const char *>(p.q) + ((seq.q0 + tok) * p.q_st + qh * p.q_sh) * 2;
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
@@ -132,7 +151,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<MT>()) attention_stream_
           for (int part = 0; part < 2; ++part) {
             // e4m3: a lane's four bytes of a key are elements 4t..4t+3 of a step, whichever column of the product they are
             const int e = 16 * s + (E4M3 ? 4 * t4 + 2 * part : 8 * part + 2 * t4);
-            qf[m][s][2 * part + half] = live && e < p.d ? *reinterpret_cast<const uint32_t *>(src + e * 2) : 0u;
+            qf[m][s][HALVES * part + half] = live && e < p.d ? *reinterpret_cast<const uint32_t *>(src + e * 2) : 0u;
           }
         }
       }
@@ -145,8 +164,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<MT>()) attention_stream_
     const char *vb = reinterpret_cast<const char *>(p.v) + head * p.v_sh * ES;
     const int32_t *pages = p.table + b * p.table_stride;
     const int key0 = unit0 * kUnit + warp * kKeys;
-    // Pages of a power of two of at least 16 slots hold a warp's 16 keys in one: every lane has their page and the slot of the
-    // first.  Else lane 0-15 have the page and slot of a key each.  The lookup is one stage ahead of the copies.
+    // Pages of a power of two of at least 16 slots hold a warp's 16 keys in one: a lookup is of 32 units, one per lane, and made up to
+    // 64 units ahead.  Else lane 0-15 have the page and slot of a key each, two units ahead of the copies.
     const bool one_page = p.page_shift >= 4;
     auto page_id = [&](int i) -> int {
       const int first = key0 + i * kUnit, key = first + (one_page ? 0 : lane & 15);
@@ -156,13 +175,16 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<MT>()) attention_stream_
       tc::report_timeout(p.status, kStatusBadIndex);
       return -1;
     };
-    int ids[S];
-#pragma unroll
-    for (int i = 0; i < S; ++i) ids[i] = page_id(i);      // lookups of the first stages at once
-    int ahead = ids[0];
+    auto swizzled = [](int row, int c) { return CH == 4 ? (c ^ ((row >> 1) & 3)) : (c ^ (row & 7)); };
+    int ids = page_id(one_page ? lane : 0), next_ids = page_id(one_page ? 32 + lane : 1);
     auto issue = [&](int i) {
-      const int id = ahead;
-      ahead = i + 1 < S ? ids[i + 1] : page_id(i + 1);
+      int id = ids;
+      if (one_page) {
+        id = __shfl_sync(0xffffffffu, ids, i & 31);
+        if ((i & 31) == 31) ids = next_ids, next_ids = page_id(i + 33 + lane);
+      } else {
+        ids = next_ids, next_ids = page_id(i + 2);
+      }
       if (i < n_units) {
         const int first = key0 + i * kUnit;
         constexpr int RP = 32 / CH;            // rows per pass of the warp
@@ -170,8 +192,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<MT>()) attention_stream_
         const int bytes = min(max(p.d * ES - c * 16, 0), 16);
         const uint32_t dst = ring_addr + (i % S) * SB;
         auto copy = [&](int row, bool live, const char *k, const char *v) {
-          const int sw = CH == 4 ? (c ^ ((row >> 1) & 3)) : (c ^ (row & 7));
-          const uint32_t at = dst + row * (CH * 16) + sw * 16;
+          const uint32_t at = dst + row * (CH * 16) + swizzled(row, c) * 16;
           cp_async16(at, live ? k : kb, live ? bytes : 0);
           cp_async16(at + SB / 2, live ? v : vb, live ? bytes : 0);
         };
@@ -179,12 +200,22 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<MT>()) attention_stream_
           const int slot = (first & (p.page - 1)) + sub;
           const char *k = kb + ((int64_t)id * p.k_sp + slot * p.k_ss) * ES + c * 16, *v = vb + ((int64_t)id * p.v_sp + slot * p.v_ss) * ES + c * 16;
           const int64_t k_step = p.k_ss * (RP * ES), v_step = p.v_ss * (RP * ES);
-          const bool any = id >= 0 && bytes > 0;
+          if (id >= 0 && first >= k_begin && first + kKeys <= k_end && p.d == DP) {      // (all of the warp)
 #pragma unroll
-          for (int j = 0; j < kKeys / RP; ++j) {
-            const int row = j * RP + sub;
-            copy(row, any && first + row >= k_begin && first + row < k_end, k, v);
-            k += k_step, v += v_step;
+            for (int j = 0; j < kKeys / RP; ++j) {
+              const int row = j * RP + sub;
+              const uint32_t at = dst + row * (CH * 16) + swizzled(row, c) * 16;
+              cp_async16(at, k), cp_async16(at + SB / 2, v);
+              k += k_step, v += v_step;
+            }
+          } else {
+            const bool any = id >= 0 && bytes > 0;
+#pragma unroll
+            for (int j = 0; j < kKeys / RP; ++j) {
+              const int row = j * RP + sub;
+              copy(row, any && first + row >= k_begin && first + row < k_end, k, v);
+              k += k_step, v += v_step;
+            }
           }
         } else {
           const int key = first + (lane & 15), slot = key - page_of(p, key) * p.page;
@@ -206,7 +237,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<MT>()) attention_stream_
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
+      for (int half = 0; half < HALVES; ++half) {
         mul[m][half] = head_scale;
         if constexpr (E4M3) {
           float top = 0.f;
@@ -214,7 +245,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<MT>()) attention_stream_
           for (int s = 0; s < KS; ++s) {
 #pragma unroll
             for (int part = 0; part < 2; ++part) {
-              const float2 f = unpack2(qf[m][s][2 * part + half], T(0.f));
+              const float2 f = unpack2(qf[m][s][HALVES * part + half], T(0.f));
               top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
             }
           }
@@ -227,20 +258,29 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<MT>()) attention_stream_
           for (int s = 0; s < KS; ++s) {
 #pragma unroll
             for (int part = 0; part < 2; ++part) {
-              const float2 f = unpack2(qf[m][s][2 * part + half], T(0.f));
-              qf[m][s][2 * part + half] = pack2(f.x * down, f.y * down, M(0.f));
+              const float2 f = unpack2(qf[m][s][HALVES * part + half], T(0.f));
+              qf[m][s][HALVES * part + half] = pack2(f.x * down, f.y * down, M(0.f));
             }
           }
         }
       }
     }
 
+    if constexpr (NARROW) {      // from the row of this lane's query fragment to the rows of its scores
+      const float mine = mul[0][0];
+#pragma unroll
+      for (int half = 0; half < 2; ++half) mul[0][half] = __shfl_sync(0xffffffffu, mine, (2 * t4 + half) * 4);
+    }
+
     // ---- one pass over the keys -------------------------------------------------------------------------------
-    float o[MT][NT][4], top[MT][2], sum[MT][2];
+    // What lane (g, t) holds of the sums: rows g and g + 8 of the item, columns 8n + 2t, + 1 (o[n][2 * half + e]).  NARROW: rows
+    // 2t and 2t + 1, columns 16n + g and + 8 (o[n][2 * which + half]).  (e4m3: see column() below.)
+    constexpr int OT = NARROW ? NT / 2 : NT;
+    float o[MT][OT][4], top[MT][2], sum[MT][2];
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
 #pragma unroll
-      for (int n = 0; n < NT; ++n) o[m][n][0] = o[m][n][1] = o[m][n][2] = o[m][n][3] = 0.f;
+      for (int n = 0; n < OT; ++n) o[m][n][0] = o[m][n][1] = o[m][n][2] = o[m][n][3] = 0.f;
       top[m][0] = top[m][1] = -INFINITY;
       sum[m][0] = sum[m][1] = 0.f;
     }
@@ -256,10 +296,32 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<MT>()) attention_stream_
 #pragma unroll
         for (int n = 0; n < 2; ++n) sc[m][n][0] = sc[m][n][1] = sc[m][n][2] = sc[m][n][3] = 0.f;
       auto frag_addr = [&](uint32_t base, int row, int c) {
-        const int sw = CH == 4 ? (c ^ ((row >> 1) & 3)) : (c ^ (row & 7));
-        return base + row * (CH * 16) + sw * 16;
+        return base + row * (CH * 16) + swizzled(row, c) * 16;
       };
-      if constexpr (!E4M3) {
+      if constexpr (NARROW) {      // keys are the rows of the product; even and odd steps are added apart
+        if constexpr (!E4M3) {
+#pragma unroll
+          for (int s = 0; s < KS; ++s) {
+            uint32_t kf[4];   // the step's first half: keys 0-7, keys 8-15; its second
+            ldmatrix4(kf, frag_addr(ks, lane & 15, 2 * s + (lane >> 4)));
+            mma16816(sc[0][s & 1], kf, qf[0][s][0], qf[0][s][1], M(0.f));
+          }
+        } else {
+#pragma unroll
+          for (int s = 0; s < KS; s += 2) {
+            uint32_t kf[4];   // step s: keys 0-7, keys 8-15; step s + 1: the same
+            ldmatrix4(kf, frag_addr(ks, lane & 15, s + (lane >> 4)));
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint2 x = e4m3x4_to_f16x4(kf[2 * h]), y = e4m3x4_to_f16x4(kf[2 * h + 1]);
+              const uint32_t a[4] = {x.x, y.x, x.y, y.y};
+              mma16816(sc[0][h], a, qf[0][s + h][0], qf[0][s + h][1], M(0.f));
+            }
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[0][0][e] += sc[0][1][e];
+      } else if constexpr (!E4M3) {
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
           uint32_t kf[4];   // keys 0-7: both halves of the step, keys 8-15: both halves
@@ -292,43 +354,55 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<MT>()) attention_stream_
       uint32_t pf[MT][4];
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
+        // scores of this lane's row `half`: columns 2t, 2t + 1 of both tiles of keys; NARROW: keys g and g + 8
+        constexpr int PER = NARROW ? 2 : 4;
+        auto score = [&](int half, int e) -> float & { return NARROW ? sc[m][0][2 * e + half] : sc[m][e >> 1][2 * half + (e & 1)]; };
         float mx[2];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           if (!inside) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int key = kbase + (e >> 1) * 8 + 2 * t4 + (e & 1);
-              if (key < max(lo[m][half], k_begin) || key >= min(hi[m][half], k_end)) sc[m][e >> 1][2 * half + (e & 1)] = -INFINITY;
+            for (int e = 0; e < PER; ++e) {
+              const int key = kbase + (NARROW ? 8 * e + g : (e >> 1) * 8 + 2 * t4 + (e & 1));
+              if (key < max(lo[m][half], k_begin) || key >= min(hi[m][half], k_end)) score(half, e) = -INFINITY;
             }
           }
-          mx[half] = fmaxf(fmaxf(sc[m][0][2 * half], sc[m][0][2 * half + 1]), fmaxf(sc[m][1][2 * half], sc[m][1][2 * half + 1]));
-          mx[half] = fmaxf(mx[half], __shfl_xor_sync(0xffffffffu, mx[half], 1));
-          mx[half] = fmaxf(mx[half], __shfl_xor_sync(0xffffffffu, mx[half], 2)) * mul[m][half];
+          mx[half] = fmaxf(score(half, 0), score(half, 1));
+          if constexpr (!NARROW) mx[half] = fmaxf(mx[half], fmaxf(score(half, 2), score(half, 3)));
+          mx[half] *= mul[m][half];
         }
         // the reference of the exponents follows the maximum only when it has fallen far behind
         if (__any_sync(0xffffffffu, mx[0] > top[m][0] + kLazyRescale || mx[1] > top[m][1] + kLazyRescale)) {
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
+            for (int v = NARROW ? 4 : 1; v < (NARROW ? 32 : 4); v *= 2) mx[half] = fmaxf(mx[half], __shfl_xor_sync(0xffffffffu, mx[half], v));
             const float to = fmaxf(top[m][half], mx[half]);
             const float f = top[m][half] == -INFINITY ? 0.f : exp2_fast(top[m][half] - to);
             sum[m][half] *= f;
 #pragma unroll
-            for (int n = 0; n < NT; ++n) o[m][n][2 * half] *= f, o[m][n][2 * half + 1] *= f;
+            for (int n = 0; n < OT; ++n)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) o[m][n][NARROW ? 2 * e + half : 2 * half + e] *= f;
             top[m][half] = to;
           }
         }
+        float x[2][4];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           const float neg = top[m][half] == -INFINITY ? 0.f : -top[m][half];
-          float x[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            x[e] = exp2_fast(fmaf(sc[m][e >> 1][2 * half + (e & 1)], mul[m][half], neg));
-            sum[m][half] += x[e];
+          for (int e = 0; e < PER; ++e) {
+            x[half][e] = exp2_fast(fmaf(score(half, e), mul[m][half], neg));
+            sum[m][half] += x[half][e];
           }
-          pf[m][half] = pack2(x[0], x[1], M(0.f));
-          pf[m][2 + half] = pack2(x[2], x[3], M(0.f));
+        }
+        if constexpr (NARROW) {    // [key][row] to [row][key]
+          pf[m][0] = transposed8x8(pack2(x[0][0], x[1][0], M(0.f)));
+          pf[m][1] = transposed8x8(pack2(x[0][1], x[1][1], M(0.f)));
+        } else {
+#pragma unroll
+          for (int half = 0; half < 2; ++half)
+            pf[m][half] = pack2(x[half][0], x[half][1], M(0.f)), pf[m][2 + half] = pack2(x[half][2], x[half][3], M(0.f));
         }
       }
       if (!inside && tok0 != tok1) {     // rows that see different keys: values that are not finite apart
@@ -345,9 +419,22 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<MT>()) attention_stream_
           for (int r = 0; r < kKeys; ++r) {
             const int key = kbase + r;
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {       // this lane's two columns of tile n
-              const uint32_t w = ld_shared4(frag_addr(vs, r, E4M3 ? n / 2 : n) + t4 * 4), x = w & bad(w);
+            for (int n = 0; n < OT; ++n) {       // this lane's two columns of tile n
               float2 f;
+              if constexpr (NARROW) {
+                const uint32_t w = E4M3 ? ld_shared2(frag_addr(vs, r, n) + g * 2)
+                                        : ld_shared2(frag_addr(vs, r, 2 * n) + g * 2) | ld_shared2(frag_addr(vs, r, 2 * n + 1) + g * 2) << 16;
+                const uint32_t x = w & bad(w);
+                if constexpr (E4M3) f = unpack2(e4m3x4_to_f16x4(x).x, M(0.f));
+                else f = unpack2(x, M(0.f));
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                  if (key < max(lo[0][half], k_begin) || key >= min(hi[0][half], k_end)) continue;
+                  o[0][n][half] += f.x, o[0][n][2 + half] += f.y;
+                }
+                continue;
+              }
+              const uint32_t w = ld_shared4(frag_addr(vs, r, E4M3 ? n / 2 : n) + t4 * 4), x = w & bad(w);
               if constexpr (E4M3) {
                 const uint2 h = e4m3x4_to_f16x4(__byte_perm(x, 0, 0x3120));
                 f = unpack2(n & 1 ? h.y : h.x, M(0.f));
@@ -375,7 +462,28 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<MT>()) attention_stream_
         }
       }
       // output rows
-      if constexpr (!E4M3) {
+      if constexpr (NARROW) {      // columns are the rows of the product
+        if constexpr (!E4M3) {
+#pragma unroll
+          for (int n = 0; n < OT; ++n) {
+            uint32_t vf[4];   // keys 0-7: columns 16n.., the next eight; keys 8-15
+            ldmatrix4_trans(vf, frag_addr(vs, (lane & 7) + ((lane >> 4) << 3), 2 * n + ((lane >> 3) & 1)));
+            mma16816(o[0][n], vf, pf[0][0], pf[0][1], M(0.f));
+          }
+        } else {
+#pragma unroll
+          for (int n = 0; n < OT; n += 2) {
+            uint32_t vf[4];   // chunk n: keys 0-7, 8-15; the next chunk.  A transposed unit is two neighbours of one key.
+            ldmatrix4_trans(vf, frag_addr(vs, lane & 15, n + (lane >> 4)));
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint2 x = e4m3x4_to_f16x4(__byte_perm(vf[2 * h], 0, 0x3120)), y = e4m3x4_to_f16x4(__byte_perm(vf[2 * h + 1], 0, 0x3120));
+              const uint32_t a[4] = {x.x, x.y, y.x, y.y};      // the even columns of the chunk, the odd ones
+              mma16816(o[0][n + h], a, pf[0][0], pf[0][1], M(0.f));
+            }
+          }
+        }
+      } else if constexpr (!E4M3) {
 #pragma unroll
         for (int n = 0; n < NT; n += 2) {
           uint32_t vf[4];   // columns 8n..: keys 0-7, 8-15; the next eight columns: the same
@@ -413,10 +521,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<MT>()) attention_stream_
     for (int m = 0; m < MT; ++m) {
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        sum[m][half] += __shfl_xor_sync(0xffffffffu, sum[m][half], 1);
-        sum[m][half] += __shfl_xor_sync(0xffffffffu, sum[m][half], 2);
+#pragma unroll
+        for (int v = NARROW ? 4 : 1; v < (NARROW ? 32 : 4); v *= 2) sum[m][half] += __shfl_xor_sync(0xffffffffu, sum[m][half], v);
         if (sum[m][half] != sum[m][half]) top[m][half] = INFINITY;   // a NaN outweighs the other warps' rows
-        if (t4 == 0) merge_ml[warp * R + m * 16 + half * 8 + g] = make_float2(top[m][half], sum[m][half]);
+        if (NARROW ? g == 0 : t4 == 0) merge_ml[warp * R + (NARROW ? 2 * t4 + half : m * 16 + half * 8 + g)] = make_float2(top[m][half], sum[m][half]);
       }
     }
     __syncthreads();
@@ -424,13 +532,19 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<MT>()) attention_stream_
     for (int m = 0; m < MT; ++m) {
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const int row = m * 16 + half * 8 + g;
+        const int row = NARROW ? 2 * t4 + half : m * 16 + half * 8 + g;
         float best = -INFINITY;
 #pragma unroll
         for (int v = 0; v < kWarps; ++v) best = fmaxf(best, merge_ml[v * R + row].x);
         const float f = top[m][half] == -INFINITY ? 0.f : exp2_fast(top[m][half] - best);
         float *dst = merge_o + (warp * R + row) * (DP + 8);
-        if constexpr (!E4M3) {
+        if constexpr (NARROW) {
+#pragma unroll
+          for (int n = 0; n < OT; ++n) {
+            if constexpr (E4M3) *reinterpret_cast<float2 *>(dst + 16 * n + 2 * g) = make_float2(o[m][n][half] * f, o[m][n][2 + half] * f);
+            else dst[16 * n + g] = o[m][n][half] * f, dst[16 * n + 8 + g] = o[m][n][2 + half] * f;
+          }
+        } else if constexpr (!E4M3) {
 #pragma unroll
           for (int n = 0; n < NT; ++n)
             *reinterpret_cast<float2 *>(dst + 8 * n + 2 * t4) = make_float2(o[m][n][2 * half] * f, o[m][n][2 * half + 1] * f);
@@ -524,37 +638,42 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<MT>()) attention_stream_
     if (threadIdx.x == 0) p.meta[blockIdx.x].cut.x = -1;
     AttnWalk<R, kUnit, kExtra> it(range);
     while (it.next(p)) work(it);
+    // Not before the end: blocks of the joining kernel that wait beside these CTAs, and of the next call behind them, cost 64 sequences of
+    // 500 - 8000 keys (e4m3) 143 us instead of 114.
+    grid_launch_dependents();
   }
 }
 
-template <typename T, bool E4M3, int DP, int MT, bool DIRECT>
+template <typename T, bool E4M3, int DP, int R, bool DIRECT>
 int launch_mode(const AttnParams &p, dim3 grid, size_t prefix, cudaStream_t st) {
-  constexpr int ring = ring_bytes<DP, E4M3, MT>(), merge = merge_bytes<16 * MT, DP>();
+  constexpr int ring = ring_bytes<DP, E4M3, R>(), merge = merge_bytes<R, DP>();
   constexpr int fixed = ring > merge ? ring : merge;
   const size_t smem = prefix > fixed ? prefix : fixed;
   static PerDeviceOnce once;
-  auto kern = attention_stream_kernel<T, E4M3, DP, MT, DIRECT>;
+  auto kern = attention_stream_kernel<T, E4M3, DP, R, DIRECT>;
   const int rc = allow_dynamic_smem(once, kern, 110 * 1024);
   if (rc != ZT_SUCCESS) return rc;
   if (!DIRECT || p.slices == 1) ZT_CUDA_OK(launch_overlapped(kern, grid, dim3(kThreads), smem, st, p));
   else ZT_CUDA_OK(launch_overlapped_cluster(kern, grid, dim3(kThreads), smem, st, dim3((unsigned)p.slices), p));
   return launch_status("attention_stream_kernel");
 }
-template <typename T, bool E4M3, int DP, int MT>
+template <typename T, bool E4M3, int DP, int R>
 int launch(const AttnParams &p, const AttnPlan &plan, cudaStream_t st) {
   // (the division of the batch comes before the first copy and has the shared memory to itself)
-  if (plan.slices == 0) return launch_mode<T, E4M3, DP, MT, false>(p, dim3(plan.grid), (size_t)(p.batch + 1) * 4, st);
-  return launch_mode<T, E4M3, DP, MT, true>(p, dim3((unsigned)(p.batch * p.hkv * plan.slices)), 0, st);
+  if (plan.slices == 0) return launch_mode<T, E4M3, DP, R, false>(p, dim3(plan.grid), (size_t)(p.batch + 1) * 4, st);
+  return launch_mode<T, E4M3, DP, R, true>(p, dim3((unsigned)(p.batch * p.hkv * plan.slices)), 0, st);
 }
 template <typename T, bool E4M3>
 int launch_sized(const AttnParams &p, const AttnPlan &plan, cudaStream_t st) {
-  if (plan.dp == 64) return plan.rows == 16 ? launch<T, E4M3, 64, 1>(p, plan, st) : launch<T, E4M3, 64, 2>(p, plan, st);
-  return plan.rows == 16 ? launch<T, E4M3, 128, 1>(p, plan, st) : launch<T, E4M3, 128, 2>(p, plan, st);
+  const bool narrow = plan.dp == 64;
+  if (plan.rows == 8) return narrow ? launch<T, E4M3, 64, 8>(p, plan, st) : launch<T, E4M3, 128, 8>(p, plan, st);
+  if (plan.rows == 16) return narrow ? launch<T, E4M3, 64, 16>(p, plan, st) : launch<T, E4M3, 128, 16>(p, plan, st);
+  return narrow ? launch<T, E4M3, 64, 32>(p, plan, st) : launch<T, E4M3, 128, 32>(p, plan, st);
 }
 
 }  // namespace
 
-int attention_stream_grid(int rows) { return (rows == 16 ? ctas_per_sm<1>() : ctas_per_sm<2>()) * sm_count(); }
+int attention_stream_grid(int rows) { return (rows <= 16 ? ctas_per_sm<16>() : ctas_per_sm<32>()) * sm_count(); }
 
 int attention_stream_launch(const AttnParams &p, const AttnPlan &plan, int dtype, int cache_dtype, cudaStream_t st) {
   const bool e4m3 = cache_dtype == ZT_E4M3;
