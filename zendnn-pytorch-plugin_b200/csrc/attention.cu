@@ -220,14 +220,16 @@ cudaError_t launch_combine(const AttnParams &p, const AttnPlan &plan, cudaStream
 
 size_t align256(size_t v) { return (v + 255) / 256 * 256; }
 
-// CTAs per sequence and kv head where block_table has room for `keys` keys each, 0: the units are dealt out.  A CTA takes about
-// 1 us for 64 keys, dealing and joining about 4 us, and clusters of 512 and more CTAs take longer to place than they save.  Direct
-// against dealt, ragged lengths of keys / 10 to keys, in us: 16 items of 2048 keys 9.9 / 12.9 (8 CTAs each), 128 of 512 11.7 / 11.9
-// (2), 128 of 1024 16.6 / 15.3, 512 of 256 14.8 / 18.1 (1), 512 of 512 21.3 / 23.1, 512 of 1024 38.4 / 35.0.
-int direct_slices(int64_t keys, int64_t items) {
+// CTAs per sequence and kv head where block_table has room for `keys` keys each, 0: the units are dealt out.  A CTA takes 1 us for
+// 64 keys, dealing and joining about 4 us, and clusters of 512 and more CTAs take longer to place than they save.  Many items even
+// themselves out as they come, but one long sequence among short ones is left to its CTA: hence the bound there too.  Direct against
+// dealt, ragged lengths of keys / 10 to keys (bf16, groups of 4), in us: 8 items of 4096 keys 6.6 / 10.1 (8 CTAs each), 32 of 4096
+// 9.9 / 12.6 (8), 128 of 1024 11.9 / 13.0 (2) and of 2048 17.6 / 15.3, 512 of 320 12.2 / 16.5 (1), of 768 25.2 / 28.0 and of 2048
+// 57.4 / 57.5, 2048 of 768 72 / 77 and of 2048 171 / 179 (e4m3: 100 / 120).
+int direct_slices(int64_t keys, int64_t items, int ctas) {
   int s = 8;
   while (s > 1 && (items * s > 256 || keys <= 64 * s)) s /= 2;
-  return keys <= 320 * s ? s : 0;
+  return keys <= (items >= 2 * ctas ? 2048 : 768 * s) ? s : 0;
 }
 
 AttnPlan make_plan(const zt_paged_attention_args_t &a) {
@@ -244,7 +246,7 @@ AttnPlan make_plan(const zt_paged_attention_args_t &a) {
   plan.grid = plan.tcgen05 ? sm_count() : attention_stream_grid(plan.rows);
   plan.few = rows <= 4 * plan.rows;
   const int64_t keys = (int64_t)a.page_size * a.max_blocks, items = (int64_t)a.batch * a.kv_heads;
-  if (!plan.tcgen05 && items > 0) plan.slices = hint ? (hint == 1 ? 0 : hint - 1) : direct_slices(keys, items);
+  if (!plan.tcgen05 && items > 0) plan.slices = hint ? (hint == 1 ? 0 : hint - 1) : direct_slices(keys, items, plan.grid);
   if (plan.slices > 0) {
     plan.grid = 0;
     plan.meta_bytes = 256;      // (nothing is kept there)

@@ -5,8 +5,19 @@
 // in shared memory (16-byte asynchronous copies, whose zero fill also blanks slots past the visible keys, so stale contents of a
 // page never meet the arithmetic) and keeps its own maxima, sums and output rows in registers: no barrier between warps until
 // the item ends, where the four are added through shared memory.  Two or three CTAs share an SM, so that others stream while one
-// is in such an end.  Rows are the 16-row (or twice 16) operand of mma.sync.m16n8k16, keys its columns; the accumulator layout of
-// the scores is the operand layout of the probabilities.  e4m3 keys and values become halves in registers, which is exact; the
+// is in such an end.
+//
+// For 16 and 32 rows those are the 16-row operand of mma.sync.m16n8k16, keys its columns; the accumulator layout of the scores is the
+// operand layout of the probabilities.  For up to 8 rows (decode with groups of up to 8) they are the 8 columns instead, and keys, then
+// columns of the values, the 16 rows: half as many accumulators, exponentials and products, for two transpositions of the
+// probabilities per 16 keys.  One token over 700 keys 7.6 us with 16 rows, 6.8 with 8; 256 sequences of 100 - 600 keys 67.6 and 64.3;
+// 17 of 9000 - 14500, heads of 64, 16.0 and 14.7; where HBM is the bound there is no difference.
+//
+// Bound by HBM for 16-bit caches: 64 sequences of 500 - 8000 keys (32 heads over 8, 128 wide) take 182 us, 6.3 TB/s of the 6.55 that a
+// copy reaches.  An e4m3 cache takes 115 us, 5.0 TB/s: half the bytes, and as many instructions for each of its keys (0.4 issued per
+// cycle, the rest is the chain of a warp's copy, conversions, products and exponentials, at twelve warps an SM).
+//
+// e4m3 keys and values become halves in registers, which is exact; the
 // products then run in fp16 with query rows brought to a maximum below 2 by a power of two (what that takes from an element is
 // below 2^-25 of its row's largest).  Probabilities are rounded to the type of the product (half a step of 2^-8 or 2^-11 of
 // each, added by the tensor cores in fp32); the sum that divides them is of the unrounded fp32 values.
@@ -22,8 +33,8 @@ constexpr int kKeys = 16;                  // of a warp per unit
 constexpr int kUnit = kWarps * kKeys;
 constexpr int kExtra = 2;                  // units that an item costs beside its own
 
-// Three CTAs share an SM where their rows leave the registers (16 rows; 64 kept keys ahead per CTA), else two.  Decode of 64
-// sequences of 500 - 8000 keys: 191 us with two, 182 with three; an e4m3 cache of 4 x 110000 keys: 220 and 202.
+// Three CTAs share an SM where their rows leave the registers (up to 16 rows; 64 kept keys ahead per CTA), else two.  Decode of 64
+// sequences of 500 - 8000 keys: 191 us with two, 182 with three; an e4m3 cache of 4 x 110000 keys (16 rows): 220 and 202.
 template <int R>
 __host__ __device__ constexpr int ctas_per_sm() { return R <= 16 ? 3 : 2; }
 template <int DP, bool E4M3>
