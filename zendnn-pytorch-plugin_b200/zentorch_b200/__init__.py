@@ -9,6 +9,9 @@ After import, the reference's operator calls work unchanged on CUDA tensors::
 
     y = torch.ops.zentorch.zentorch_woq_linear(x, packed.t(), scales, None, bias)
     y = torch.ops.zentorch.zentorch_dynamic_qlinear(x, w_int8, w_scales, bias)
+
+and beside them stand this library's own for what comes between a decoder layer's projections: ``zentorch_rope``,
+``zentorch_rope_cache``, ``zentorch_cache_copy_pages`` and ``zentorch_paged_attention``, with ``zentorch_b200.cache`` around them.
 """
 from __future__ import annotations
 
