@@ -8,9 +8,11 @@
 //
 // Bound by memory: every element is read once and written once.  A block takes up to eight tokens, as many as its 256 threads have
 // angles to compute at once, and the first 16-byte loads are in flight meanwhile: with one token per block three quarters of the
-// threads waited for the others' angles, and 8192 tokens of 64 heads took 69 us.
+// threads waited for the others' angles, and 8192 tokens of 64 heads took 69 us instead of 48 (5.5 TB/s).
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
+
+#include <algorithm>
 
 #include "tc05.cuh"
 
@@ -235,11 +237,13 @@ cudaError_t launch_rope(RopeParams p, int cache, cudaStream_t st) {   // cache: 
   p.magic_rot = magic_of(rot), p.magic_rest = magic_of(rest), p.magic_whole = magic_of(whole);
   const int items = (p.hq + p.hkv) * (rot + rest) + (cache ? p.hkv * whole : 0);
   p.magic_token = magic_of(items);
-  // as many tokens as give every thread an angle, or (tokens of few items) an item; fewer where that leaves SMs without a block
-  const int by_angles = p.rot > 0 ? kRopeThreads / (p.rot / 2) : kMaxTokens, by_items = ceil_div(kRopeThreads, items);
-  int t = by_angles > by_items ? by_angles : by_items;
-  const int spread = ceil_div(p.tokens, 2 * sm_count());
-  if (t > spread) t = spread;
+  // As many tokens as give every thread an angle, or (tokens of few items) an item; fewer where that leaves SMs with few blocks, which
+  // end unevenly: 8192 tokens of 64 heads, half rotated, 55.7 us in 1024 blocks of 8 tokens, 48.4 in 2048.  (Threads without an item
+  // cost more: 8192 tokens of 3 heads of 64 take 5.8 us in blocks of 8 tokens, 7.8 in blocks of 4.)
+  int by_angles = p.rot > 0 ? kRopeThreads / (p.rot / 2) : kMaxTokens, by_items = ceil_div(kRopeThreads, items);
+  by_angles = std::min(by_angles, ceil_div(p.tokens, 16 * sm_count()));
+  by_items = std::min(by_items, ceil_div(p.tokens, 2 * sm_count()));
+  int t = std::max(by_angles, by_items);
   t = t < 1 ? 1 : t > kMaxTokens ? kMaxTokens : t;
   while (t > 1 && (int64_t)items * items * t >= (int64_t)1 << 32) --t;      // quotient() is exact up to there
   p.block_tokens = t;
