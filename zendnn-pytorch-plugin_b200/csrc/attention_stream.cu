@@ -14,8 +14,8 @@
 // 17 of 9000 - 14500, heads of 64, 16.0 and 14.7; where HBM is the bound there is no difference.
 //
 // Bound by HBM for 16-bit caches: 64 sequences of 500 - 8000 keys (32 heads over 8, 128 wide) take 182 us, 6.3 TB/s of the 6.55 that a
-// copy reaches.  An e4m3 cache takes 115 us, 5.0 TB/s: half the bytes, and as many instructions for each of its keys (0.4 issued per
-// cycle, the rest is the chain of a warp's copy, conversions, products and exponentials, at twelve warps an SM).
+// copy reaches.  An e4m3 cache takes 115 us, 5.0 TB/s: its rows are 128 bytes, 1 KB apart (16-bit heads of 64 elements, the same rows,
+// reach 5.8; 6.1 with one kv head, where they are contiguous), and as many instructions go to each key for half the bytes.
 //
 // e4m3 keys and values become halves in registers, which is exact; the
 // products then run in fp16 with query rows brought to a maximum below 2 by a power of two (what that takes from an element is
