@@ -5,6 +5,7 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/record_function.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <c10/util/SmallVector.h>
 #include <torch/library.h>
 
 #include <algorithm>
@@ -162,7 +163,7 @@ at::Tensor rope_cache(const at::Tensor &query, const at::Tensor &key, const at::
 // ---- pages ------------------------------------------------------------------------------------------------
 // Whether the dimensions behind the first are one block without holes, in any order.
 bool dense_pages(const at::Tensor &t) {
-  std::vector<std::pair<int64_t, int64_t>> dims;   // stride, size
+  c10::SmallVector<std::pair<int64_t, int64_t>, 8> dims;   // stride, size
   for (int64_t i = 1; i < t.dim(); ++i)
     if (t.size(i) != 1) dims.emplace_back(t.stride(i), t.size(i));
   std::sort(dims.begin(), dims.end());
@@ -183,15 +184,17 @@ void cache_copy_pages(at::TensorList caches, const at::Tensor &src, const at::Te
   check_index(dst, src, op, "dst", src.size(0));
   TORCH_CHECK(src.scalar_type() == dst.scalar_type(), op, ": src and dst must have one dtype");
   if (caches.empty()) return;
-  std::vector<void *> base;
-  std::vector<int64_t> stride, bytes;
+  c10::SmallVector<void *, 64> base;
+  c10::SmallVector<int64_t, 64> stride, bytes;
+  const at::Tensor &model = caches[0];      // the layers' caches are mostly alike
   for (const at::Tensor &t : caches) {
     check_on_device(t, src, op, "every cache");
     TORCH_CHECK(t.dim() >= 2, op, ": a cache must be [pages, ...], got ", t.dim(), "D");
-    TORCH_CHECK(t.size(0) == caches[0].size(0), op, ": the caches must have one number of pages");
+    TORCH_CHECK(t.size(0) == model.size(0), op, ": the caches must have one number of pages");
     TORCH_CHECK(t.size(0) < (int64_t)1 << 31, op, ": pages of the cache out of range");
     if (t.numel() == 0) continue;
-    TORCH_CHECK(dense_pages(t), op, ": a page of a cache must be one block of memory; got strides ", t.strides(), " for ", t.sizes());
+    const bool alike = !base.empty() && model.numel() > 0 && t.sizes() == model.sizes() && t.strides() == model.strides();
+    TORCH_CHECK(alike || dense_pages(t), op, ": a page of a cache must be one block of memory; got strides ", t.strides(), " for ", t.sizes());
     const int64_t es = (int64_t)t.element_size();
     base.push_back(t.data_ptr());
     bytes.push_back(t.numel() / t.size(0) * es);
@@ -203,7 +206,7 @@ void cache_copy_pages(at::TensorList caches, const at::Tensor &src, const at::Te
   zt_cache_copy_args_t a{};
   a.n_caches = (int32_t)base.size();
   a.caches = base.data(), a.page_stride_bytes = stride.data(), a.page_bytes = bytes.data();
-  a.num_pages = (int32_t)caches[0].size(0);
+  a.num_pages = (int32_t)model.size(0);
   a.n_pairs = s.size(0);
   a.src = s.data_ptr(), a.dst = d.data_ptr(), a.index_64 = s.scalar_type() == at::kLong;
   ZT_TORCH_CALL(zt_cache_copy_pages(&a, at::cuda::getCurrentCUDAStream()));
