@@ -464,7 +464,8 @@ ZT_API int zt_cache_copy_pages(const zt_cache_copy_args_t *args, void *stream);
  * block_table  [batch, max_blocks] int32, row stride in elements: the pages of a sequence in order
  * max_query_len  the most new tokens of a sequence, 0 if unknown: chooses the kernel, results do not depend on it being exact
  * zero_tail    rows of out behind cu[batch] are zeroed; otherwise they are left as they were
- * workspace    zt_paged_attention_workspace_bytes() bytes, 256-byte aligned, contents irrelevant; calls that can overlap need one each
+ * workspace    zt_paged_attention_workspace_bytes() bytes, 256-byte aligned, contents irrelevant; calls that can overlap need one each.
+ *              0 for short contexts (block_table of few keys): then NULL will do
  * out          shares no memory with q or the caches
  * A score of minus infinity counts as a key that is not seen; NaN and infinities of other keys do not reach a row.
  * Lengths that do not fit the tensors are cut, page ids outside the cache read as zeros; both set the device status word (106). */

@@ -248,8 +248,7 @@ AttnPlan make_plan(const zt_paged_attention_args_t &a) {
   const int64_t keys = (int64_t)a.page_size * a.max_blocks, items = (int64_t)a.batch * a.kv_heads;
   if (!plan.tcgen05 && items > 0) plan.slices = hint ? (hint == 1 ? 0 : hint - 1) : direct_slices(keys, items, plan.grid);
   if (plan.slices > 0) {
-    plan.grid = 0;
-    plan.meta_bytes = 256;      // (nothing is kept there)
+    plan.grid = 0;      // nothing is kept between CTAs
     return plan;
   }
   // units of the whole call at most (an item has up to three beside those of its keys)
@@ -314,7 +313,7 @@ extern "C" int zt_paged_attention(const zt_paged_attention_args_t *a, void *stre
              ZT_INVALID_ARGUMENT, "zt_paged_attention: rows of the caches must be 16-byte aligned");
   const AttnPlan plan = make_plan(*a);
   ZT_REQUIRE(plan.most_units < 2147483648.0, ZT_UNSUPPORTED, "zt_paged_attention: more work than one call can number");
-  ZT_REQUIRE(a->workspace && a->workspace_bytes >= plan.total(), ZT_WORKSPACE_TOO_SMALL,
+  ZT_REQUIRE(plan.total() == 0 || (a->workspace && a->workspace_bytes >= plan.total()), ZT_WORKSPACE_TOO_SMALL,
              "zt_paged_attention: workspace of %zu bytes is smaller than the %zu required", a->workspace_bytes, plan.total());
   ZT_REQUIRE((reinterpret_cast<uintptr_t>(a->workspace) & 255) == 0, ZT_INVALID_ARGUMENT,
              "zt_paged_attention: workspace must be 256-byte aligned");

@@ -273,8 +273,11 @@ void paged_attention_into(at::Tensor &out, const at::Tensor &query, const at::Te
   a.scale = (float)scale.value_or(1.0 / std::sqrt((double)D));
   a.causal = causal, a.window = (int32_t)window, a.zero_tail = zero_tail;
   const size_t bytes = zt_paged_attention_workspace_bytes(&a);
-  at::Tensor ws = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
-  a.workspace = ws.data_ptr(), a.workspace_bytes = bytes;
+  at::Tensor ws;
+  if (bytes > 0) {
+    ws = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
+    a.workspace = ws.data_ptr(), a.workspace_bytes = bytes;
+  }
   ZT_TORCH_CALL(zt_paged_attention(&a, at::cuda::getCurrentCUDAStream()));
   if (!direct) out.copy_(y);
 }
