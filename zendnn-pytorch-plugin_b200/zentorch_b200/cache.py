@@ -223,10 +223,14 @@ class PagedKVCache:
                 self._owners[old] -= 1
                 s.pages[-1] = page
             s.pages.extend(self._take() for _ in range(fresh))
-            for t in range(s.length, s.length + count):
-                positions.append(t)
-                slots.append(s.pages[t // self.page_size] * self.page_size + t % self.page_size)
-            s.length += count
+            t, end = s.length, s.length + count
+            positions.extend(range(t, end))
+            while t < end:                                    # page by page
+                first = s.pages[t // self.page_size] * self.page_size + t % self.page_size
+                here = min(end - t, self.page_size - t % self.page_size)
+                slots.extend(range(first, first + here))
+                t += here
+            s.length = end
             starts.append(starts[-1] + count)
             lens.append(s.length)
         self._copy_pages(src, dst)
