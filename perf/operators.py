@@ -9,7 +9,6 @@ and values written to their slots of the cache), ``copy`` (pages of a cache copi
 The inputs are synthetic: queries N(0, 2), keys and values N(0, 1), cache pages handed out in random order, lengths drawn from
 the case's ranges.  Queries, keys and values are views of a fused projection's output, as the layer has them.
 """
-import functools
 import math
 import random
 import sys
@@ -314,9 +313,10 @@ def _plain_attn(s):
 
 
 # ---- one pass --------------------------------------------------------------------------------------------
-@functools.cache
 def _ops():
-    sys.path.insert(0, str(Path.cwd() / "zendnn-pytorch-plugin_b200"))   # the working folder is the repository's root
+    where = str(Path.cwd() / "zendnn-pytorch-plugin_b200")   # the working folder is the repository's root
+    if where not in sys.path:
+        sys.path.insert(0, where)
     import zentorch_b200  # noqa: F401  (registers torch.ops.zentorch)
     return torch.ops.zentorch
 
