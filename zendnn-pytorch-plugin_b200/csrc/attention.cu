@@ -75,8 +75,10 @@ __device__ __forceinline__ float cache_value(const void *base, int64_t at) {
   }
 }
 
-// Goes through a row of the output again, by one warp, where it is not finite: unless its query or a key that it sees holds a NaN,
-// or every such column has a value that is not finite among the keys that the row sees, the row is computed from those keys alone.
+// Goes through a row of the output again, by one warp, where it is not finite: unless its query or a key that it sees holds a NaN, or
+// the values that it sees account for every such column, the row is computed from those keys alone.  A NaN is accounted for by
+// a NaN or by infinities of both signs, an infinity by one of its sign: 0 times the value of a key that the row does not see makes a NaN
+// of an infinity that it does see.
 template <typename T, bool E4M3>
 __device__ __noinline__ void redo_row(const AttnParams &p, int b, const SeqInfo &seq, int head, int r) {
   constexpr int V = 4;                                   // columns of a lane
@@ -88,29 +90,37 @@ __device__ __noinline__ void redo_row(const AttnParams &p, int b, const SeqInfo 
     const int id = p.table[b * p.table_stride + page_of(p, key)];
     return id >= 0 && id < p.num_pages ? id * sp + (key - page_of(p, key) * p.page) * ss + head * sh : -1;
   };
-  uint32_t open = 0;                                     // this lane's columns that want an explanation
+  uint32_t nans = 0, infs[2] = {0, 0};                   // this lane's columns that are NaN, infinite (positive, negative)
+  uint32_t seen_nan = 0, seen_inf[2] = {0, 0};           // columns with such a value among the keys that the row sees
+  auto note = [](float x, int e, uint32_t &is_nan, uint32_t (&is_inf)[2]) {
+    if (isnan(x)) is_nan |= 1u << e;
+    else if (isinf(x)) is_inf[x < 0.f] |= 1u << e;
+  };
+  auto open = [&]() {                                    // columns that want an explanation
+    return (nans & ~(seen_nan | (seen_inf[0] & seen_inf[1]))) | (infs[0] & ~seen_inf[0]) | (infs[1] & ~seen_inf[1]);
+  };
 #pragma unroll
   for (int e = 0; e < V; ++e)
-    if (lane * V + e < p.d && !isfinite((float)out[lane * V + e])) open |= 1u << e;
-  if (!__any_sync(0xffffffffu, open != 0)) return;
+    if (lane * V + e < p.d) note((float)out[lane * V + e], e, nans, infs);
+  if (!__any_sync(0xffffffffu, open() != 0)) return;
   bool nan = false;
 #pragma unroll
   for (int e = 0; e < V; ++e)
     if (lane * V + e < p.d) nan |= isnan((float)q[lane * V + e]);
   if (hi > lo && __any_sync(0xffffffffu, nan)) return;
-  for (int key = hi - 1; key >= lo && __any_sync(0xffffffffu, open != 0); --key) {
+  for (int key = hi - 1; key >= lo && __any_sync(0xffffffffu, open() != 0); --key) {
     const int64_t at = row_of(key, p.v_sp, p.v_ss, p.v_sh), k_at = row_of(key, p.k_sp, p.k_ss, p.k_sh);
 #pragma unroll
     for (int e = 0; e < V; ++e) {
       if (at < 0 || lane * V + e >= p.d) continue;
-      if ((open >> e & 1) && !isfinite(cache_value<T, E4M3>(p.v, at + lane * V + e))) open &= ~(1u << e);
+      note(cache_value<T, E4M3>(p.v, at + lane * V + e), e, seen_nan, seen_inf);
       nan |= isnan(cache_value<T, E4M3>(p.k, k_at + lane * V + e));
     }
     if (__any_sync(0xffffffffu, nan)) return;
   }
-  if (!__any_sync(0xffffffffu, open != 0)) return;
+  if (!__any_sync(0xffffffffu, open() != 0)) return;
   const float mul = p.scale_log2 * (E4M3 ? p.k_scale[head] : 1.f);
-  float acc[V] = {}, top = -INFINITY, sum = 0.f;
+  float acc[V] = {}, special[V] = {}, top = -INFINITY, sum = 0.f;      // special: values that are not finite, which no factor may touch
   for (int first = lo; first < hi; first += 32) {        // a key per lane, then its value by all lanes
     const int key = first + lane;
     float s = -INFINITY;
@@ -134,8 +144,12 @@ __device__ __noinline__ void redo_row(const AttnParams &p, int b, const SeqInfo 
       const float xi = __shfl_sync(0xffffffffu, x, i);
       const int64_t at = row_of(first + i, p.v_sp, p.v_ss, p.v_sh);
 #pragma unroll
-      for (int e = 0; e < V; ++e)
-        if (at >= 0 && lane * V + e < p.d) acc[e] = fmaf(xi, cache_value<T, E4M3>(p.v, at + lane * V + e), acc[e]);
+      for (int e = 0; e < V; ++e) {
+        if (at < 0 || lane * V + e >= p.d) continue;
+        const float v = cache_value<T, E4M3>(p.v, at + lane * V + e);
+        if (isfinite(v)) acc[e] = fmaf(xi, v, acc[e]);
+        else special[e] += v;
+      }
     }
   }
 #pragma unroll
@@ -143,7 +157,7 @@ __device__ __noinline__ void redo_row(const AttnParams &p, int b, const SeqInfo 
   const float f = sum == 0.f ? 0.f : (E4M3 ? p.v_scale[head] : 1.f) / sum;
 #pragma unroll
   for (int e = 0; e < V; ++e)
-    if (lane * V + e < p.d) out[lane * V + e] = (T)(acc[e] * f);
+    if (lane * V + e < p.d) out[lane * V + e] = (T)(acc[e] * f + special[e]);
 }
 
 // The same for the pieces of the tcgen05 kernel, whose rows are neighbours in the workspace: a lane per row, a warp per 16 columns.
