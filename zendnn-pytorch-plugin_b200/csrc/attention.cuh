@@ -307,6 +307,9 @@ __device__ __forceinline__ float2 unpack2(uint32_t w, __nv_bfloat16) {
   return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
 __device__ __forceinline__ float2 unpack2(uint32_t w, __half) { return __half22float2(*reinterpret_cast<const __half2 *>(&w)); }
+// What scores are multiplied by: a cache scale of zero becomes the smallest number there is, so that masked scores stay minus
+// infinity (others come to 2^-21 at most); NaN stays NaN.
+__device__ __forceinline__ float score_factor(float mul) { return mul == 0.f ? __int_as_float(1) : mul; }
 // Power of two that brings a row whose largest element is `top` to a maximum in [1, 2); none for rows of zeros or not finite.
 __device__ __forceinline__ int row_exponent(float top) {
   return top > 0.f && top < __int_as_float(0x7f800000) ? min(max(ilogbf(top), -126), 126) : 0;

@@ -264,7 +264,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<R>()) attention_stream_k
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
           const int ex = row_exponent(top);
           const float down = copysignf(ldexpf(1.f, -ex), p.k_scale[head]);
-          mul[m][half] = fmaxf(head_scale * ldexpf(1.f, ex), 1e-30f);   // (a scale of zero: masked scores stay minus infinity)
+          mul[m][half] = score_factor(head_scale * ldexpf(1.f, ex));
 #pragma unroll
           for (int s = 0; s < KS; ++s) {
 #pragma unroll
@@ -281,6 +281,13 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<R>()) attention_stream_k
       const float mine = mul[0][0];
 #pragma unroll
       for (int half = 0; half < 2; ++half) mul[0][half] = __shfl_sync(0xffffffffu, mine, (2 * t4 + half) * 4);
+    }
+    if constexpr (E4M3) {        // (minus infinity times a scale of NaN, in a row that sees no key)
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+          if (hi[m][half] <= lo[m][half]) mul[m][half] = 1.f;
     }
 
     // ---- one pass over the keys -------------------------------------------------------------------------------

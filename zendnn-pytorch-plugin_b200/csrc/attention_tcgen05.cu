@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tcgen05_kernel(const __
         }
         mul *= fabsf(k_scale) * ldexpf(1.f, my_ex);
       }
-      return fmaxf(mul, 1e-30f);    // a scale of zero: masked scores stay minus infinity
+      return score_factor(mul);
     };
     auto query_ready = [&]() {
       if constexpr (!E4M3) asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -251,6 +251,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tcgen05_kernel(const __
       if (rows > 0) {
         const int tok = it->token(p, i * kTile + (live ? row : 0));
         lo = key_lo(p, it->seq, tok), hi = live ? key_hi(p, it->seq, tok) : 0;
+        if (E4M3 && hi <= lo) mul = 1.f;               // (minus infinity times a scale of NaN, in a row that sees no key)
         all_lo = key_lo(p, it->seq, it->token(p, i * kTile + rows - 1)), all_hi = key_hi(p, it->seq, it->token(p, i * kTile));
       }
       float ref = -INFINITY, sum = 0.f;
