@@ -75,6 +75,23 @@ constexpr int kTcgen05Rows = 256, kTcgen05Unit = 128, kTcgen05Extra = 3;   // ro
 
 constexpr float kLazyRescale = 8.f;   // log2 units that a running maximum may lag behind before sums are rescaled
 
+// The reference of a row's exponents, to which all its probabilities and sums are relative (it cancels in the division).  In
+// bf16 products it follows the maximum.  fp16 numbers end at 2^16 and, with 11 bits, at 2^-14, so there the reference lies 7
+// below the maximum: the largest probability is 2^15 (with the lag), and one of 2^-21 of the largest still has its 11 bits.  Below,
+// a probability is off by up to 2^-25 (half the spacing of subnormals), 2^-32 of a row's sum.  Without this, thousands of keys
+// behind one that outweighs each by 2^25 were lost to the output, while the sum counts them.
+template <typename M>
+constexpr float kHeadroom = std::is_same_v<M, __half> ? 7.f : 0.f;
+// (Rounded up, and the limit down, so that no probability passes 2^15 where scores are so large that fp32 has them 16 apart.)
+template <typename M>
+__device__ __forceinline__ float scaled_maximum(float best, float mul) {
+  return std::is_same_v<M, __half> ? __fmul_ru(best, mul) : best * mul;
+}
+template <typename M>
+__device__ __forceinline__ bool far_ahead(float top, float ref) {
+  return top > (std::is_same_v<M, __half> ? __fadd_rd(ref, kLazyRescale + kHeadroom<M>) : ref + kLazyRescale);
+}
+
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

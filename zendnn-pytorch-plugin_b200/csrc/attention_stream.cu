@@ -20,7 +20,8 @@
 // e4m3 keys and values become halves in registers, which is exact; the
 // products then run in fp16 with query rows brought to a maximum below 2 by a power of two (what that takes from an element is
 // below 2^-25 of its row's largest).  Probabilities are rounded to the type of the product (half a step of 2^-8 or 2^-11 of
-// each, added by the tensor cores in fp32); the sum that divides them is of the unrounded fp32 values.
+// each, in fp16 2^-32 of the row's sum for those that are its subnormals; added by the tensor cores in fp32); the sum that
+// divides them is of the unrounded fp32 values.
 #include "attention.cuh"
 
 namespace zt {
@@ -387,14 +388,14 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<R>()) attention_stream_k
           }
           mx[half] = fmaxf(score(half, 0), score(half, 1));
           if constexpr (!NARROW) mx[half] = fmaxf(mx[half], fmaxf(score(half, 2), score(half, 3)));
-          mx[half] *= mul[m][half];
+          mx[half] = scaled_maximum<M>(mx[half], mul[m][half]);
         }
         // the reference of the exponents follows the maximum only when it has fallen far behind
-        if (__any_sync(0xffffffffu, mx[0] > top[m][0] + kLazyRescale || mx[1] > top[m][1] + kLazyRescale)) {
+        if (__any_sync(0xffffffffu, far_ahead<M>(mx[0], top[m][0]) || far_ahead<M>(mx[1], top[m][1]))) {
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             for (int v = NARROW ? 4 : 1; v < (NARROW ? 32 : 4); v *= 2) mx[half] = fmaxf(mx[half], __shfl_xor_sync(0xffffffffu, mx[half], v));
-            const float to = fmaxf(top[m][half], mx[half]);
+            const float to = fmaxf(top[m][half], mx[half] - kHeadroom<M>);
             const float f = top[m][half] == -INFINITY ? 0.f : exp2_fast(top[m][half] - to);
             sum[m][half] *= f;
 #pragma unroll

@@ -20,7 +20,8 @@
 //
 // The reference of the exponents follows the row maximum only when that has run 8 (log2) ahead of it, so the rows of O are
 // rescaled a few times at the start and hardly ever after; the thread that finds it does it itself.  Probabilities are rounded
-// to the products' type; their sum is of the unrounded fp32 values.  e4m3: fp16 products, query rows brought below 2 by a power of
+// to the products' type (2^-32 of the row's sum is lost of those that are subnormals of fp16); their sum is of the unrounded fp32
+// values.  e4m3: fp16 products, query rows brought below 2 by a power of
 // two as in the streaming kernel.
 #include <algorithm>
 
@@ -291,11 +292,11 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tcgen05_kernel(const __
         if (masked) mask(x[0], 2), mask(x[1], 3);
         maximum(x[0]);
         maximum(x[1]);
-        const float top = fmaxf(best[0], best[1]) * mul;
+        const float top = scaled_maximum<M>(fmaxf(best[0], best[1]), mul);
         if (j == 0) {
-          ref = top;
-        } else if (__any_sync(0xffffffffu, top > ref + kLazyRescale)) {
-          const float to = fmaxf(ref, top), f = ref == -INFINITY ? 0.f : exp2_fast(ref - to);
+          ref = top - kHeadroom<M>;
+        } else if (__any_sync(0xffffffffu, far_ahead<M>(top, ref))) {
+          const float to = fmaxf(ref, top - kHeadroom<M>), f = ref == -INFINITY ? 0.f : exp2_fast(ref - to);
           if (!(ok = tc::warp_wait(o_full, (n_o - 1) & 1))) break;      // the products so far are in O
           tc::fence_after_sync();
 #pragma unroll 1
