@@ -65,19 +65,21 @@ __device__ __forceinline__ Pack<T, VEC> load_pack(const char *base, int64_t elem
     r.e[0] = reinterpret_cast<const T *>(base)[elem];
   return r;
 }
-// VEC values to `base`, as T or, times `inv_scale` and saturated, as e4m3 (round to nearest even in both).
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
+  return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3) |
+         (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3) << 16;
+}
+// VEC values to `base`, as T or, divided by `scale` and saturated, as e4m3 (round to nearest even in both; a product with the rounded
+// reciprocal would move ties, and there is none for scales below 2^-128).
 template <typename T, int VEC, bool E4M3>
-__device__ __forceinline__ void store_pack(char *base, int64_t elem, const float (&v)[VEC], float inv_scale) {
+__device__ __forceinline__ void store_pack(char *base, int64_t elem, const float (&v)[VEC], float scale) {
   if constexpr (E4M3 && VEC == 1) {
-    base[elem] = (char)__nv_cvt_float_to_fp8(v[0] * inv_scale, __NV_SATFINITE, __NV_E4M3);
+    base[elem] = (char)__nv_cvt_float_to_fp8(__fdiv_rn(v[0], scale), __NV_SATFINITE, __NV_E4M3);
   } else if constexpr (E4M3) {
     uint32_t w[VEC / 4];
 #pragma unroll
-    for (int i = 0; i < VEC; i += 4) {
-      const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[i] * inv_scale, v[i + 1] * inv_scale), __NV_SATFINITE, __NV_E4M3);
-      const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[i + 2] * inv_scale, v[i + 3] * inv_scale), __NV_SATFINITE, __NV_E4M3);
-      w[i / 4] = lo | hi << 16;
-    }
+    for (int i = 0; i < VEC; i += 4)
+      w[i / 4] = e4m3x4(__fdiv_rn(v[i], scale), __fdiv_rn(v[i + 1], scale), __fdiv_rn(v[i + 2], scale), __fdiv_rn(v[i + 3], scale));
     if constexpr (VEC == 8) *reinterpret_cast<uint2 *>(base + elem) = make_uint2(w[0], w[1]);
     else *reinterpret_cast<uint32_t *>(base + elem) = w[0];
   } else {
@@ -101,8 +103,10 @@ uint32_t magic_of(int d) { return d > 1 ? (uint32_t)(((1ull << 32) + d - 1) / d)
 
 // An item is two vectors: the two sides of the pairs of a rotated head, or two of the part of a head that passes through or of a
 // value (of an odd number of vectors the last item has one).  Heads are counted through: queries, keys, values; items through the block's tokens.
+// Five blocks share an SM, four with the divisions of an e4m3 cache: 8192 tokens of 64 + 8 heads take 67 us so and 79 with
+// five, whose 48 registers spill (66 with products instead).
 template <typename T, int VEC, bool CACHE, bool E4M3>
-__global__ void __launch_bounds__(kRopeThreads, 5) rope_kernel(const __grid_constant__ RopeParams p) {
+__global__ void __launch_bounds__(kRopeThreads, E4M3 ? 4 : 5) rope_kernel(const __grid_constant__ RopeParams p) {
   __shared__ float2 s_turn[kMaxTokens * kMaxHalf];      // [token][element of a vector][vector]: neighbouring lanes, neighbouring words
   __shared__ int64_t s_row[kMaxTokens][2];              // a token's row in the caches
   grid_launch_dependents();
@@ -214,10 +218,10 @@ __global__ void __launch_bounds__(kRopeThreads, 5) rope_kernel(const __grid_cons
       if (s_row[i.token][0] >= 0) {
         const int h = i.head - (value ? heads : p.hq);
         const int64_t o = row + h * (value ? p.vc_sh : p.kc_sh);
-        const float inv_scale = E4M3 ? __frcp_rn(value ? p.v_scale[h] : p.k_scale[h]) : 1.f;
+        const float scale = E4M3 ? (value ? p.v_scale[h] : p.k_scale[h]) : 1.f;
         char *base = value ? p.v_cache : p.k_cache;
-        store_pack<T, VEC, E4M3>(base, o + e0, a, inv_scale);
-        if (e1 >= 0) store_pack<T, VEC, E4M3>(base, o + e1, b, inv_scale);
+        store_pack<T, VEC, E4M3>(base, o + e0, a, scale);
+        if (e1 >= 0) store_pack<T, VEC, E4M3>(base, o + e1, b, scale);
       }
     } else {
       const int64_t o = token * p.ko_st + (i.head - p.hq) * p.ko_sh;
