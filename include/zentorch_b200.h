@@ -458,11 +458,11 @@ ZT_API int zt_cache_copy_pages(const zt_cache_copy_args_t *args, void *stream);
  *              k_scale / v_scale [kv_heads] fp32 that its values are multiplied by; 16-byte aligned rows.  Slots past a
  *              sequence's length are not read, whatever they hold.
  * head_dim     a multiple of 8 (16 for ZT_E4M3) up to 128
- * cu_seqlens_q [batch + 1] int32: the new tokens of sequence b are rows [cu[b], cu[b+1]); ascending
+ * cu_seqlens_q [batch + 1] int32: the new tokens of sequence b are rows [cu[b], cu[b+1]); ascending, from 0 or more
  * seq_lens     [batch] int32: keys of a sequence, its new tokens' among them
  * block_table  [batch, max_blocks] int32, row stride in elements: the pages of a sequence in order
  * max_query_len  the most new tokens of a sequence, 0 if unknown: chooses the kernel, results do not depend on it being exact
- * zero_tail    rows of out behind cu[batch] are zeroed; otherwise they are left as they were
+ * zero_tail    rows of out before cu[0] and behind cu[batch] are zeroed; otherwise they are left as they were
  * workspace    zt_paged_attention_workspace_bytes() bytes, 256-byte aligned, contents irrelevant; calls that can overlap need one each.
  *              0 for short contexts (block_table of few keys): then NULL will do
  * out          shares no memory with q or the caches

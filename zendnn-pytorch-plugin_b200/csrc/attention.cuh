@@ -36,7 +36,7 @@ struct AttnParams {
   float scale_log2;                             // softmax scale times log2(e)
   int slices;                                   // streaming kernel: CTAs per sequence and kv head (0: all units are dealt out)
   int few;                                      // no sequence can have more than a few tiles of rows
-  int zero_tail;                                // rows behind the last sequence are zeroed
+  int zero_tail;                                // rows before the first sequence and behind the last are zeroed
   float *part_o;                                // [2 * grid][R][DP]
   float2 *part_ml;                              // [2 * grid][R]: maximum (log2 units), sum
   struct AttnMeta *meta;                        // [grid]
@@ -298,15 +298,15 @@ struct AttnWalk {
 // Row of the cache that holds a key: page id, slot in it.  An id outside the cache reads as no row and is reported.
 __device__ __forceinline__ int page_of(const AttnParams &p, int key) { return p.page_shift >= 0 ? key >> p.page_shift : key / p.page; }
 
-// Rows of `out` behind the last sequence, by all threads of the grid.
+// Rows of `out` before the first sequence and behind the last one, by all threads of the grid.
 template <typename T>
 __device__ __forceinline__ void zero_tail_rows(const AttnParams &p, int threads) {
   if (!p.zero_tail) return;
-  const int end = min(max(p.cu[p.batch], 0), p.tokens);
+  const int end = min(max(p.cu[p.batch], 0), p.tokens), begin = min(max(p.cu[0], 0), end);
   const int vecs = p.d / 8, per = p.hq * vecs;      // (rows are whole 16-byte vectors)
-  const int64_t n = (int64_t)(p.tokens - end) * per;
+  const int64_t n = (int64_t)(begin + p.tokens - end) * per;
   for (int64_t i = (int64_t)blockIdx.x * threads + threadIdx.x; i < n; i += (int64_t)gridDim.x * threads) {
-    const int64_t t = end + i / per;
+    const int64_t row = i / per, t = row < begin ? row : row - begin + end;
     const int c = (int)(i % per);
     *reinterpret_cast<uint4 *>(reinterpret_cast<T *>(p.out) + t * p.o_st + (c / vecs) * p.o_sh + c % vecs * 8) = make_uint4(0, 0, 0, 0);
   }
