@@ -396,7 +396,8 @@ ZT_API int zt_allreduce_bf16(const zt_allreduce_args_t *args, void *stream);
  * caches     NULL, or [num_pages, page_size, kv_heads, head_dim] with strides {page, slot, head}, of dtype or ZT_E4M3.  Token t's
  *            key and value go to row slots[t] = page * page_size + offset (int32, or int64 with slots_64).  A negative slot
  *            stores nothing (padding); one past the cache stores nothing and sets the device status word (106).  The slots of a
- *            call must differ from one another: of two tokens with one slot either may remain, element by element.
+ *            call must differ from one another: of two tokens with one slot either may remain, element by element.  The caches share
+ *            no memory with q, k, v or one another; one that is given as both (same strides) holds the values.
  * scales     ZT_E4M3 only: [kv_heads] fp32 each; what is stored is x / scale, rounded to nearest even and saturated */
 typedef struct {
   const void *q, *k, *v;

@@ -29,6 +29,7 @@ struct RopeParams {
   const float *inv_freq, *k_scale, *v_scale;
   int64_t capacity;   // slots of the cache
   int tokens, hq, hkv, d, rot, page, pos64, slot64, interleaved;
+  int one_cache;      // keys and values have the same rows: only values are stored
   uint32_t magic_token, magic_rot, magic_rest, magic_whole;   // divisions by the items of a token, the vectors of a head's parts
   int block_tokens;
   float factor;
@@ -215,7 +216,7 @@ __global__ void __launch_bounds__(kRopeThreads, E4M3 ? 4 : 5) rope_kernel(const 
     } else if constexpr (CACHE) {
       const bool value = i.head >= heads;
       const int64_t row = s_row[i.token][value];
-      if (s_row[i.token][0] >= 0) {
+      if (s_row[i.token][0] >= 0 && (value || !p.one_cache)) {
         const int h = i.head - (value ? heads : p.hq);
         const int64_t o = row + h * (value ? p.vc_sh : p.kc_sh);
         const float scale = E4M3 ? (value ? p.v_scale[h] : p.k_scale[h]) : 1.f;
@@ -302,6 +303,7 @@ extern "C" int zt_rope(const zt_rope_args_t *a, void *stream) {
   p.tokens = (int)a->tokens, p.hq = a->q_heads, p.hkv = a->kv_heads, p.d = a->head_dim, p.rot = a->rot_dim;
   p.page = cache ? a->page_size : 1, p.pos64 = a->positions_64, p.slot64 = a->slots_64, p.interleaved = a->interleaved != 0;
   p.factor = a->attention_factor, p.status = status;
+  p.one_cache = cache && a->k_cache == a->v_cache && std::equal(a->k_cache_stride, a->k_cache_stride + 3, a->v_cache_stride);
 
   // 16-byte vectors where every row and both parts of a head start on one; else element by element
   const int es = a->dtype == ZT_F32 ? 4 : 2, vec = 16 / es;

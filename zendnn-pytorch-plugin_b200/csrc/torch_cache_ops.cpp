@@ -45,10 +45,59 @@ void check_lengths(const at::Tensor &t, const at::Tensor &input, const char *op,
 void check_written(const at::Tensor &t, const char *op, const char *name) {
   TORCH_CHECK(at::has_internal_overlap(t) != at::MemOverlap::Yes, op, ": ", name, " is written and must not hold an element twice");
 }
+// The bytes of a tensor are its address plus sums of i * stride, 0 <= i < size.  Two tensors share one where their addresses differ by
+// such a sum over the strides of both, i down to 1 - size for the other's: `from` is what the dimensions from `d` on, the widest
+// first, have to add up to.  Strides of views are nested, which leaves one or two i each; `steps` bounds the search where they
+// are not (nothing is found then).
+struct Reach {
+  int64_t stride, lo, hi;           // i from lo to hi
+  int64_t rest_lo, rest_hi;         // what the dimensions behind this one add up to
+};
+using Reaches = c10::SmallVector<Reach, 12>;
+bool adds_up(const Reaches &dims, size_t d, int64_t from, int &steps) {
+  if (d == dims.size()) return from == 0;
+  const Reach &r = dims[d];
+  auto floor_div = [](int64_t x, int64_t y) { return x / y - (x % y < 0); };
+  const int64_t lo = std::max(r.lo, -floor_div(r.rest_hi - from, r.stride)), hi = std::min(r.hi, floor_div(from - r.rest_lo, r.stride));
+  for (int64_t i = lo; i <= hi && --steps >= 0; ++i)
+    if (adds_up(dims, d + 1, from - i * r.stride, steps)) return true;
+  return false;
+}
+int64_t bytes_spanned(const at::Tensor &t) {
+  const at::IntArrayRef sizes = t.sizes(), strides = t.strides();
+  int64_t last = 0;
+  for (size_t i = 0; i < sizes.size(); ++i) last += (sizes[i] - 1) * strides[i];
+  return (last + 1) * (int64_t)t.element_size();
+}
+bool share_memory(const at::Tensor &a, const at::Tensor &b) {
+  if (a.numel() == 0 || b.numel() == 0) return false;
+  const int64_t apart = (int64_t)(reinterpret_cast<uintptr_t>(b.data_ptr()) - reinterpret_cast<uintptr_t>(a.data_ptr()));
+  if (apart >= bytes_spanned(a) || -apart >= bytes_spanned(b)) return false;
+  Reaches dims;                     // one per stride, the widest first
+  auto dim = [&](int64_t stride, int64_t lo, int64_t hi) {
+    if (stride == 0 || lo == hi) return;
+    auto *at = std::find_if(dims.begin(), dims.end(), [&](const Reach &r) { return r.stride <= stride; });
+    if (at != dims.end() && at->stride == stride) at->lo += lo, at->hi += hi;
+    else dims.insert(at, Reach{stride, lo, hi, 0, 0});
+  };
+  for (const at::Tensor *t : {&a, &b}) {
+    const at::IntArrayRef sizes = t->sizes(), strides = t->strides();
+    const int64_t es = (int64_t)t->element_size(), sign = t == &a ? 1 : -1;
+    dim(1, std::min<int64_t>(sign * (es - 1), 0), std::max<int64_t>(sign * (es - 1), 0));
+    for (size_t i = 0; i < sizes.size(); ++i) {
+      const int64_t far = sign * (sizes[i] - 1);
+      dim(strides[i] * es, std::min<int64_t>(far, 0), std::max<int64_t>(far, 0));
+    }
+  }
+  for (size_t d = dims.size(); d-- > 1;) {
+    dims[d - 1].rest_lo = dims[d].rest_lo + dims[d].lo * dims[d].stride;
+    dims[d - 1].rest_hi = dims[d].rest_hi + dims[d].hi * dims[d].stride;
+  }
+  int steps = 1000;
+  return adds_up(dims, 0, apart, steps);
+}
 void check_apart(const at::Tensor &t, const at::Tensor &other, const char *op, const char *name, const char *other_name) {
-  const auto status = at::get_overlap_status(t, other);
-  TORCH_CHECK(status != at::MemOverlapStatus::Full && status != at::MemOverlapStatus::Partial, op, ": ", name,
-              " is written and must not share memory with ", other_name);
+  TORCH_CHECK(!share_memory(t, other), op, ": ", name, " is written and must not share memory with ", other_name);
 }
 
 // A pair of caches [pages, page_size, heads, head_dim] of one shape and type; for `input` of `head_dim`.
@@ -142,6 +191,11 @@ at::Tensor rope_cache(const at::Tensor &query, const at::Tensor &key, const at::
   check_caches(key_cache, value_cache, q, q.size(2), op);
   TORCH_CHECK(key_cache.size(2) == k.size(1), op, ": the caches have ", key_cache.size(2), " heads, the key ", k.size(1));
   check_written(key_cache, op, "key_cache"), check_written(value_cache, op, "value_cache");
+  if (key_cache.data_ptr() != value_cache.data_ptr() || key_cache.strides() != value_cache.strides())      // (one tensor as both holds the values)
+    check_apart(key_cache, value_cache, op, "key_cache", "value_cache");
+  for (const auto &[name, cache] : {std::pair<const char *, const at::Tensor &>("key_cache", key_cache), {"value_cache", value_cache}}) {
+    check_apart(cache, query, op, name, "query"), check_apart(cache, key, op, name, "key"), check_apart(cache, value, op, name, "value");
+  }
   a.k_scale = cache_scale(k_scale, key_cache, q, op, "k_scale");
   a.v_scale = cache_scale(v_scale, value_cache, q, op, "v_scale");
   c10::cuda::CUDAGuard device_guard(q.device());
