@@ -110,15 +110,16 @@ class PagedKVCache:
                  copy_pages: Optional[Callable] = None):
         if min(layers, pages, page_size, kv_heads, head_dim) < 1:
             raise ValueError("layers, pages, page_size, kv_heads and head_dim must be positive")
-        self.page_size, self.num_pages, self.device = int(page_size), int(pages), torch.device(device)
+        self.page_size, self.num_pages = int(page_size), int(pages)
         # keys and values of a page next to each other: a page is one block to copy
         self.layers = [torch.zeros((pages, 2, page_size, kv_heads, head_dim), dtype=torch.uint8 if dtype == torch.float8_e4m3fn else dtype,
                                    device=device) for _ in range(layers)]
+        self.device = self.layers[0].device      # with its index: the current device may change
         if dtype == torch.float8_e4m3fn:
             self.layers = [t.view(dtype) for t in self.layers]
-            ones = torch.ones(layers, kv_heads, dtype=torch.float32, device=device)
-            self.k_scale = ones if k_scale is None else k_scale.to(device=device, dtype=torch.float32).contiguous()
-            self.v_scale = ones if v_scale is None else v_scale.to(device=device, dtype=torch.float32).contiguous()
+            ones = torch.ones(layers, kv_heads, dtype=torch.float32, device=self.device)
+            self.k_scale = ones if k_scale is None else k_scale.to(device=self.device, dtype=torch.float32).contiguous()
+            self.v_scale = ones if v_scale is None else v_scale.to(device=self.device, dtype=torch.float32).contiguous()
             for name, t in (("k_scale", self.k_scale), ("v_scale", self.v_scale)):
                 if t.shape != (layers, kv_heads):
                     raise ValueError(f"{name} must have shape {(layers, kv_heads)}, got {tuple(t.shape)}")
