@@ -64,106 +64,299 @@ __global__ void __launch_bounds__(kCombineWarps * 32) attention_combine_kernel(c
     *reinterpret_cast<uint32_t *>(dst) = pack2(acc[0] * f, acc[1] * f, T(0.f));
 }
 
-// One element of a cache.
+// Four neighbouring elements of a cache.
 template <typename T, bool E4M3>
-__device__ __forceinline__ float cache_value(const void *base, int64_t at) {
+__device__ __forceinline__ float4 cache_values(const void *base, int64_t at) {
+  float2 lo, hi;
   if constexpr (E4M3) {
-    const uint2 h = e4m3x4_to_f16x4(reinterpret_cast<const uint8_t *>(base)[at]);
-    return unpack2(h.x, __half(0.f)).x;
+    const uint2 h = e4m3x4_to_f16x4(*reinterpret_cast<const uint32_t *>(reinterpret_cast<const uint8_t *>(base) + at));
+    lo = unpack2(h.x, __half(0.f)), hi = unpack2(h.y, __half(0.f));
   } else {
-    return (float)reinterpret_cast<const T *>(base)[at];
+    const uint2 w = *reinterpret_cast<const uint2 *>(reinterpret_cast<const T *>(base) + at);
+    lo = unpack2(w.x, T(0.f)), hi = unpack2(w.y, T(0.f));
   }
+  return make_float4(lo.x, lo.y, hi.x, hi.y);
+}
+template <typename T, bool E4M3>
+__device__ __forceinline__ uint32_t not_finite_bits(uint32_t w) {
+  if constexpr (E4M3) return not_finite_mask_e4m3(w);
+  else return not_finite_mask(w, T(0.f));
 }
 
-// Goes through a row of the output again, by one warp, where it is not finite: unless its query or a key that it sees holds a NaN, or
-// the values that it sees account for every such column, the row is computed from those keys alone.  A NaN is accounted for by
-// a NaN or by infinities of both signs, an infinity by one of its sign: 0 times the value of a key that the row does not see makes a NaN
-// of an infinity that it does see.
-template <typename T, bool E4M3>
-__device__ __noinline__ void redo_row(const AttnParams &p, int b, const SeqInfo &seq, int head, int r) {
-  constexpr int V = 4;                                   // columns of a lane
-  const int lane = threadIdx.x & 31, tok = r / p.group, qh = head * p.group + r % p.group;
-  const int lo = key_lo(p, seq, tok), hi = key_hi(p, seq, tok);
-  T *out = reinterpret_cast<T *>(p.out) + (seq.q0 + tok) * p.o_st + qh * p.o_sh;
-  const T *q = reinterpret_cast<const T *>(p.q) + (seq.q0 + tok) * p.q_st + qh * p.q_sh;
-  auto row_of = [&](int key, int64_t sp, int64_t ss, int64_t sh) -> int64_t {      // -1: no such page
-    const int id = p.table[b * p.table_stride + page_of(p, key)];
-    return id >= 0 && id < p.num_pages ? id * sp + (key - page_of(p, key) * p.page) * ss + head * sh : -1;
-  };
-  uint32_t nans = 0, infs[2] = {0, 0};                   // this lane's columns that are NaN, infinite (positive, negative)
-  uint32_t seen_nan = 0, seen_inf[2] = {0, 0};           // columns with such a value among the keys that the row sees
-  auto note = [](float x, int e, uint32_t &is_nan, uint32_t (&is_inf)[2]) {
-    if (isnan(x)) is_nan |= 1u << e;
-    else if (isinf(x)) is_inf[x < 0.f] |= 1u << e;
-  };
-  auto open = [&]() {                                    // columns that want an explanation
-    return (nans & ~(seen_nan | (seen_inf[0] & seen_inf[1]))) | (infs[0] & ~seen_inf[0]) | (infs[1] & ~seen_inf[1]);
-  };
-#pragma unroll
-  for (int e = 0; e < V; ++e)
-    if (lane * V + e < p.d) note((float)out[lane * V + e], e, nans, infs);
-  if (!__any_sync(0xffffffffu, open() != 0)) return;
-  bool nan = false;
-#pragma unroll
-  for (int e = 0; e < V; ++e)
-    if (lane * V + e < p.d) nan |= isnan((float)q[lane * V + e]);
-  if (hi > lo && __any_sync(0xffffffffu, nan)) return;
-  for (int key = hi - 1; key >= lo && __any_sync(0xffffffffu, open() != 0); --key) {
-    const int64_t at = row_of(key, p.v_sp, p.v_ss, p.v_sh), k_at = row_of(key, p.k_sp, p.k_ss, p.k_sh);
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      if (at < 0 || lane * V + e >= p.d) continue;
-      note(cache_value<T, E4M3>(p.v, at + lane * V + e), e, seen_nan, seen_inf);
-      nan |= isnan(cache_value<T, E4M3>(p.k, k_at + lane * V + e));
-    }
-    if (__any_sync(0xffffffffu, nan)) return;
+constexpr int kRedoWords = 16;     // flags of a block that goes through rows again
+
+// Which of some columns hold NaN or an infinity (positive, negative), a bit per column.
+struct Special {
+  uint32_t nan, inf[2];
+  __device__ __forceinline__ void note(float x, int e) {
+    if (isnan(x)) nan |= 1u << e;
+    else if (isinf(x)) inf[x < 0.f] |= 1u << e;
   }
-  if (!__any_sync(0xffffffffu, open() != 0)) return;
-  const float mul = p.scale_log2 * (E4M3 ? p.k_scale[head] : 1.f);
-  float acc[V] = {}, special[V] = {}, top = -INFINITY, sum = 0.f;      // special: values that are not finite, which no factor may touch
-  for (int first = lo; first < hi; first += 32) {        // a key per lane, then its value by all lanes
-    const int key = first + lane;
-    float s = -INFINITY;
-    if (key < hi) {
-      const int64_t at = row_of(key, p.k_sp, p.k_ss, p.k_sh);
-      s = 0.f;
-      if (at >= 0)
-        for (int e = 0; e < p.d; ++e) s = fmaf((float)q[e], cache_value<T, E4M3>(p.k, at + e), s);
-      s *= mul;
-    }
-    float to = s;
+  __device__ __forceinline__ void note(float4 x) { note(x.x, 0), note(x.y, 1), note(x.z, 2), note(x.w, 3); }
+  // Columns of an output that the values `seen` do not account for: a NaN comes of a NaN or of infinities of both signs, an infinity of
+  // one of its sign.
+  __device__ __forceinline__ uint32_t open(const Special &seen) const {
+    return (nan & ~(seen.nan | (seen.inf[0] & seen.inf[1]))) | (inf[0] & ~seen.inf[0]) | (inf[1] & ~seen.inf[1]);
+  }
+};
+
+// Goes through up to 32 neighbouring rows of an item again, by the whole block: of those whose output is not finite, unless the
+// query or a key that the row sees holds a NaN, or the values that it sees account for every such column, a row is computed from
+// the keys that it sees alone.  (0 times the value of a key that a row does not see is NaN where that is not finite, and makes a
+// NaN of an infinity that the row does see.)
+//
+// The keys that all of the rows see are gone through once, by all threads; those at either end, which differ by as many tokens as there
+// are rows, by a warp per row; sums are taken again four rows at a time.  With NaN among the values that most rows see, a prompt of 2048
+// tokens (32 heads over 8 of 128) takes 0.5 ms instead of 0.06.  Rows that are computed again are at most a tile of rows per kv head and
+// value: with NaN in the last value of 8000, which 252 rows of a chunk's last tile do not see, 8 ms instead of 0.08.  (One key after
+// another in every row: 38 and 114 ms.)
+template <typename T, bool E4M3, int DP>
+__device__ __noinline__ void redo_rows(const AttnParams &p, int b, const SeqInfo &seq, int head, int r0, int n) {
+  constexpr int NT = DP * 2, WARPS = NT / 32, PER = E4M3 ? 16 : 8, CH = DP / PER, STEP = NT / CH, AHEAD = 4;
+  // flags of this block: a word per 32 columns for NaN and infinities of either sign, and whether a key holds a NaN
+  // (behind the pieces in the workspace)
+  uint32_t *flags = reinterpret_cast<uint32_t *>(p.part_o + (int64_t)2 * gridDim.x * kTcgen05Rows * DP) + (blockIdx.x * gridDim.y + blockIdx.y) * kRedoWords;
+  uint32_t *key_nan = flags + kRedoWords - 1;
+  auto seen_by_all = [&](int kind, int col) { return __ldcg(flags + 4 * kind + col / 32) >> col % 32; };
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c4 = lane * 4;      // (of a row, a lane has four columns)
+  auto slot_of = [&](int key, int64_t &k_at, int64_t &v_at) -> bool {             // false: no such page (zeros)
+    const int page = page_of(p, key), id = p.table[b * p.table_stride + page], slot = key - page * p.page;
+    k_at = id * p.k_sp + slot * p.k_ss + head * p.k_sh, v_at = id * p.v_sp + slot * p.v_ss + head * p.v_sh;
+    return id >= 0 && id < p.num_pages;
+  };
+  auto out_row = [&](int r) { return reinterpret_cast<T *>(p.out) + (seq.q0 + r / p.group) * p.o_st + (head * p.group + r % p.group) * p.o_sh; };
+  auto query_row = [&](int r) { return reinterpret_cast<const T *>(p.q) + (seq.q0 + r / p.group) * p.q_st + (head * p.group + r % p.group) * p.q_sh; };
+  auto has_nan = [](float4 x) { return isnan(x.x) || isnan(x.y) || isnan(x.z) || isnan(x.w); };
+  auto special_outputs = [&](int r) {
+    Special x{0, {0, 0}};
+    if (c4 < p.d) x.note(cache_values<T, false>(out_row(r), c4));
+    return x;
+  };
+
+  __syncthreads();            // the flags of an earlier call have been read
+  if (threadIdx.x < kRedoWords) flags[threadIdx.x] = 0;
+  bool any = false;
+  for (int i = warp; i < n; i += WARPS) any |= special_outputs(r0 + i).open({0, {0, 0}}) != 0;
+  if (!__syncthreads_or(any)) return;
+
+  // ---- the keys that all rows see ----
+  int all_lo = key_lo(p, seq, (r0 + n - 1) / p.group), all_hi = key_hi(p, seq, r0 / p.group);
+  {
+    const int c = threadIdx.x % CH * PER, sub = threadIdx.x / CH;
+    for (int first = all_lo, round = 1; first < all_hi; first += AHEAD * STEP, ++round) {
+      uint4 k[AHEAD], v[AHEAD];
 #pragma unroll
-    for (int o = 16; o; o >>= 1) to = fmaxf(to, __shfl_xor_sync(0xffffffffu, to, o));
-    to = fmaxf(to, top);
-    const float f = top == -INFINITY ? 0.f : exp2_fast(top - to), x = key < hi ? exp2_fast(s - (to == -INFINITY ? 0.f : to)) : 0.f;
-    top = to;
-    sum = sum * f + x;
+      for (int u = 0; u < AHEAD; ++u) {
+        const int key = first + u * STEP + sub;
+        int64_t k_at, v_at;
+        k[u] = v[u] = make_uint4(0, 0, 0, 0);
+        if (key < all_hi && c < p.d && slot_of(key, k_at, v_at)) {
+          constexpr int ES = E4M3 ? 1 : 2;
+          k[u] = *reinterpret_cast<const uint4 *>(reinterpret_cast<const char *>(p.k) + (k_at + c) * ES);
+          v[u] = *reinterpret_cast<const uint4 *>(reinterpret_cast<const char *>(p.v) + (v_at + c) * ES);
+        }
+      }
 #pragma unroll
-    for (int e = 0; e < V; ++e) acc[e] *= f;
-    for (int i = 0; i < min(32, hi - first); ++i) {
-      const float xi = __shfl_sync(0xffffffffu, x, i);
-      const int64_t at = row_of(first + i, p.v_sp, p.v_ss, p.v_sh);
+      for (int u = 0; u < AHEAD; ++u) {
+        const uint32_t kw[4] = {k[u].x, k[u].y, k[u].z, k[u].w}, vw[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        if (at < 0 || lane * V + e >= p.d) continue;
-        const float v = cache_value<T, E4M3>(p.v, at + lane * V + e);
-        if (isfinite(v)) acc[e] = fmaf(xi, v, acc[e]);
-        else special[e] += v;
+        for (int e = 0; e < 4; ++e) {
+          if (not_finite_bits<T, E4M3>(kw[e])) {
+            bool nan = true;
+            if constexpr (!E4M3) {
+              const float2 x = unpack2(kw[e], T(0.f));
+              nan = isnan(x.x) || isnan(x.y);
+            }
+            if (nan) *key_nan = 1;
+          }
+          if (const uint32_t bad = not_finite_bits<T, E4M3>(vw[e])) {
+            Special x{0, {0, 0}};
+            int at = c + e * (PER / 4);
+            if constexpr (E4M3) {
+              x.nan = (bad & 1) | (bad >> 7 & 2) | (bad >> 14 & 4) | (bad >> 21 & 8);
+            } else {
+              const float2 f = unpack2(vw[e], T(0.f));
+              x.note(f.x, 0), x.note(f.y, 1);
+            }
+            const uint32_t bits[3] = {x.nan, x.inf[0], x.inf[1]};
+#pragma unroll
+            for (int kind = 0; kind < 3; ++kind)
+              if (bits[kind]) atomicOr(flags + 4 * kind + at / 32, bits[kind] << at % 32);
+          }
+        }
+      }
+      if (round % 16 == 0) {      // a key of NaN, or values of NaN in all columns: nothing else matters
+        bool done = false;
+        if (threadIdx.x == 0) {
+          done = true;
+          for (int col = 0; col < p.d; col += 8) done &= (seen_by_all(0, col) & 0xffu) == 0xffu;
+          done |= __ldcg(key_nan) != 0;
+        }
+        if (__syncthreads_or(done)) return;
       }
     }
   }
+  __syncthreads();
+  if (__ldcg(key_nan)) return;
+
+  // ---- the keys that not all of them see, a row per warp: which rows need their sums again ----
+  constexpr int ROWS = 32 / WARPS, G = 4;                // a warp's rows, neighbours; of those, at once
+  uint32_t todo = 0, mine[ROWS];                         // mine: NaN, infinities among the values that a row sees, in this lane's columns
+#pragma unroll 1
+  for (int i = 0; i < ROWS; ++i) {
+    mine[i] = 0;
+    if (warp * ROWS + i >= n) continue;
+    const int r = r0 + warp * ROWS + i, tok = r / p.group, lo = key_lo(p, seq, tok), hi = key_hi(p, seq, tok);
+    const Special out = special_outputs(r);
+    Special seen{0, {0, 0}};
+    if (c4 < p.d) seen = {seen_by_all(0, c4) & 15, {seen_by_all(1, c4) & 15, seen_by_all(2, c4) & 15}};
+    if (!__any_sync(0xffffffffu, out.open(seen) != 0)) continue;
+    bool nan = false;
+    if (c4 < p.d && hi > lo) nan = has_nan(cache_values<T, false>(query_row(r), c4));
+    const bool some = all_hi > all_lo;
+    const int before = max((some ? all_lo : hi) - lo, 0), after = some ? max(hi - all_hi, 0) : 0;
+    for (int j0 = 0; j0 < before + after; j0 += 32) {
+      const int j = j0 + lane;
+      int64_t k_at = 0, v_at = 0;
+      const bool live = j < before + after && slot_of(j < before ? lo + j : all_hi + (j - before), k_at, v_at);
+      const uint32_t lives = __ballot_sync(0xffffffffu, live);
+#pragma unroll 4
+      for (int u = 0; u < 32; ++u) {
+        const int64_t ka = __shfl_sync(0xffffffffu, k_at, u), va = __shfl_sync(0xffffffffu, v_at, u);
+        if (!(lives >> u & 1) || c4 >= p.d) continue;
+        seen.note(cache_values<T, E4M3>(p.v, va + c4));
+        nan |= has_nan(cache_values<T, E4M3>(p.k, ka + c4));
+      }
+    }
+    mine[i] = seen.nan | seen.inf[0] << 4 | seen.inf[1] << 8;
+    if (!__any_sync(0xffffffffu, nan) && __any_sync(0xffffffffu, out.open(seen) != 0)) todo |= 1u << i;
+  }
+
+  // ---- their sums, four rows at a time over the finite values ----
+  const float mul = p.scale_log2 * (E4M3 ? p.k_scale[head] : 1.f), v_scale = E4M3 ? p.v_scale[head] : 1.f;
+  const int c = lane % CH * PER, sub = lane / CH;        // of a key's row: this lane's elements; key of a load
+#pragma unroll 1
+  for (int g = 0; g < ROWS; g += G) {
+    if (!(todo >> g & 15)) continue;
+    uint4 q[G][PER / 8];
+    int lo[G], hi[G], first = 1 << 30, last = 0;
+    float acc[G][4] = {}, top[G], sum[G];
 #pragma unroll
-  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  const float f = sum == 0.f ? 0.f : (E4M3 ? p.v_scale[head] : 1.f) / sum;
+    for (int i = 0; i < G; ++i) {
+      const bool does = todo >> (g + i) & 1;
+      const int r = r0 + warp * ROWS + g + (does ? i : __ffs(todo >> g & 15) - 1), tok = r / p.group;
+      lo[i] = does ? key_lo(p, seq, tok) : 0, hi[i] = does ? key_hi(p, seq, tok) : 0;
+      if (hi[i] > lo[i]) first = min(first, lo[i]), last = max(last, hi[i]);
+      top[i] = -INFINITY, sum[i] = 0.f;
 #pragma unroll
-  for (int e = 0; e < V; ++e)
-    if (lane * V + e < p.d) out[lane * V + e] = (T)(acc[e] * f + special[e]);
+      for (int h = 0; h < PER / 8; ++h)
+        q[i][h] = c + 8 * h < p.d ? *reinterpret_cast<const uint4 *>(query_row(r) + c + 8 * h) : make_uint4(0, 0, 0, 0);
+    }
+    for (; first < last; first += 32) {                  // a key per lane, then its value by all lanes
+      int64_t k_at = 0, v_at = 0;
+      const bool live = first + lane < last && slot_of(first + lane, k_at, v_at);
+      const uint32_t lives = __ballot_sync(0xffffffffu, live);
+      float x[G] = {};
+#pragma unroll 4
+      for (int u = 0; u < CH; ++u) {                     // 32 / CH keys at once
+        const int from = u * (32 / CH) + sub;
+        const int64_t at = __shfl_sync(0xffffffffu, k_at, from);
+        uint4 k = make_uint4(0, 0, 0, 0);
+        if ((lives >> from & 1) && c < p.d) k = *reinterpret_cast<const uint4 *>(reinterpret_cast<const char *>(p.k) + (at + c) * (E4M3 ? 1 : 2));
+        const uint32_t kw[4] = {k.x, k.y, k.z, k.w};
+        float2 kf[PER / 2];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if constexpr (E4M3) {
+            const uint2 h = e4m3x4_to_f16x4(kw[e]);
+            kf[2 * e] = unpack2(h.x, __half(0.f)), kf[2 * e + 1] = unpack2(h.y, __half(0.f));
+          } else {
+            kf[e] = unpack2(kw[e], T(0.f));
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < G; ++i) {
+          float2 part = make_float2(0.f, 0.f);
+#pragma unroll
+          for (int e = 0; e < PER / 2; ++e) {
+            const uint4 &w = q[i][e / 4];
+            const float2 f = unpack2(e % 4 == 0 ? w.x : e % 4 == 1 ? w.y : e % 4 == 2 ? w.z : w.w, T(0.f));
+            part.x = fmaf(f.x, kf[e].x, part.x), part.y = fmaf(f.y, kf[e].y, part.y);
+          }
+          float s = part.x + part.y;
+#pragma unroll
+          for (int m = 1; m < CH; m *= 2) s += __shfl_xor_sync(0xffffffffu, s, m);
+          s = __shfl_sync(0xffffffffu, s, lane % (32 / CH) * CH);
+          if (lane / (32 / CH) == u) x[i] = s;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < G; ++i) {
+        const bool sees = first + lane >= lo[i] && first + lane < hi[i];
+        const float s = sees ? x[i] * mul : -INFINITY;
+        float to = s;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) to = fmaxf(to, __shfl_xor_sync(0xffffffffu, to, o));
+        to = fmaxf(to, top[i]);
+        const float f = top[i] == -INFINITY ? 0.f : exp2_fast(top[i] - to);
+        x[i] = sees ? exp2_fast(s - (to == -INFINITY ? 0.f : to)) : 0.f;
+        top[i] = to, sum[i] = sum[i] * f + x[i];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][e] *= f;
+      }
+#pragma unroll 8
+      for (int u = 0; u < 32; ++u) {
+        const int64_t va = __shfl_sync(0xffffffffu, v_at, u);
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if ((lives >> u & 1) && c4 < p.d) v = cache_values<T, E4M3>(p.v, va + c4);
+        v.x = isfinite(v.x) ? v.x : 0.f, v.y = isfinite(v.y) ? v.y : 0.f, v.z = isfinite(v.z) ? v.z : 0.f, v.w = isfinite(v.w) ? v.w : 0.f;
+#pragma unroll
+        for (int i = 0; i < G; ++i) {
+          const float xi = __shfl_sync(0xffffffffu, x[i], u);
+          acc[i][0] = fmaf(xi, v.x, acc[i][0]), acc[i][1] = fmaf(xi, v.y, acc[i][1]);
+          acc[i][2] = fmaf(xi, v.z, acc[i][2]), acc[i][3] = fmaf(xi, v.w, acc[i][3]);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+#pragma unroll
+      for (int o = 16; o; o >>= 1) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], o);
+      if (!(todo >> (g + i) & 1) || c4 >= p.d) continue;
+      const float f = sum[i] == 0.f ? 0.f : v_scale / sum[i];
+      float y[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        y[e] = acc[i][e] * f;
+        if (mine[g + i] >> (4 + e) & 1) y[e] += INFINITY;
+        if (mine[g + i] >> (8 + e) & 1) y[e] -= INFINITY;
+        if (mine[g + i] >> e & 1) y[e] = NAN;
+      }
+      *reinterpret_cast<uint2 *>(out_row(r0 + warp * ROWS + g + i) + c4) = make_uint2(pack2(y[0], y[1], T(0.f)), pack2(y[2], y[3], T(0.f)));
+    }
+  }
+}
+
+// The rows of block (x, y) of the joining kernel: the y-th 32 of the item that is cut at the end of CTA x's range and, where that CTA
+// found outputs that are not finite, of its whole items.  (A function of its own, held to 64 registers: with
+// more, calls without such outputs take 2 - 7 % longer; as a third kernel, 4 us.)
+template <typename T, bool E4M3, int DP>
+__device__ __noinline__ void redo_items(const AttnParams &p) {
+  const AttnMeta &meta = p.meta[blockIdx.x];
+  const int4 item = meta.cut;
+  const int r32 = blockIdx.y * 32;
+  if (item.x >= 0 && item.z % 512 > r32)
+    redo_rows<T, E4M3, DP>(p, meta.cut_b, load_seq(p, meta.cut_b), item.z / 512, item.y + r32, min(item.z % 512 - r32, 32));
+  if (!meta.not_finite) return;
+  AttnWalk<kTcgen05Rows, kTcgen05Unit, kTcgen05Extra> it(meta.range);
+  while (it.next(p))              // (the block of the first CTA of an item that was cut has it)
+    if (it.whole && it.n_rows > r32) redo_rows<T, E4M3, DP>(p, it.b, it.seq, it.head, it.r0 + r32, min(it.n_rows - r32, 32));
 }
 
 // The same for the pieces of the tcgen05 kernel, whose rows are neighbours in the workspace: a lane per row, a warp per 16 columns.
 // A block whose CTA found outputs that are not finite goes through the rows of its items again.
 template <typename T, bool E4M3, int DP>
-__global__ void __launch_bounds__(DP * 2) attention_combine_rows_kernel(const __grid_constant__ AttnParams p, int R) {
+__global__ void __launch_bounds__(DP * 2, 512 / DP) attention_combine_rows_kernel(const __grid_constant__ AttnParams p, int R) {
   grid_launch_dependents();
   grid_dependency_wait();
   const AttnMeta &meta = p.meta[blockIdx.x];
@@ -205,19 +398,7 @@ __global__ void __launch_bounds__(DP * 2) attention_combine_rows_kernel(const __
     redo |= __any_sync(0xffffffffu, others) != 0;
   }
   if (!redo) return;
-  __syncthreads();        // this block's part of the cut item is written
-  if (item.x >= 0) {
-    const SeqInfo seq = load_seq(p, meta.cut_b);
-    for (int i = warp; i < 32; i += DP * 2 / 32)
-      if (blockIdx.y * 32 + i < item.z % 512) redo_row<T, E4M3>(p, meta.cut_b, seq, item.z / 512, item.y + blockIdx.y * 32 + i);
-  }
-  if (!meta.not_finite) return;
-  AttnWalk<kTcgen05Rows, kTcgen05Unit, kTcgen05Extra> it(meta.range);
-  while (it.next(p)) {
-    if (!it.whole) continue;      // (the block of the item's first CTA has it)
-    for (int i = warp; i < 32; i += DP * 2 / 32)
-      if (blockIdx.y * 32 + i < it.n_rows) redo_row<T, E4M3>(p, it.b, it.seq, it.head, it.r0 + blockIdx.y * 32 + i);
-  }
+  redo_items<T, E4M3, DP>(p);
 }
 
 template <typename T, bool E4M3>
@@ -271,6 +452,7 @@ AttnPlan make_plan(const zt_paged_attention_args_t &a) {
   plan.meta_bytes = align256((size_t)plan.grid * sizeof(AttnMeta));
   plan.ml_bytes = align256((size_t)2 * plan.grid * plan.rows * sizeof(float2));
   plan.o_bytes = align256((size_t)2 * plan.grid * plan.rows * plan.dp * sizeof(float));
+  if (plan.tcgen05) plan.flag_bytes = align256((size_t)plan.grid * (plan.rows / 32) * kRedoWords * sizeof(uint32_t));
   return plan;
 }
 

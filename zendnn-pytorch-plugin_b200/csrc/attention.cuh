@@ -62,8 +62,8 @@ struct AttnPlan {         // of one call, on the host
   int rows, dp, grid;     // rows per item, padded head, CTAs
   int slices;             // see AttnParams
   double most_units;
-  size_t meta_bytes, ml_bytes, o_bytes;
-  size_t total() const { return meta_bytes + ml_bytes + o_bytes; }
+  size_t meta_bytes, ml_bytes, o_bytes, flag_bytes;
+  size_t total() const { return meta_bytes + ml_bytes + o_bytes + flag_bytes; }
 };
 
 int attention_stream_launch(const AttnParams &p, const AttnPlan &plan, int dtype, int cache_dtype, cudaStream_t st);
