@@ -91,6 +91,7 @@ struct Barriers {
   uint64_t kv_full[8], kv_free[8];
   uint64_t q_full[2], s_full[2], p_half[2], p_full[2], o_full[2];
   uint64_t piece_full[4], piece_free[4];
+  uint64_t drain;                // after a wait that gave up: the products that were issued
   uint32_t not_finite;           // some output that may be another row's doing
   uint32_t tmem;
 };
@@ -137,6 +138,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tcgen05_kernel(const __
       tc::mbar_init(&bars.s_full[i], 1), tc::mbar_init(&bars.o_full[i], 1);
     }
     for (int i = 0; i < kPieces; ++i) tc::mbar_init(&bars.piece_full[i], 1), tc::mbar_init(&bars.piece_free[i], kPieceReaders);
+    tc::mbar_init(&bars.drain, 1);
     bars.not_finite = 0;
     tc::mbar_fence_init();
   }
@@ -536,6 +538,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tcgen05_kernel(const __
     }
     if (ok) finish_all();
     asm volatile("cp.async.wait_group 0;" ::: "memory");      // (none is left in flight by a wait that gave up)
+    if (!ok)                // nor a box: each has a microsecond or so to arrive, a stage that others left incomplete its polls
+      for (uint32_t k = n + 1 > S ? n + 1 - S : 0; k <= n; ++k) tc::mbar_wait(&bars.kv_full[k % S], (k / S) & 1, 1u << 10);
     if (!ok && lane == 0) tc::report_timeout(p.status, kStatusProducerTimeout);
   } else {
     // ---- MMAs -----------------------------------------------------------------------------------------------------
@@ -619,7 +623,12 @@ __global__ void __launch_bounds__(kThreads, 1) attention_tcgen05_kernel(const __
       }
       // the last arrival that the tensor core owes this CTA
       if (ok && n > 0) ok = tc::warp_wait(smem_u32(&bars.kv_free[(n - 1) % S]), ((n - 1) / S) & 1);
-      if (!ok && lane == 0) tc::report_timeout(p.status, kStatusMmaTimeout);
+      if (!ok) {              // tensor memory goes back when the products that were issued are done
+        if (leader) tc::mma_commit(&bars.drain);
+        __syncwarp();
+        tc::warp_wait(smem_u32(&bars.drain), 0);
+        if (lane == 0) tc::report_timeout(p.status, kStatusMmaTimeout);
+      }
     } else if (warp == 13) {
       // ---- the walk -----------------------------------------------------------------------------------------------
       Walk it(range);
