@@ -1,0 +1,26 @@
+"""Arguments of the paged cache and its operators that are refused before anything changes: no GPU needed."""
+import pytest
+import torch
+
+from _cache_ref import plain_copy_pages
+
+
+def make_cache(**kw):
+    from zentorch_b200.cache import PagedKVCache
+    return PagedKVCache(**{**dict(layers=1, pages=6, page_size=4, kv_heads=1, head_dim=8, device="cpu", copy_pages=plain_copy_pages,
+                                  dtype=torch.float32), **kw})
+
+
+@pytest.mark.parametrize("count", [1.5, "1", None])
+def test_a_step_takes_whole_numbers_of_tokens(zt, count):
+    """... and a batch with another one leaves every sequence as it was."""
+    cache = make_cache()
+    cache.add("a")
+    cache.add("b")
+    cache.step([("a", 3)])
+    with pytest.raises(TypeError):
+        cache.step([("a", 2), ("b", count)])
+    with pytest.raises(TypeError):
+        cache.truncate("a", 1.5)
+    assert cache.length("a") == 3 and cache.pages("a") == (0,) and cache.length("b") == 0 and cache.free_pages == 5
+    assert cache.step([("a", torch.tensor(2).item()), ("b", torch.tensor(1))]).cu_seqlens_q.tolist() == [0, 2, 3]

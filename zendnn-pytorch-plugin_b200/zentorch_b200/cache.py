@@ -16,6 +16,7 @@ copied by ``torch.ops.zentorch.zentorch_cache_copy_pages`` on the current stream
 from __future__ import annotations
 
 import math
+import operator
 from dataclasses import dataclass
 from typing import Callable, Dict, Hashable, List, Optional, Sequence, Tuple
 
@@ -177,7 +178,7 @@ class PagedKVCache:
 
     def truncate(self, name, length: int) -> None:
         """Takes back the tokens from ``length`` on (rejected drafts, an edited prompt)."""
-        s = self._get(name)
+        s, length = self._get(name), operator.index(length)
         if not 0 <= length <= s.length:
             raise ValueError(f"cannot cut a sequence of {s.length} tokens to {length}")
         keep = -(-length // self.page_size)
@@ -194,6 +195,7 @@ class PagedKVCache:
     def step(self, new: Sequence[Tuple[Hashable, int]]) -> CacheStep:
         """Room for ``new`` tokens [(sequence, count), ...] and the tensors of the step.  A last page that others share is copied
         first (on the current stream).  Raises MemoryError, with nothing changed, when the free pages do not suffice."""
+        new = [(name, operator.index(count)) for name, count in new]
         names = [n for n, _ in new]
         if len(set(names)) != len(names):
             raise ValueError("a sequence may appear once in a step")
