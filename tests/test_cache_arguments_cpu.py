@@ -24,3 +24,26 @@ def test_a_step_takes_whole_numbers_of_tokens(zt, count):
         cache.truncate("a", 1.5)
     assert cache.length("a") == 3 and cache.pages("a") == (0,) and cache.length("b") == 0 and cache.free_pages == 5
     assert cache.step([("a", torch.tensor(2).item()), ("b", torch.tensor(1))]).cu_seqlens_q.tolist() == [0, 2, 3]
+
+
+def test_a_copy_that_fails_leaves_the_cache_as_it_was(zt):
+    def fails(caches, src, dst):
+        raise RuntimeError("no copy")
+    cache = make_cache(copy_pages=fails)
+    cache.add("a")
+    cache.step([("a", 6)])
+    cache.fork("a", "b")
+    with pytest.raises(RuntimeError, match="no copy"):
+        cache.step([("a", 4), ("b", 1)])
+    assert cache.pages("a") == cache.pages("b") == (0, 1) and cache.length("a") == cache.length("b") == 6 and cache.free_pages == 4
+    cache.free("b")
+    assert cache.free_pages == 4
+    cache.free("a")
+    assert cache.free_pages == 6
+    for name in "abc":
+        cache.add(name)
+        cache.step([(name, 4)])
+    cache.free("a")
+    with pytest.raises(RuntimeError, match="no copy"):
+        cache.compact()
+    assert cache.pages("b") == (1,) and cache.pages("c") == (2,) and cache.free_pages == 4

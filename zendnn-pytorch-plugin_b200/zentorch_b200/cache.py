@@ -216,15 +216,18 @@ class PagedKVCache:
             plan.append((s, count, fresh, split))
         if need > len(self._free):
             raise MemoryError(f"the step needs {need} pages, {len(self._free)} are free")
-        src, dst = [], []
+        src, dst, taken = [], [], 0
+        for s, _, fresh, split in plan:
+            if split:
+                src.append(s.pages[-1])
+                dst.append(self._free[-1 - taken])
+            taken += split + fresh
+        self._copy_pages(src, dst)                     # (where it raises, nothing has changed)
         positions, slots, starts, lens = [], [], [0], []
         for s, count, fresh, split in plan:
             if split:
-                old, page = s.pages[-1], self._take()
-                src.append(old)
-                dst.append(page)
-                self._owners[old] -= 1
-                s.pages[-1] = page
+                self._owners[s.pages[-1]] -= 1
+                s.pages[-1] = self._take()
             s.pages.extend(self._take() for _ in range(fresh))
             t, end = s.length, s.length + count
             positions.extend(range(t, end))
@@ -236,7 +239,6 @@ class PagedKVCache:
             s.length = end
             starts.append(starts[-1] + count)
             lens.append(s.length)
-        self._copy_pages(src, dst)
         width = max((len(s.pages) for s, *_ in plan), default=0)
         table = [s.pages + [0] * (width - len(s.pages)) for s, *_ in plan]
         return CacheStep(self._tensor(positions, torch.int64), self._tensor(slots, torch.int64), self._tensor(starts, torch.int32),
