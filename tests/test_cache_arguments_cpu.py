@@ -1,4 +1,6 @@
 """Arguments of the paged cache and its operators that are refused before anything changes: no GPU needed."""
+import ctypes as C
+
 import pytest
 import torch
 
@@ -47,3 +49,13 @@ def test_a_copy_that_fails_leaves_the_cache_as_it_was(zt):
     with pytest.raises(RuntimeError, match="no copy"):
         cache.compact()
     assert cache.pages("b") == (1,) and cache.pages("c") == (2,) and cache.free_pages == 4
+
+
+def test_a_softmax_scale_whose_base_two_form_is_infinite(zt):
+    from zentorch_b200 import _capi
+    lib, p = _capi.lib(), _capi.PagedAttentionArgs()
+    p.tokens, p.batch, p.q_heads, p.kv_heads, p.head_dim, p.dtype, p.cache_dtype = 4, 2, 8, 4, 64, _capi.ZT_BF16, _capi.ZT_BF16
+    p.page_size, p.max_blocks, p.num_pages = 16, 4, 8
+    for scale, text in ((3e38, b"positive and finite"), (2e38, b"null tensor pointer")):
+        p.scale = scale
+        assert lib.zt_paged_attention(C.byref(p), None) == 1 and text in lib.zt_last_error()

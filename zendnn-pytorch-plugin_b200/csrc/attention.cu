@@ -491,7 +491,7 @@ extern "C" int zt_paged_attention(const zt_paged_attention_args_t *a, void *stre
   ZT_REQUIRE((int64_t)a->page_size * a->max_blocks <= (1 << 30), ZT_UNSUPPORTED,
              "zt_paged_attention: block_table holds more than 2^30 keys per sequence");
   ZT_REQUIRE(a->window >= 0, ZT_INVALID_ARGUMENT, "zt_paged_attention: the window must not be negative");
-  ZT_REQUIRE(std::isfinite(a->scale) && a->scale > 0.f, ZT_INVALID_ARGUMENT, "zt_paged_attention: the scale must be positive and finite");
+  ZT_REQUIRE(std::isfinite(a->scale * 1.4426950408889634f) && a->scale > 0.f, ZT_INVALID_ARGUMENT, "zt_paged_attention: the scale must be positive and finite");
   ZT_REQUIRE(!e4m3 || (a->k_scale && a->v_scale), ZT_INVALID_ARGUMENT,
              "zt_paged_attention: a float8_e4m3 cache needs k_scale and v_scale");
   const int algo = a->algo & 0xff, hint = (a->algo >> 8) & 0xffff;
