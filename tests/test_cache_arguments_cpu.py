@@ -51,6 +51,19 @@ def test_a_copy_that_fails_leaves_the_cache_as_it_was(zt):
     assert cache.pages("b") == (1,) and cache.pages("c") == (2,) and cache.free_pages == 4
 
 
+@pytest.mark.parametrize("head_dim", [4, 68, 136, 256])
+def test_a_decoder_layer_takes_heads_that_its_attention_reads(zt, head_dim):
+    """The cache would be filled before the attention refused it."""
+    from zentorch_b200 import tp
+
+    class Lin:
+        world = 1
+    with pytest.raises(ValueError, match="multiple of 8 elements up to 128"):
+        tp.DecoderLayer(Lin(), 8, 2, head_dim, torch.ones(2))
+    assert tp.DecoderLayer(Lin(), 8, 2, head_dim, torch.ones(2), ops=object()).head_dim == head_dim      # another attention
+    assert tp.DecoderLayer(Lin(), 8, 2, 80, torch.ones(2)).head_dim == 80
+
+
 def test_a_softmax_scale_whose_base_two_form_is_infinite(zt):
     from zentorch_b200 import _capi
     lib, p = _capi.lib(), _capi.PagedAttentionArgs()

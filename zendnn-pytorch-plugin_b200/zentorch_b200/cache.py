@@ -102,7 +102,9 @@ class PagedKVCache:
     """Pages of keys and values for ``layers`` layers.
 
     ``dtype`` is that of the activations, or ``torch.float8_e4m3fn`` with ``k_scale`` / ``v_scale`` [layers, kv_heads] fp32 (ones
-    if not given): stored values are divided by them.  ``copy_pages(caches, src, dst)`` replaces the operator, for checks on a
+    if not given): stored values are divided by them.  ``zentorch_paged_attention`` reads bfloat16, float16 and float8_e4m3fn with
+    heads of a multiple of 8 elements (16 in 8 bits) up to 128; other caches (float32, wider heads) can be filled and copied, for
+    an attention of the caller's.  ``copy_pages(caches, src, dst)`` replaces the operator, for checks on a
     machine without a GPU.
     """
 

@@ -323,6 +323,8 @@ class DecoderLayer:
         world = linears.world
         if q_heads % kv_heads or kv_heads % world:
             raise ValueError(f"{q_heads} query and {kv_heads} key/value heads do not divide over groups and {world} ranks")
+        if ops is None and (head_dim % 8 or not 8 <= head_dim <= 128):
+            raise ValueError(f"the attention reads heads of a multiple of 8 elements up to 128, got {head_dim}")
         self.linears, self.q_heads, self.kv_heads, self.head_dim = linears, q_heads // world, kv_heads // world, head_dim
         self.inv_freq, self.attention_factor, self.interleaved = inv_freq, attention_factor, interleaved
         self.window, self.scale, self.ops = window, scale, ops
