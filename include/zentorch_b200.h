@@ -467,7 +467,8 @@ ZT_API int zt_cache_copy_pages(const zt_cache_copy_args_t *args, void *stream);
  * workspace    zt_paged_attention_workspace_bytes() bytes, 256-byte aligned, contents irrelevant; calls that can overlap need one each.
  *              0 for short contexts (block_table of few keys): then NULL will do
  * out          shares no memory with q or the caches
- * A score of minus infinity counts as a key that is not seen; NaN and infinities of other keys do not reach a row.
+ * NaN and infinities of keys that a row does not see do not reach it; an infinite value that it does see with a probability that rounds
+ * to zero may give NaN.  A score of minus infinity has probability zero, and a row of no others is zero.
  * Lengths that do not fit the tensors are cut, page ids outside the cache read as zeros; both set the device status word (106). */
 typedef struct {
   const void *q;

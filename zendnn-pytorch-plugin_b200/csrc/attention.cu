@@ -528,7 +528,10 @@ extern "C" int zt_paged_attention(const zt_paged_attention_args_t *a, void *stre
   p.page_shift = -1;
   for (int s = 0; s < 31; ++s)
     if (a->page_size == 1 << s) p.page_shift = s;
-  p.causal = a->causal != 0, p.window = a->window < 1 << 30 ? a->window : 1 << 30 /* no context is longer */, p.scale_log2 = a->scale * 1.4426950408889634f, p.zero_tail = a->zero_tail != 0, p.few = plan.few, p.slices = plan.slices;
+  p.causal = a->causal != 0, p.zero_tail = a->zero_tail != 0;
+  p.window = a->window < 1 << 30 ? a->window : 1 << 30;      // (no context is longer)
+  p.scale_log2 = a->scale * 1.4426950408889634f;
+  p.few = plan.few, p.slices = plan.slices;
   char *ws = reinterpret_cast<char *>(a->workspace);
   p.meta = reinterpret_cast<AttnMeta *>(ws);
   p.part_ml = reinterpret_cast<float2 *>(ws + plan.meta_bytes);

@@ -295,7 +295,7 @@ struct AttnWalk {
   bool started_;
 };
 
-// Row of the cache that holds a key: page id, slot in it.  An id outside the cache reads as no row and is reported.
+// Entry of a sequence's row of block_table that holds the page of a key.
 __device__ __forceinline__ int page_of(const AttnParams &p, int key) { return p.page_shift >= 0 ? key >> p.page_shift : key / p.page; }
 
 // Rows of `out` before the first sequence and behind the last one, by all threads of the grid.
